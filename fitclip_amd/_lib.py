@@ -44,6 +44,18 @@ class fc_prof_record(C.Structure):
                 ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("ms", C.c_float)]
 
 
+class fc_docs(C.Structure):
+    """`fc_docs` (operands and masks of the attention over packed documents); `struct_size` is filled in here."""
+    _fields_ = ([(n, C.c_int32) for n in ("struct_size", "kind", "docs", "q_heads", "kv_heads", "causal", "fill")]
+                + [(n, C.c_float) for n in ("scale", "cap")] + [(n, C.c_int64) for n in ("q_rows", "k_rows")]
+                + [(n, C.c_void_p) for n in ("q", "k", "v")]
+                + [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+                + [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "prefix", "slopes")])
+
+    def __init__(self, **kw):
+        super().__init__(struct_size=C.sizeof(type(self)), **kw)
+
+
 _vp, _i32, _i64, _sz, _f32, _f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float, C.c_double
 
 # name -> (restype, argtypes); mirrors include/fitclip_hip.h
@@ -68,6 +80,9 @@ SIGNATURES = {
     "fc_ranks": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "fc_ranks_of": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "fc_group_mean": (_i32, [_vp, _vp, _i32, _i32, _i32, _vp]),
+    "fc_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, C.POINTER(_i32), _i32, _i32, _i32, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "fc_attention_docs_scratch_bytes": (_sz, [C.POINTER(fc_docs)]),
+    "fc_attention_docs": (_i32, [C.POINTER(fc_docs), _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "fc_nce_loss": (_i32, [_vp, _i32, _vp, _vp, _vp]),
     "fc_kd_loss": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp]),
     "fc_kd_loss_rect": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp]),

@@ -16,10 +16,13 @@ CSRC = Path(__file__).resolve().parent / "csrc"
 REPO = CSRC.parent.parent
 LIB = CSRC / "libfitclip_hip.so"
 SOURCES = ["api.hip", "gemm.hip", "gemm_split3.hip", "gemm_split2.hip", "attention.hip", "attention_split.hip", "attention_split2.hip", "rowops.hip", "score.hip", "wgrad.hip", "attention_bwd.hip", "backward.hip",
-           "train.hip", "bpe.cpp"]
-HEADERS = [CSRC / "common.h", CSRC / "gemm_kernel.h", CSRC / "gemm_split3.h", CSRC / "gemm_split2.h", CSRC / "handle.h", CSRC / "unicode_ranges.inc",
+           "train.hip", "rotary.hip", "attention_docs.hip", "bpe.cpp"]
+HEADERS = [CSRC / "common.h", CSRC / "gemm_kernel.h", CSRC / "gemm_split3.h", CSRC / "gemm_split2.h", CSRC / "handle.h", CSRC / "attention_docs.h", CSRC / "unicode_ranges.inc",
            REPO / "include" / "fitclip_hip.h"]
 ARCH = "gfx950"
+# The packed fp32 instructions stay out of these sources (v_pk_mul_f32 and its like: hipcc -O3 forms them from scalar float code)
+_NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"rotary.hip": _NO_PACKED_F32, "attention_docs.hip": _NO_PACKED_F32, "attention_docs_bwd.hip": _NO_PACKED_F32}
 
 # Kernels the bench lines name (bench.py: `roofline.kernel`, the time split) must not touch scratch memory: a spilled register in
 # a kernel that lives at 256 VGPRs turns into scratch traffic inside the K loop.  Checked on the generated ISA after every
@@ -32,6 +35,7 @@ NO_SCRATCH_AUDIT = {
     "attention_split2.hip": ["attn_split2_kernel"],
     "attention.hip": ["attn_f32_blocks_kernel", "attn_f32_mfma_kernel", "attn_bf16_v2_kernel"],
     "rowops.hip": ["layernorm_kernel", "layernorm_pair_kernel"],
+    "attention_docs.hip": ["attention_docs_kernel"],
     "wgrad.hip": ["gemm_tn_kernel"],   # (the KD training step: 24 % of its kernel time)
 }
 
@@ -210,7 +214,7 @@ def build(force: bool = False, save_temps: bool = False, verbose: bool = True, l
         # an audited source is compiled with -save-temps and its ISA checked on EVERY build: an up-to-date object whose .s file is
         # missing or older than the source (built before the source joined an audit table) is recompiled, never linked unaudited
         if force or _stale(obj, [CSRC / src, *HEADERS]) or (audited and _stale(asm, [CSRC / src, *HEADERS])):
-            cmd = [hipcc, *flags, "-c", str(CSRC / src), "-o", str(obj)]
+            cmd = [hipcc, *flags, *SOURCE_FLAGS.get(src, []), "-c", str(CSRC / src), "-o", str(obj)]
             if save_temps or audited:
                 cmd += ["-save-temps=obj"]
             if verbose:

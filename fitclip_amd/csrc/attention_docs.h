@@ -1,0 +1,284 @@
+// Attention over packed documents: what the forward and the gradient kernels share.
+//
+//   score(i, j) = scale q_i . k_j;  capped: cap tanh(score / cap);  biased: - slope_h |p_i - j|
+//   out_i = sum_j softmax_j(score)(i, j) v_j over the keys j that row i sees
+//
+// Rows and keys of all documents lie one behind the other; document d owns rows q_off[d] .. q_off[d+1] and keys k_off[d] .. k_off[d+1].
+// Query i of a document of Lq rows and Lk keys stands at key p_i = i + Lk - Lq (the last query at the last key) and sees, if causal, the
+// keys up to p_i and the first prefix[d] ones.  Each of these masks leaves ONE interval [lo, hi) of packed keys per row: the kernels know
+// no other mask.  Query heads h G .. h G + G - 1 share key head h; their rows are laid side by side as "kernel rows" m = row G + (head in
+// the group), so a tile of 32 kernel rows reads a key once for all heads that share it and works the same for G = 1.
+//
+// Common to all kernels:
+//   * 32 x 32 MFMA tiles, head dim 64.  In the C layout lane (r = lane & 31, hh = lane >> 5) holds column r, rows 8 b + 4 hh + e.
+//   * LDS tiles keep rows of 64 values row-major; the 16-byte chunk c of row w is stored at chunk c ^ swizzle(w), which makes BOTH ways of
+//     reading a tile free of bank conflicts: rows as an operand (16 bytes per lane, 16 rows at a time) and columns as an operand
+//     (ds_read_b64_tr_b16 for bf16, 4-byte reads for fp32).  bf16: 8 chunks, swizzle = row bits 1, 2, 3 reversed (two rows share a
+//     256-byte bank line; bit 1 must move a 64-byte half for the transposing read).  fp32: 16 chunks, row bit 2 moves a 128-byte half.
+//   * tiles arrive by LDS-DMA, double-buffered: the swizzle is applied to each lane's source address.
+#pragma once
+#include "common.h"
+
+#include <climits>
+
+namespace fc {
+namespace docs {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff();
+
+// n / d for 0 <= n < 2^31 by one multiplication: mul = ceil(2^(32 + shift) / d) with 2^shift >= d
+struct FastDiv {
+  unsigned d, mul, shift;
+  FastDiv(unsigned div = 1) : d(div), mul(0), shift(0) {
+    while ((1u << shift) < div) ++shift;
+    mul = div == 1 ? 0 : (unsigned)((((uint64_t)1 << (31 + shift)) + div - 1) / div);
+  }
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, mul) >> (shift - 1)); }
+};
+
+struct Args {
+  const char *q, *k, *v;                                // strides in bytes
+  long q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t *q_off, *k_off, *prefix;
+  const float* slopes;
+  int docs, kv_heads, rows, q_rows, k_rows;             // rows = kernel rows = q_rows * group
+  FastDiv group;
+  int causal, fill;
+  float c;                                              // scale log2 e (no cap): score in log2 units = raw * c
+  float cap_in, cap_out;                                // scale / cap, cap log2 e: score = cap_out tanh(raw cap_in)
+  // forward
+  char* out;
+  long out_row, out_head;
+  float* stats;                                         // [q_rows][heads] (maximum in log2 units, sum of 2^(score - maximum))
+  float* part;                                          // split over keys: [splits][kv_heads][rows][64] and behind it [..][2]
+  int tiles, splits;
+  // gradients
+  const char* d_out;
+  long do_row, do_head;
+  char *dq, *dk, *dv;
+  long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  float* d_slopes;
+  float scale;
+};
+
+#ifdef __HIPCC__
+
+__device__ __forceinline__ float swap_max(float x) {  // maximum of lanes l and l ^ 32
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float swap_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));  // (lanes l and l + 32 hold the same row)
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
+
+// how many of the sorted off[0 .. n) are <= x, found by the whole wave: 64 probes a step
+__device__ __forceinline__ int wave_count_le(const int32_t* off, int n, int x, int lane) {
+  int lo = 0, hi = n;
+  while (hi > lo) {
+    const int step = (hi - lo + 63) >> 6, at = lo + lane * step + step - 1;
+    const bool le = at < hi && off[at] <= x;
+    const int c = __popcll(__ballot(le));
+    hi = min(hi, lo + c * step + step - 1);
+    lo += c * step;
+  }
+  return lo;
+}
+
+struct Row {
+  int lo, hi;   // the packed keys that the row sees
+  int pos;      // packed key at which the query stands
+  bool valid;   // a row of a document
+};
+
+// the 32 kernel rows m0 .. m0 + 31, row m0 + (lane & 31) in every lane.  Offsets that are no offsets (decreasing, outside the rows) give
+// wrong intervals but never one outside [0, k_rows).
+__device__ __forceinline__ Row find_row(const Args& a, int m0, int lane) {
+  const int m = m0 + (lane & 31);
+  const int t0 = a.group.div(min(m0, a.rows - 1)), t1 = a.group.div(min(m0 + 31, a.rows - 1));
+  const int token = a.group.div(min(m, a.rows - 1));
+  const int first = min(max(wave_count_le(a.q_off, a.docs + 1, t0, lane) - 1, 0), a.docs - 1);
+  int lo = first, hi = first;
+  if (a.docs > 1 && a.q_off[first + 1] <= t1) hi = min(max(wave_count_le(a.q_off, a.docs + 1, t1, lane) - 1, first), a.docs - 1);
+  for (int span = hi - lo; span > 0; span >>= 1) {  // (wave-uniform trip count; each lane narrows to its own document)
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.q_off[mid] <= token) lo = mid; else hi = mid - 1;
+    hi = max(hi, lo);
+  }
+  const int d = lo;
+  const int qs = min(max(a.q_off[d], 0), a.q_rows), qe = min(max(a.q_off[d + 1], qs), a.q_rows);
+  const int ks = min(max(a.k_off[d], 0), a.k_rows), ke = min(max(a.k_off[d + 1], ks), a.k_rows);
+  const int lk = ke - ks, p = token - qs + lk - (qe - qs);
+  int seen = lk;
+  if (a.causal) seen = min(lk, max(p + 1, a.prefix ? a.prefix[d] : 0));
+  Row r;
+  r.valid = m < a.rows && token >= qs && token < qe;
+  r.lo = r.valid ? ks : 0;
+  r.hi = r.valid ? ks + max(seen, 0) : 0;
+  r.pos = ks + p;
+  return r;
+}
+
+// tanh: exact to 1.2e-7 (fp32 scores) or to 3e-7 of 1 in three instructions less (bf16 scores, whose own rounding is 2^-9)
+template <bool EXACT>
+__device__ __forceinline__ float tanh_f32(float u) {
+  if constexpr (EXACT) {
+    const float au = fabsf(u), w = u * u;
+    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(au * (2.f * kLog2e)) + 1.f);
+    float p = -0.006178273353725672f;  // tanh(u) = u + u^3 P(u^2) for |u| <= 9 / 16: least squares on Chebyshev nodes, 7e-8
+    p = __builtin_fmaf(p, w, 0.021006036549806595f);
+    p = __builtin_fmaf(p, w, -0.05383696034550667f);
+    p = __builtin_fmaf(p, w, 0.13332445919513702f);
+    p = __builtin_fmaf(p, w, -0.3333331346511841f);
+    return au < 0.5625f ? __builtin_fmaf(u * w, p, u) : copysignf(big, u);
+  } else {
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * (2.f * kLog2e)) + 1.f);
+  }
+}
+
+// geometry of an LDS tile of rows of 64 values of T
+template <typename T> struct Tile;
+template <> struct Tile<bf16> {
+  static constexpr int kRow = 128, kPiece = 8;  // bytes of a row; rows of a 1 KiB LDS-DMA piece
+  static __device__ __forceinline__ int swizzle(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
+};
+template <> struct Tile<float> {
+  static constexpr int kRow = 256, kPiece = 4;
+  static __device__ __forceinline__ int swizzle(int row) { return ((row >> 2) & 1) << 3 | ((row >> 3) & 1) << 2 | (row & 3); }
+};
+
+__device__ __forceinline__ void lds_dma(const char* src, char* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// a 64-value row in the registers of two lanes (lane r and r + 32), in the order of the row-operand reads below: bf16: 4 x 8 values
+// (d = 16 s + 8 hh ..), fp32: 8 x 4 values (d = 8 c + 4 hh ..)
+template <typename T> struct RowFrag;
+template <> struct RowFrag<bf16> {
+  bf16x8 v[4];
+  __device__ __forceinline__ void load(const char* row, int hh) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) v[s] = *reinterpret_cast<const bf16x8*>(row + 32 * s + 16 * hh);
+  }
+};
+template <> struct RowFrag<float> {
+  f32x4 v[8];
+  __device__ __forceinline__ void load(const char* row, int hh) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const f32x4*>(row + 32 * c + 16 * hh);
+  }
+};
+
+// per-lane byte offsets of the row-operand reads: chunk (2 s + hh) of LDS row r
+template <typename T> struct RowOff;
+template <> struct RowOff<bf16> {
+  int o[4];
+  __device__ __forceinline__ void init(int r, int hh) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) o[s] = r * 128 + (((2 * s + hh) ^ Tile<bf16>::swizzle(r)) << 4);
+  }
+};
+template <> struct RowOff<float> {
+  int o[8];
+  __device__ __forceinline__ void init(int r, int hh) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] = r * 256 + (((2 * c + hh) ^ Tile<float>::swizzle(r)) << 4);
+  }
+};
+
+// acc[row of the LDS tile][column = the lane's fragment] += tile row . fragment, 32 rows starting at `tile`
+__device__ __forceinline__ f32x16 rows_dot(const char* tile, const RowOff<bf16>& off, const RowFrag<bf16>& f, f32x16 acc) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(tile + off.o[s]), f.v[s], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ f32x16 rows_dot(const char* tile, const RowOff<float>& off, const RowFrag<float>& f, f32x16 acc) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const f32x4 k = *reinterpret_cast<const f32x4*>(tile + off.o[c]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], f.v[c][e], acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+// per-lane byte offsets of the column-operand reads (32 columns 32 n .. 32 n + 31 of a tile; n = 0, 1)
+template <typename T> struct ColOff;
+template <> struct ColOff<bf16> {
+  int o[2];
+  // ds_read_b64_tr_b16: lane 4 w + p of a 16-lane group names columns 4 p .. 4 p + 3 of row w of the group's four; lane i gets column i
+  __device__ __forceinline__ void init(int lane) {
+    const int hh = lane >> 5, half = (lane >> 4) & 1, w = (lane >> 2) & 3, p = lane & 3, row = 4 * hh + w;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)  // (row bit 3 is the parity of the 8-row block: added by the reader)
+      o[n] = row * 128 + (((4 * n + 2 * half + (p >> 1)) ^ (((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1)) << 4) + (p & 1) * 8;
+  }
+};
+template <> struct ColOff<float> {
+  int o[2][4];
+  __device__ __forceinline__ void init(int lane) {
+    const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)  // row 4 hh + e of an 8-row block (its parity, swizzle bit 2, is added by the reader)
+        o[n][e] = (4 * hh + e) * 256 + (((8 * n + (r >> 2)) ^ (hh << 3 | e)) << 4) + (r & 3) * 4;
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ s16x4 read_tr(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+
+// weights: a 32 x 32 accumulator tile (rows = the 32 rows of the LDS tile) as the second operand of a product over those rows
+struct WeightsB { bf16x8 v[2]; };
+__device__ __forceinline__ void to_weights(const f32x16& p, WeightsB& w) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w.v[s][j] = static_cast<bf16>(p[8 * s + j]);  // blocks b = 2 s, 2 s + 1 of four rows each
+}
+
+// out[32 n + column][lane's column of p] += sum over the 32 LDS rows of tile[row][32 n + ..] p[row][..]
+__device__ __forceinline__ void cols_dot(const char* tile, const ColOff<bf16>& off, const f32x16& p, f32x16 (&out)[2]) {
+  WeightsB w;
+  to_weights(p, w);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      // rows 16 s + 4 hh .. and 16 s + 8 + 4 hh ..: the odd 8-row block has row bit 3 set, which moves chunk bit 0
+      const s16x4 a = read_tr(tile + off.o[n] + s * 2048), b = read_tr(tile + (off.o[n] ^ 16) + s * 2048 + 1024);
+      const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+      out[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, w.v[s], out[n], 0, 0, 0);
+    }
+  }
+}
+__device__ __forceinline__ void cols_dot(const char* tile, const ColOff<float>& off, const f32x16& p, f32x16 (&out)[2]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float f = *reinterpret_cast<const float*>(tile + (off.o[n][e] ^ ((b & 1) << 6)) + b * 2048);
+        out[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, p[4 * b + e], out[n], 0, 0, 0);
+      }
+    }
+  }
+}
+
+#endif  // __HIPCC__
+
+}  // namespace docs
+}  // namespace fc

@@ -2,7 +2,7 @@
 checks shapes / dtypes / device, allocates the output with torch, and makes ONE C-ABI call on the current stream."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -502,3 +502,149 @@ def wise_axpby(a: torch.Tensor, b: torch.Tensor, weight_for_2: float, out: Optio
             _lib.check(_lib.load().fc_wise(a.data_ptr(), b.data_ptr(), float(weight_for_2), out.data_ptr(), a.numel(),
                                            _lib.current_stream()), "fc_wise")
     return out
+
+
+def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dim: Optional[int] = 64) -> torch.Tensor:
+    """[rows, heads, dim] with contiguous heads; rows and heads at any stride (views of a fused projection)."""
+    if t.dim() != 3 or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must be [rows, heads, {'dim' if dim is None else dim}], got {tuple(t.shape)}")
+    if t.dtype != dtype or dtype not in _KIND:
+        raise TypeError(f"{name} must be {dtype if dtype in _KIND else 'float32 or bfloat16'}, got {t.dtype}")
+    if t.numel() and t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous")
+    return t
+
+
+def _strides(t: torch.Tensor) -> "tuple[int, int]":
+    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    _heads(t, name, like.dtype, like.shape[2])
+    if t.shape != like.shape:
+        raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    row, head = _strides(t)
+    rows, heads, dim = t.shape
+    apart = lambda a, b, n: a >= (n - 1) * b + dim  # noqa: E731  (heads inside a row, or rows inside a head: no two overlap)
+    if t.numel() and (heads > 1 and head < dim or rows > 1 and row < dim
+                      or rows > 1 and heads > 1 and not (apart(row, head, heads) or apart(head, row, rows))):
+        raise ValueError(f"the rows and heads of {name} overlap")
+    return t
+
+
+def _on_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise _lib.FitclipHipError(f"{name} must live on the ROCm device (got {t.device}); there is no CPU fallback")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, n: Optional[int] = None) -> None:
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 1 or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections: Optional[Sequence[int]] = None,
+           interleaved: bool = False, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions with one to three axes (time, height, width): pair i of the dimensions of every head of x [rows, heads,
+    dim] (float32 or bfloat16; rows and heads may be strided: `qkv[:, :2 * D].view(rows, -1, 64)` turns q and k of a fused
+    projection) turns by positions[row, axis(i)] * inv_freq[i].  positions int32 [rows, axes] (or [rows]); inv_freq float32
+    [pairs], 2 pairs <= dim, the dimensions behind them are copied; `sections`: how many pairs turn with each axis; pairs are
+    (i, i + pairs), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in 64 bits: exact at far positions.  `inverse` turns
+    back - the gradient.  `out` may be x (in place)."""
+    _heads(x, "x", x.dtype, None)
+    positions = positions[:, None] if positions.dim() == 1 else positions
+    rows, heads, dim = x.shape
+    if positions.dtype != torch.int32:
+        raise TypeError(f"positions must be {torch.int32}, got {positions.dtype}")
+    if positions.dim() != 2 or positions.shape[0] != rows or not 1 <= positions.shape[1] <= 3:
+        raise ValueError(f"positions must be [{rows}, axes] with 1 to 3 axes, got {tuple(positions.shape)}")
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
+    _vector(inv_freq, "inv_freq", torch.float32)
+    axes, pairs = positions.shape[1], inv_freq.numel()
+    sections = [pairs] if sections is None and axes == 1 else list(sections or ())
+    if len(sections) != axes or sum(sections) != pairs:
+        raise ValueError(f"{axes} sections that sum up to {pairs} pairs are needed, got {sections}")
+    if out is not None:
+        _written(out, "out", x)
+        if out.data_ptr() == x.data_ptr() and _strides(out) != _strides(x):
+            raise ValueError("in place needs the same strides")
+    _on_device(x.device, x=x, positions=positions, inv_freq=inv_freq, out=out)
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().fc_rotary(_KIND[x.dtype], x.data_ptr(), *_strides(x), positions.data_ptr(), axes, inv_freq.data_ptr(),
+                                         (_lib._i32 * axes)(*sections), pairs, int(interleaved), int(inverse), out.data_ptr(),
+                                         *_strides(out), rows, heads, dim, _lib.current_stream()), "fc_rotary")
+    return out
+
+
+def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill) -> "_lib.fc_docs":
+    _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
+    if k.shape != v.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the same shape")
+    if not k.shape[1] or q.shape[1] % k.shape[1] or not q.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads over {k.shape[1]} key heads: a multiple is needed")
+    _vector(q_offsets, "q_offsets", torch.int32)
+    if not q_offsets.numel():
+        raise ValueError("q_offsets must hold docs + 1 numbers")
+    if k_offsets is None:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError("k_offsets is needed where keys and queries differ in number")
+        k_offsets = q_offsets
+    docs = q_offsets.numel() - 1
+    _vector(k_offsets, "k_offsets", torch.int32, docs + 1)
+    _vector(prefix, "prefix", torch.int32, docs)
+    _vector(slopes, "slopes", torch.float32, q.shape[1])
+    if prefix is not None and not causal:
+        raise ValueError("a prefix mask needs causal=True")
+    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
+        raise ValueError(f"scale must be positive and cap 0 (none) or positive, got {scale} and {cap}")
+    _on_device(q.device, q=q, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, prefix=prefix, slopes=slopes)
+    (q_row, q_head), (k_row, k_head), (v_row, v_head) = _strides(q), _strides(k), _strides(v)
+    return _lib.fc_docs(kind=_KIND[q.dtype], docs=docs, q_heads=q.shape[1], kv_heads=k.shape[1], causal=int(causal), fill=int(fill),
+                        scale=scale, cap=float(cap), q_rows=q.shape[0], k_rows=k.shape[0], q=q.data_ptr(), k=k.data_ptr(),
+                        v=v.data_ptr(), q_row=q_row, q_head=q_head, k_row=k_row, k_head=k_head, v_row=v_row, v_head=v_head,
+                        q_offsets=q_offsets.data_ptr(), k_offsets=k_offsets.data_ptr(), prefix=_ptr(prefix), slopes=_ptr(slopes))
+
+
+def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None,
+                   causal: bool = False, prefix: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, cap: float = 0.0,
+                   scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> "tuple[torch.Tensor, torch.Tensor]":
+    """Attention over packed documents: q [q_rows, heads, 64], k and v [k_rows, kv_heads, 64] (float32 or bfloat16; rows and heads
+    may be strided; heads a multiple of kv_heads: consecutive query heads share a key head) -> (out [q_rows, heads, 64], stats
+    float32 [q_rows, heads, 2]).
+
+    Document d owns rows q_offsets[d] .. q_offsets[d + 1] and keys k_offsets[d] .. k_offsets[d + 1] (int32 [docs + 1] on the device,
+    not decreasing; k_offsets defaults to q_offsets).  Its last query stands at its last key.  `causal`: a query sees the keys up to
+    its own place, and the first prefix[d] ones (`prefix` int32 [docs]).  Scores are scale q.k (scale 1 / 8 by default), bent to
+    cap tanh(score / cap) if `cap` > 0, minus slopes[head] * distance if `slopes` (float32 [heads]) is given.  A row that sees no
+    key gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
+
+    Rows behind the last document are left as they were in a given `out` (which may not overlap k or v), and 0 otherwise."""
+    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill=out is None)
+    if out is None:
+        out = (torch.zeros if d.docs == 0 else torch.empty)(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _written(out, "out", q)
+        _on_device(q.device, out=out)
+    stats = torch.empty((*q.shape[:2], 2), dtype=torch.float32, device=q.device)
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        if d.docs == 0 or not d.fill:  # (rows of no document keep these)
+            stats[..., 0], stats[..., 1] = float("-inf"), 0.0
+        scratch = torch.empty(lib.fc_attention_docs_scratch_bytes(d), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.fc_attention_docs(d, out.data_ptr(), *_strides(out), stats.data_ptr(), scratch.data_ptr(), scratch.numel(),
+                                         _lib.current_stream()), "fc_attention_docs")
+    return out, stats

@@ -184,6 +184,48 @@ FC_API int fc_kd_loss(const float* scores, const float* teacher_scores, int32_t 
 FC_API int fc_kd_loss_rect(const float* scores, const float* teacher_scores, int32_t rows, int32_t cols, float* out,
                     float* ws, fc_stream stream);
 
+/* ---- video-token operators: rotary positions, attention over packed documents -----------------------------------
+ * For token streams that the towers' fixed sequences do not cover (all frames of a clip at once, captions packed without their
+ * padding, frames in front of captions, single tokens over what a sequence holds so far).  Head dimension 64; element kinds as in
+ * fc_gemm; every row and head starts on a 16-byte boundary; strides count ELEMENTS, the 64 (fc_rotary: dim) values of a head are
+ * contiguous.  The q | k | v columns of a fused projection are such operands as they lie.
+ *
+ * fc_rotary: pair i of a head's dimensions - (i, i + pairs), or (2 i, 2 i + 1) if `interleaved` - turns by
+ *   positions[row, axis(i)] * inv_freq[i]; `sections` (HOST, `axes` numbers that sum up to `pairs`) says how many consecutive pairs
+ *   belong to each axis; dimensions behind 2 pairs are copied.  `inverse` != 0 turns back: the gradient.  positions dev int32
+ *   [rows, axes], inv_freq dev f32 [pairs].  out may be x (with x's strides).  dim <= 256, pairs and dim multiples of 16 bytes. */
+FC_API int fc_rotary(int32_t kind, const void* x, int64_t x_row, int64_t x_head, const int32_t* positions, int32_t axes,
+              const float* inv_freq, const int32_t* sections, int32_t pairs, int32_t interleaved, int32_t inverse, void* out,
+              int64_t out_row, int64_t out_head, int64_t rows, int32_t heads, int32_t dim, fc_stream stream);
+
+/* Operands and masks of the attention over packed documents.  Document d owns query rows q_offsets[d] .. q_offsets[d + 1] and keys
+ * k_offsets[d] .. k_offsets[d + 1] (dev int32 [docs + 1], not decreasing, inside the rows; the same array where every token is both).
+ * Its query i stands at its key p = i + keys - queries.  score = scale q.k, then cap tanh(score / cap) if cap > 0, then
+ * - slopes[head] |p - j| if slopes (dev f32 [q_heads]) is given.  A query sees all keys of its document or, if causal, those up to p and
+ * the first prefix[d] ones (dev int32 [docs], may be null).  Query heads h g .. h g + g - 1, g = q_heads / kv_heads, share key head h. */
+typedef struct {
+  int32_t struct_size; /* sizeof(fc_docs) as the caller declared it: checked first */
+  int32_t kind;        /* fc_precision of q, k, v, out and the gradients */
+  int32_t docs, q_heads, kv_heads;
+  int32_t causal;
+  int32_t fill;        /* 1: rows of no document are set to 0 (stats: -inf, 0) in the outputs; 0: they are left as they were */
+  float scale, cap;    /* scale > 0; cap 0: none */
+  int64_t q_rows, k_rows;
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t *q_offsets, *k_offsets, *prefix;
+  const float* slopes;
+} fc_docs;
+#define FC_DOCS_INIT {(int32_t)sizeof(fc_docs)}
+/* out = softmax(scores) v per row and head (0 where a row sees nothing); stats dev f32 [q_rows, q_heads, 2] <- the row's largest
+ * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 where it sees nothing): what the gradients and a later
+ * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
+ * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
+ * infinities included.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
+FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
+FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
+                      size_t scratch_bytes, fc_stream stream);
+
 /* ---- WiSE (aligner/wise.py:16): out = (1 - weight_for_2) * a + weight_for_2 * b over n floats ------------------ */
 FC_API int fc_wise(const float* a, const float* b, double weight_for_2, float* out, size_t n, fc_stream stream);
 
