@@ -83,6 +83,8 @@ SIGNATURES = {
     "fc_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i32, _vp, C.POINTER(_i32), _i32, _i32, _i32, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
     "fc_attention_docs_scratch_bytes": (_sz, [C.POINTER(fc_docs)]),
     "fc_attention_docs": (_i32, [C.POINTER(fc_docs), _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "fc_attention_docs_backward_scratch_bytes": (_sz, [C.POINTER(fc_docs)]),
+    "fc_attention_docs_backward": (_i32, [C.POINTER(fc_docs), _vp, _i64, _i64, _vp] + [_vp, _i64, _i64] * 4 + [_vp, _vp, _sz, _vp]),
     "fc_nce_loss": (_i32, [_vp, _i32, _vp, _vp, _vp]),
     "fc_kd_loss": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp]),
     "fc_kd_loss_rect": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp]),

@@ -16,7 +16,7 @@ CSRC = Path(__file__).resolve().parent / "csrc"
 REPO = CSRC.parent.parent
 LIB = CSRC / "libfitclip_hip.so"
 SOURCES = ["api.hip", "gemm.hip", "gemm_split3.hip", "gemm_split2.hip", "attention.hip", "attention_split.hip", "attention_split2.hip", "rowops.hip", "score.hip", "wgrad.hip", "attention_bwd.hip", "backward.hip",
-           "train.hip", "rotary.hip", "attention_docs.hip", "bpe.cpp"]
+           "train.hip", "rotary.hip", "attention_docs.hip", "attention_docs_bwd.hip", "bpe.cpp"]
 HEADERS = [CSRC / "common.h", CSRC / "gemm_kernel.h", CSRC / "gemm_split3.h", CSRC / "gemm_split2.h", CSRC / "handle.h", CSRC / "attention_docs.h", CSRC / "unicode_ranges.inc",
            REPO / "include" / "fitclip_hip.h"]
 ARCH = "gfx950"
@@ -36,6 +36,7 @@ NO_SCRATCH_AUDIT = {
     "attention.hip": ["attn_f32_blocks_kernel", "attn_f32_mfma_kernel", "attn_bf16_v2_kernel"],
     "rowops.hip": ["layernorm_kernel", "layernorm_pair_kernel"],
     "attention_docs.hip": ["attention_docs_kernel"],
+    "attention_docs_bwd.hip": ["docs_grad_rows_kernel", "docs_grad_keys_kernel"],
     "wgrad.hip": ["gemm_tn_kernel"],   # (the KD training step: 24 % of its kernel time)
 }
 

@@ -61,6 +61,8 @@ struct Args {
   long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
   float* d_slopes;
   float scale;
+  float* table;                                         // see attention_docs_bwd.hip
+  int rows_pad;
 };
 
 #ifdef __HIPCC__
@@ -278,7 +280,77 @@ __device__ __forceinline__ void cols_dot(const char* tile, const ColOff<float>& 
   }
 }
 
+// cols_dot value by value, for the (row, column) pairs that `sees(row)` says only: p = 0 does not keep an infinite or NaN value of a
+// masked row out of a matrix product
+template <typename T, typename Sees>
+__device__ __forceinline__ void cols_dot_careful(const char* tile, const f32x16& p, int lane, f32x16 (&out)[2], Sees sees) {
+  const int r = lane & 31, hh = lane >> 5;
+#pragma unroll 1
+  for (int w = 0; w < 32; ++w) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((w & ~4) == 8 * (i >> 2) + (i & 3)) x = p[i];
+    x = __shfl(x, r + ((w >> 2) & 1) * 32, 64);
+    const bool see = sees(w);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int byte = (32 * n + 8 * b + 4 * hh) * (int)sizeof(T);
+        typedef T vec __attribute__((ext_vector_type(4)));
+        const vec f = *reinterpret_cast<const vec*>(tile + w * Tile<T>::kRow + (((byte >> 4) ^ Tile<T>::swizzle(w)) << 4) + (byte & 15));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (see) out[n][4 * b + e] = __builtin_fmaf(x, static_cast<float>(f[e]), out[n][4 * b + e]);
+        asm volatile("" ::: "memory");  // (one load at a time: this path is rare, its registers are everybody's)
+      }
+  }
+}
+
+// NaN if a value is not finite, else 0
+__device__ __forceinline__ float not_finite(const f32x16 (&o)[2]) {
+  float x = 0.f;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x = __builtin_fmaf(o[n][i], 0.f, x);
+  return x;
+}
+
+// o[n][..] = value (32 n + 8 b + 4 hh + e) of the lane's row, times `by` -> 32 rows of 64 values, through the wave's patch of LDS (32 rows)
+// and from there 16 bytes per lane; `at(w)` is row w's address, rows without their bit in `good` are left alone
+template <typename T, typename At>
+__device__ __forceinline__ void store_rows(char* patch, const f32x16 (&o)[2], float by, int lane, unsigned long long good, At at) {
+  const int r = lane & 31, hh = lane >> 5;
+  constexpr int ROWB = Tile<T>::kRow, CH = ROWB / 16;  // 16-byte chunks of a row
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 y = {o[n][4 * b] * by, o[n][4 * b + 1] * by, o[n][4 * b + 2] * by, o[n][4 * b + 3] * by};
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4*>(patch + r * 256 + (((8 * n + 2 * b + hh) ^ (r & 15)) << 4)) = y;
+      } else {
+        bf16x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(y[e]);
+        *reinterpret_cast<bf16x4*>(patch + r * 128 + (((4 * n + b) ^ ((r >> 1) & 7)) << 4) + hh * 8) = w;
+      }
+    }
+#pragma unroll
+  for (int it = 0; it < 32 * CH / 64; ++it) {
+    const int w = it * (64 / CH) + lane / CH, ch = lane % CH;
+    const f32x4 y = *reinterpret_cast<const f32x4*>(patch + w * ROWB + ((ch ^ (sizeof(T) == 4 ? w & 15 : (w >> 1) & 7)) << 4));
+    if (good >> w & 1) *reinterpret_cast<f32x4*>(at(w) + ch * 16) = y;
+  }
+}
+
 #endif  // __HIPCC__
+
+int check_docs(const fc_docs* d, const char* what);
+bool rows_aligned(const void* p, int64_t row, int64_t head, int kind);
+Args make_args(const fc_docs& d);
 
 }  // namespace docs
 }  // namespace fc

@@ -160,37 +160,16 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
           l += s[u][i];
         }
       if (careful && !full) {
-#pragma unroll 1
-        for (int w = 0; w < TK; ++w) {
-          float p = 0.f;
 #pragma unroll
-          for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (w == 32 * u + 8 * (i >> 2) + (i & 3) || w == 32 * u + 8 * (i >> 2) + (i & 3) + 4) p = s[u][i];
-          p = __shfl(p, r + ((w >> 2) & 1) * 32, 64);
-          const bool visible = (unsigned)(k0 + w - row.lo) < len;
-          const char* vrow = vt + w * ROWB;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int d = 32 * n + 8 * (i >> 2) + 4 * hh + (i & 3), byte = d * (int)sizeof(T);
-              const float v = static_cast<float>(*reinterpret_cast<const T*>(vrow + (((byte >> 4) ^ Tile<T>::swizzle(w)) << 4) + (byte & 15)));
-              if (visible) o[n][i] = __builtin_fmaf(p, v, o[n][i]);
-            }
-        }
+        for (int u = 0; u < NT; ++u)
+          cols_dot_careful<T>(vt + u * 32 * ROWB, s[u], lane, o, [&](int w) { return rel - 4 * hh + 32 * u + w < len; });
       } else {
 #pragma unroll
         for (int u = 0; u < NT; ++u) cols_dot(vt + u * 32 * ROWB, voff, s[u], o);
       }
     }
     if (careful) break;
-    float probe = 0.f;  // NaN if any value of O is not finite
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) probe = __builtin_fmaf(o[n][i], 0.f, probe);
+    const float probe = not_finite(o);
     if (!__syncthreads_or(row.valid && probe != probe)) break;
     careful = true;
   }
@@ -217,34 +196,11 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
   const float inv = sees ? down / l : 0.f;
   if (hh == 0 && m0 + r < a.rows && (row.valid || a.fill))
     *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
-  // O^T -> rows of 64 values: through the wave's patch of LDS, then 16 bytes per lane
-  __syncthreads();
-  char* patch = smem + wave * 32 * ROWB;
-#pragma unroll
-  for (int n = 0; n < 2; ++n)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const f32x4 y = {o[n][4 * b] * inv, o[n][4 * b + 1] * inv, o[n][4 * b + 2] * inv, o[n][4 * b + 3] * inv};
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<f32x4*>(patch + r * 256 + (((8 * n + 2 * b + hh) ^ (r & 15)) << 4)) = y;
-      } else {
-        bf16x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(y[e]);
-        *reinterpret_cast<bf16x4*>(patch + r * 128 + (((4 * n + b) ^ ((r >> 1) & 7)) << 4) + hh * 8) = w;
-      }
-    }
-  constexpr int CH = ROWB / 16;  // 16-byte chunks of a row
-  const unsigned long long good = __ballot(row.valid || (a.fill && m0 + r < a.rows));
-#pragma unroll
-  for (int it = 0; it < 32 * CH / 64; ++it) {
-    const int w = it * (64 / CH) + lane / CH, ch = lane % CH;
-    const f32x4 y = *reinterpret_cast<const f32x4*>(patch + w * ROWB + ((ch ^ (sizeof(T) == 4 ? w & 15 : (w >> 1) & 7)) << 4));
-    if (good >> w & 1) {
-      const int mm = m0 + w, tk = a.group.div(mm), h = head * (int)a.group.d + (mm - tk * (int)a.group.d);
-      *reinterpret_cast<f32x4*>(a.out + tk * a.out_row + h * a.out_head + ch * 16) = y;
-    }
-  }
+  __syncthreads();  // (the patches reuse the stages)
+  store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(row.valid || (a.fill && m0 + r < a.rows)), [&](int w) {
+    const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+    return a.out + tk * a.out_row + h * a.out_head;
+  });
 }
 
 // joins the parts of a key range: 16 lanes per kernel row, parts in order
@@ -356,8 +312,8 @@ int check_docs(const fc_docs* d, const char* what) {
   if (!(d->scale > 0.f) || !(d->scale < kInf)) return fail(FC_EINVAL, "%s: scale %g: a positive number is needed", what, d->scale);
   if (!(d->cap >= 0.f) || !(d->cap < kInf)) return fail(FC_EINVAL, "%s: cap %g: 0 (none) or a positive number is needed", what, d->cap);
   if (d->prefix && !d->causal) return fail(FC_EINVAL, "%s: a prefix mask needs causal = 1", what);
-  if (d->docs == 0 || d->q_rows == 0) return FC_OK;
-  if (!d->q || !d->q_offsets || !d->k_offsets || (d->k_rows && (!d->k || !d->v))) return fail(FC_EINVAL, "%s: null operand", what);
+  if (d->docs == 0 || (d->q_rows == 0 && d->k_rows == 0)) return FC_OK;
+  if ((d->q_rows && !d->q) || !d->q_offsets || !d->k_offsets || (d->k_rows && (!d->k || !d->v))) return fail(FC_EINVAL, "%s: null operand", what);
   const int size = d->kind == PREC_F32 ? 4 : 2;
   if ((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) ||
       ((d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head) * size & 15))

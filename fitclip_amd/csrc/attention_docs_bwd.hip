@@ -1,0 +1,495 @@
+// Gradients of the attention over packed documents (attention_docs.h: the formulas, the masks, the tiles).
+//
+//   P = 2^(score - maximum) / sum (score in units of ln 2; both from the forward's stats)
+//   D_i = sum_d dO_id O_id,   dP = dO V^T,   dS = P (dP - D)      (0 exactly where a row sees one key)
+//   dV = P^T dO,   dQ = scale dS' K,   dK = scale dS'^T Q         dS' = dS (1 - tanh^2) behind a cap
+//   d slope_h = - sum dS |p_i - j| = - (sum_j P dP |p - j| - (sum_j P dP) (sum_j P |p - j|)) per row: every factor in fp32 (the D of a
+//   bf16 output is rounded)
+//
+// Two kernels, no atomics: every sum has one owner and a fixed order.
+//   rows: as the forward (a wave owns 32 kernel rows and walks over keys): dQ, and the row table that the other kernel reads.
+//   keys: a wave owns 32 keys (K and V in registers) and walks over the kernel rows that see them - all heads of the group, so the gradients
+//   of shared heads need no further sum: S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
+//   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
+// The products that weigh a masked row or key with 0 are guarded against NaN and infinities there as in the forward.
+#include "attention_docs.h"
+
+#include <algorithm>
+
+namespace fc {
+namespace docs {
+namespace {
+
+// Row table in scratch, one array of rows_pad numbers per quantity and key head: what a kernel row needs to have its weights formed again
+enum Column : int { COL_MAX = 0, COL_D = 1, COL_LO = 2, COL_HI = 3, COL_INV = 4, COL_POS = 5, COL_SLOPE = 6, COL_DSLOPE = 7, COLS = 8 };
+// (maximum; bf16: maximum + log2 sum, and no COL_INV; fp32: 1 / sum apart, so that the forward's P is formed exactly again)
+// and behind the columns four ints per 32 kernel rows and key head: lowest and highest key that one of them sees; the keys from .. to that ALL see
+__device__ __forceinline__ float* column(const Args& a, int c, int head) { return a.table + ((long)c * a.kv_heads + head) * a.rows_pad; }
+__device__ __forceinline__ int32_t* block_keys(const Args& a, int head, int block) {
+  return reinterpret_cast<int32_t*>(a.table + (long)COLS * a.kv_heads * a.rows_pad) + ((long)head * (a.rows_pad / 32) + block) * 4;
+}
+
+__device__ __forceinline__ float dot(const RowFrag<bf16>& x, const RowFrag<bf16>& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(static_cast<float>(x.v[c][e]), static_cast<float>(y.v[c][e]), s);
+  return s;
+}
+__device__ __forceinline__ float dot(const RowFrag<float>& x, const RowFrag<float>& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = __builtin_fmaf(x.v[c][e], y.v[c][e], s);
+  return s;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ rows
+template <typename T, int NW, int TK, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NW * 64) docs_grad_rows_kernel(const Args a) {
+  constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
+  constexpr int STAGE = 2 * TK * ROWB, NP = 2 * TK / PIECE, NT = TK / 32;
+  static_assert(NP % NW == 0 && NW * 32 * ROWB <= 2 * STAGE, "pieces of a wave; patches");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int range[2 * NW];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads;
+  const int m0 = (tile * NW + wave) * 32;
+
+  const Row row = find_row(a, m0, lane);
+  const bool sees = row.lo < row.hi;
+  const int wlo = wave_min_i(sees ? row.lo : INT_MAX), whi = wave_max_i(sees ? row.hi : -INT_MAX);
+  const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);
+  const int full_hi = wave_min_i(row.valid ? (sees ? row.hi : -INT_MAX) : INT_MAX);
+  int kbeg = wlo, kend = whi;
+  if constexpr (NW > 1) {
+    if (lane == 0) {
+      range[wave] = wlo;
+      range[NW + wave] = whi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      kbeg = min(kbeg, range[w]);
+      kend = max(kend, range[NW + w]);
+    }
+    kbeg = __builtin_amdgcn_readfirstlane(kbeg);
+    kend = __builtin_amdgcn_readfirstlane(kend);
+  }
+  const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
+
+  const int m = min(m0 + r, a.rows - 1);
+  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+  RowFrag<T> qf, dof;
+  qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
+  dof.load(a.d_out + token * a.do_row + qh * a.do_head, hh);
+  float D;
+  {
+    RowFrag<T> of;
+    of.load(a.out + token * a.out_row + qh * a.out_head, hh);
+    D = swap_sum(dot(of, dof));
+  }
+  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2);
+  // a row that sees nothing weighs nothing: its maximum is taken as +inf
+  float top = sees ? st[0] : kInf, inv = sees ? 1.f / st[1] : 0.f;
+  if constexpr (sizeof(T) == 2) {
+    if (sees) top += __builtin_amdgcn_logf(st[1]);
+    inv = 1.f;
+  }
+  if (!sees) D = 0.f;
+  const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
+  if (hh == 0 && m0 + r < a.rows_pad) {
+    const int at = m0 + r;
+    column(a, COL_MAX, head)[at] = top;
+    column(a, COL_D, head)[at] = D;
+    column(a, COL_LO, head)[at] = __int_as_float(row.lo);
+    column(a, COL_HI, head)[at] = __int_as_float(row.hi);
+    if constexpr (sizeof(T) == 4) column(a, COL_INV, head)[at] = inv;
+    if constexpr (BIAS) {
+      column(a, COL_POS, head)[at] = __int_as_float(row.pos);
+      column(a, COL_SLOPE, head)[at] = slope;
+    }
+  }
+  const int all_lo = wave_max_i(sees ? row.lo : INT_MAX), all_hi = wave_min_i(sees ? row.hi : -INT_MAX);
+  if (lane == 0) {
+    int32_t* b = block_keys(a, head, m0 / 32);
+    b[0] = wlo;
+    b[1] = whi;
+    b[2] = all_lo;  // (here a row of no document asks for the mask too: its Q and dO may hold anything)
+    b[3] = all_hi;
+  }
+
+  const char* kbase = a.k + head * a.k_head;
+  const char* vbase = a.v + head * a.v_head;
+  auto stage = [&](int t) {
+    char* dst = smem + (t & 1) * STAGE;
+    const int in = lane / (64 / PIECE), pc = lane % (64 / PIECE);
+#pragma unroll
+    for (int j = 0; j < NP / NW; ++j) {
+      const int piece = wave + j * NW, isv = piece >= NP / 2;
+      const int w = (isv ? piece - NP / 2 : piece) * PIECE + in;
+      const long key = min(kbeg + t * TK + w, kend - 1);
+      lds_dma((isv ? vbase + key * a.v_row : kbase + key * a.k_row) + ((pc ^ Tile<T>::swizzle(w)) << 4), dst + piece * 1024);
+    }
+  };
+  RowOff<T> roff;
+  roff.init(r, hh);
+  ColOff<T> coff;
+  coff.init(lane);
+
+  f32x16 o[2];
+  float pd, pf, pdf;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
+  bool careful = false;
+  while (true) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+    pd = pf = pdf = 0.f;
+    if (ntile) stage(0);
+    for (int t = 0; t < ntile; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (t + 1 < ntile) stage(t + 1);
+      const int k0 = kbeg + t * TK;
+      const char* kt = smem + (t & 1) * STAGE;
+      const char* vt = kt + TK * ROWB;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int ku = k0 + 32 * u;
+        if (ku >= whi || ku + 32 <= wlo) continue;  // (wave-uniform)
+        const bool full = full_lo <= ku && ku + 32 <= full_hi;
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+        s = rows_dot(kt + u * 32 * ROWB, roff, qf, s);
+        dp = rows_dot(vt + u * 32 * ROWB, roff, dof, dp);
+        const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
+        const unsigned rel = (unsigned)(ku + 4 * hh - row.lo), len = (unsigned)(row.hi - row.lo);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int w = 8 * (i >> 2) + (i & 3);
+          float bent = 0.f, x;
+          if constexpr (CAP) {
+            bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
+            x = a.cap_out * bent;
+          } else {
+            x = s[i] * a.c;
+          }
+          const float far = BIAS ? fabsf(at - (float)w) : 0.f;
+          if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
+          float p = __builtin_amdgcn_exp2f(x - top);
+          if constexpr (sizeof(T) == 4) p *= inv;
+          float g = dp[i];
+          if (!full) {
+            const bool see = rel + w < len;
+            p = see ? p : 0.f;
+            g = see ? (len == 1 ? D : g) : 0.f;  // one key: P = 1 whatever its score
+          }
+          if constexpr (BIAS) {
+            const float y = p * g;
+            pd += y;
+            pf = __builtin_fmaf(p, far, pf);
+            pdf = __builtin_fmaf(y, far, pdf);
+          }
+          float ds = p * (g - D);
+          if constexpr (CAP) ds *= 1.f - bent * bent;
+          if (!full) ds = rel + w < len ? ds : 0.f;
+          s[i] = ds;
+        }
+        if (careful && !full)
+          cols_dot_careful<T>(kt + u * 32 * ROWB, s, lane, o, [&](int w) { return rel - 4 * hh + w < len; });
+        else
+          cols_dot(kt + u * 32 * ROWB, coff, s, o);
+      }
+    }
+    if (careful) break;
+    const float probe = not_finite(o);
+    if (!__syncthreads_or(row.valid && probe != probe)) break;
+    careful = true;
+  }
+  if constexpr (BIAS) {
+    pd = swap_sum(pd);
+    pf = swap_sum(pf);
+    pdf = swap_sum(pdf);
+    if (hh == 0 && m0 + r < a.rows_pad) column(a, COL_DSLOPE, head)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
+  }
+  __syncthreads();
+  store_rows<T>(smem + wave * 32 * ROWB, o, a.scale, lane, __ballot(row.valid || (a.fill && m0 + r < a.rows)), [&](int w) {
+    const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+    return a.dq + tk * a.dq_row + h * a.dq_head;
+  });
+}
+
+// ------------------------------------------------------------------------------------------------------------------ keys
+template <typename T, int NW, int TQ, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(NW * 64) docs_grad_keys_kernel(const Args a) {
+  constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
+  constexpr int OFF_DO = TQ * ROWB, OFF_TAB = 2 * TQ * ROWB;
+  constexpr bool kInv = sizeof(T) == 4;
+  constexpr int NTAB = BIAS ? 7 : kInv ? 5 : 4;           // columns of the row table that come along (in the order of Column)
+  constexpr int COLB = 256;                               // a column's share of a stage: 64 numbers, of which TQ count
+  constexpr int STAGE = OFF_TAB + 7 * COLB;
+  constexpr int NROW = 2 * TQ / PIECE, NP = NROW + NTAB;  // pieces: 1 KiB of Q, then of dO; 64 numbers of a column
+  static_assert(NW * 32 * ROWB <= 2 * STAGE, "patches");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;  // (earlier keys first: causal, they cost most)
+  const int k0 = tile * NW * 32, kw = k0 + wave * 32;
+
+  // kernel rows of the documents that own keys k0 .. k0 + 32 NW - 1; causal: in the first of them from the first row that sees k0
+  int r_lo, r_hi;
+  {
+    const int last = min(k0 + NW * 32, a.k_rows) - 1;
+    const int d0 = min(max(wave_count_le(a.k_off, a.docs + 1, k0, lane) - 1, 0), a.docs - 1);
+    const int d1 = min(max(wave_count_le(a.k_off, a.docs + 1, last, lane) - 1, d0), a.docs - 1);
+    const int qs = min(max(a.q_off[d0], 0), a.q_rows), qe = min(max(a.q_off[d0 + 1], qs), a.q_rows);
+    int skip = 0;
+    if (a.causal) {
+      const int ks = min(max(a.k_off[d0], 0), a.k_rows), ke = min(max(a.k_off[d0 + 1], ks), a.k_rows);
+      const int j = k0 - ks;
+      if (!(a.prefix && a.prefix[d0] > j)) skip = min(max(j - (ke - ks) + (qe - qs), 0), qe - qs);
+    }
+    r_lo = (qs + skip) * (int)a.group.d;
+    r_hi = min(max(a.q_off[d1 + 1], 0), a.q_rows) * (int)a.group.d;
+  }
+  const int t_first = r_lo / TQ, t_last = r_hi > r_lo ? (r_hi + TQ - 1) / TQ : t_first;
+
+  const int key = kw + r;
+  const long kc = min(key, a.k_rows - 1);
+  RowFrag<T> kf, vf;
+  kf.load(a.k + kc * a.k_row + head * a.k_head, hh);
+  vf.load(a.v + kc * a.v_row + head * a.v_head, hh);
+
+  auto stage = [&](int t) {
+    char* dst = smem + (t & 1) * STAGE;
+    const int in = lane / (64 / PIECE), pc = lane % (64 / PIECE);
+#pragma unroll
+    for (int j = 0; j < (NP + NW - 1) / NW; ++j) {
+      const int piece = wave + j * NW;
+      if (piece < NROW) {
+        const int isd = piece >= NROW / 2, w = (isd ? piece - NROW / 2 : piece) * PIECE + in;
+        const int m = min(t * TQ + w, a.rows - 1);
+        const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+        lds_dma((isd ? a.d_out + token * a.do_row + qh * a.do_head : a.q + token * a.q_row + qh * a.q_head) +
+                    ((pc ^ Tile<T>::swizzle(w)) << 4), dst + piece * 1024);
+      } else if (piece < NP) {
+        const int c = piece - NROW;
+        if (c != COL_INV || kInv)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(column(a, c, head) + (long)t * TQ + lane),
+                                           (__attribute__((address_space(3))) void*)(dst + OFF_TAB + c * COLB), 4, 0, 0);
+      }
+    }
+  };
+  RowOff<T> roff;
+  roff.init(r, hh);
+  ColOff<T> coff;
+  coff.init(lane);
+
+  f32x16 dk[2], dv[2];
+  bool careful = false;
+  while (true) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
+    if (t_first < t_last) stage(t_first);
+    for (int t = t_first; t < t_last; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (t + 1 < t_last) stage(t + 1);
+      const char* st = smem + (t & 1) * STAGE;
+#pragma unroll
+      for (int u = 0; u < TQ / 32; ++u) {
+        const int block = t * (TQ / 32) + u;
+        if (block * 32 >= a.rows) continue;
+        const int32_t* bk = block_keys(a, head, block);
+        if (kw >= bk[1] || kw + 32 <= bk[0]) continue;  // (wave-uniform)
+        const bool full = bk[2] <= kw && kw + 32 <= bk[3];
+        const char* qt = st + u * 32 * ROWB;
+        const char* dt = qt + OFF_DO;
+        const char* tab = st + OFF_TAB + u * 128;
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+        s = rows_dot(qt, roff, kf, s);
+        dp = rows_dot(dt, roff, vf, dp);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const char* at = tab + (8 * b + 4 * hh) * 4;
+          const f32x4 top = *reinterpret_cast<const f32x4*>(at + COL_MAX * COLB), D = *reinterpret_cast<const f32x4*>(at + COL_D * COLB);
+          f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, slope = {}, lo = {}, hi = {};
+          if constexpr (kInv) inv = *reinterpret_cast<const f32x4*>(at + COL_INV * COLB);
+          if constexpr (BIAS) {
+            pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
+            slope = *reinterpret_cast<const f32x4*>(at + COL_SLOPE * COLB);
+          }
+          if (!full) {
+            lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB);
+            hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 4 * b + e;
+            float bent = 0.f, x;
+            if constexpr (CAP) {
+              bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
+              x = a.cap_out * bent;
+            } else {
+              x = s[i] * a.c;
+            }
+            if constexpr (BIAS) x = __builtin_fmaf(-slope[e], fabsf((float)(__float_as_int(pos[e]) - key)), x);
+            float p = __builtin_amdgcn_exp2f(x - top[e]);
+            if constexpr (kInv) p *= inv[e];
+            float ds = p * (dp[i] - D[e]);
+            if constexpr (CAP) ds *= 1.f - bent * bent;
+            if (!full) {
+              const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
+              p = rel < len ? p : 0.f;
+              ds = rel < len && len > 1 ? ds : 0.f;
+            }
+            s[i] = p;
+            dp[i] = ds;
+          }
+        }
+        if (careful && !full) {
+          const auto sees = [&](int w) {
+            const int lo = *reinterpret_cast<const int*>(tab + COL_LO * COLB + w * 4), hi = *reinterpret_cast<const int*>(tab + COL_HI * COLB + w * 4);
+            return (unsigned)(key - lo) < (unsigned)(hi - lo);
+          };
+          cols_dot_careful<T>(dt, s, lane, dv, sees);
+          cols_dot_careful<T>(qt, dp, lane, dk, sees);
+        } else {
+          cols_dot(dt, coff, s, dv);
+          cols_dot(qt, coff, dp, dk);
+        }
+      }
+    }
+    if (careful) break;
+    const float probe = not_finite(dk) + not_finite(dv);
+    if (!__syncthreads_or(key < a.k_rows && probe != probe)) break;
+    careful = true;
+  }
+  __syncthreads();
+  const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
+  const unsigned long long good = __ballot(key < a.k_rows && (owned || a.fill));
+  char* patch = smem + wave * 32 * ROWB;
+  store_rows<T>(patch, dk, a.scale, lane, good, [&](int w) { return a.dk + (long)(kw + w) * a.dk_row + head * a.dk_head; });
+  store_rows<T>(patch, dv, 1.f, lane, good, [&](int w) { return a.dv + (long)(kw + w) * a.dv_row + head * a.dv_head; });
+}
+
+// d_slopes[h] = sum over the rows of head h, in an order that depends on the number of rows alone
+__global__ void __launch_bounds__(256) docs_grad_slopes_kernel(const Args a) {
+  const int head = blockIdx.x / (int)a.group.d, g = blockIdx.x - head * (int)a.group.d;
+  const float* v = column(a, COL_DSLOPE, head);
+  double s = 0.0;
+  for (int t = threadIdx.x; t < a.q_rows; t += 256) s += (double)v[(long)t * (int)a.group.d + g];
+  __shared__ double part[256];
+  part[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) a.d_slopes[blockIdx.x] = (float)part[0];
+}
+
+int pad_rows(const fc_docs& d) { return (int)((d.q_rows * (d.q_heads / d.kv_heads) + 127) / 128 * 128) + 64; }  // (a column is read 64 numbers at a time)
+
+size_t grad_bytes(const fc_docs& d) {
+  const size_t n = (size_t)pad_rows(d) * d.kv_heads;
+  return n * COLS * 4 + n / 32 * 16;
+}
+
+template <typename K>
+int launch_docs(K kern, long blocks, int waves, int lds, const Args& a, const char* what, hipStream_t st) {
+  if (blocks <= 0) return FC_OK;
+  if (blocks > 0x7fffffffL) return fail(FC_EINVAL, "%s: grid of %ld workgroups", what, blocks);
+  if (lds > 60 * 1024 && raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds) != hipSuccess)
+    return fail(FC_ELAUNCH, "%s: cannot raise dynamic LDS", what);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(waves * 64), lds, st, a);
+  FC_CHECK_LAUNCH(what);
+  return FC_OK;
+}
+
+template <typename T, bool CAP, bool BIAS>
+int launch_grads(Args a, hipStream_t st) {
+  const long cus = device_cus();
+  int rc;
+  // four waves share a tile where that still gives every compute unit a workgroup, as in the forward
+  a.tiles = (a.rows + 127) / 128;
+  if ((long)a.tiles * a.kv_heads >= cus) {
+    rc = launch_docs(docs_grad_rows_kernel<T, 4, 64, CAP, BIAS>, (long)a.tiles * a.kv_heads, 4, 4 * 64 * Tile<T>::kRow, a, "fc_attention_docs_backward (rows)", st);
+  } else {
+    a.tiles = (a.rows + 31) / 32;
+    rc = launch_docs(docs_grad_rows_kernel<T, 1, 32, CAP, BIAS>, (long)a.tiles * a.kv_heads, 1, 4 * 32 * Tile<T>::kRow, a, "fc_attention_docs_backward (rows)", st);
+  }
+  if (rc != FC_OK) return rc;
+  constexpr int row = Tile<T>::kRow;
+  const long four = (a.k_rows + 127) / 128 * (long)a.kv_heads;
+  if (four >= cus)
+    rc = launch_docs(docs_grad_keys_kernel<T, 4, 64, CAP, BIAS>, four, 4, 2 * (128 * row + 7 * 256), a, "fc_attention_docs_backward (keys)", st);
+  else
+    rc = launch_docs(docs_grad_keys_kernel<T, 1, 32, CAP, BIAS>, (a.k_rows + 31) / 32 * (long)a.kv_heads, 1, 2 * (64 * row + 7 * 256), a, "fc_attention_docs_backward (keys)", st);
+  if (rc != FC_OK || !a.d_slopes) return rc;
+  return launch_docs(docs_grad_slopes_kernel, (long)a.kv_heads * a.group.d, 4, 0, a, "fc_attention_docs_backward (slopes)", st);
+}
+
+template <typename T>
+int launch_grads_type(const Args& a, bool cap, hipStream_t st) {
+  if (a.slopes) return cap ? launch_grads<T, true, true>(a, st) : launch_grads<T, false, true>(a, st);
+  return cap ? launch_grads<T, true, false>(a, st) : launch_grads<T, false, false>(a, st);
+}
+
+}  // namespace
+}  // namespace docs
+}  // namespace fc
+
+using namespace fc;
+
+extern "C" {
+
+size_t fc_attention_docs_backward_scratch_bytes(const fc_docs* d) {
+  if (docs::check_docs(d, "fc_attention_docs_backward_scratch_bytes") != FC_OK || d->docs == 0) return 0;
+  return docs::grad_bytes(*d);
+}
+
+int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_row, int64_t out_head, const float* stats, const void* d_out,
+                               int64_t do_row, int64_t do_head, void* d_q, int64_t dq_row, int64_t dq_head, void* d_k, int64_t dk_row,
+                               int64_t dk_head, void* d_v, int64_t dv_row, int64_t dv_head, float* d_slopes, void* scratch,
+                               size_t scratch_bytes, fc_stream st) {
+  const int rc = docs::check_docs(d, "fc_attention_docs_backward");
+  if (rc != FC_OK) return rc;
+  if (d_slopes && !d->slopes) return fail(FC_EINVAL, "fc_attention_docs_backward: a gradient of slopes that are not given");
+  if (d->docs == 0 || (d->q_rows == 0 && d->k_rows == 0)) return FC_OK;
+  if ((d->q_rows && (!out || !stats || !d_out || !d_q)) || (d->k_rows && (!d_k || !d_v)))
+    return fail(FC_EINVAL, "fc_attention_docs_backward: null operand");
+  if (!docs::rows_aligned(out, out_row, out_head, d->kind) || !docs::rows_aligned(d_out, do_row, do_head, d->kind) ||
+      !docs::rows_aligned(d_q, dq_row, dq_head, d->kind) || !docs::rows_aligned(d_k, dk_row, dk_head, d->kind) ||
+      !docs::rows_aligned(d_v, dv_row, dv_head, d->kind) || ((uintptr_t)stats & 7))
+    return fail(FC_EINVAL, "fc_attention_docs_backward: rows and heads must start on 16-byte boundaries");
+  const size_t need = docs::grad_bytes(*d);
+  if (need && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 15)))
+    return fail(FC_ENOMEM, "fc_attention_docs_backward: scratch of %zu bytes (16-byte aligned) needed, %zu given", need, scratch ? scratch_bytes : 0);
+  const int size = d->kind == PREC_F32 ? 4 : 2;
+  docs::Args a = docs::make_args(*d);
+  a.out = (char*)const_cast<void*>(out);
+  a.out_row = out_row * size; a.out_head = out_head * size;
+  a.stats = const_cast<float*>(stats);
+  a.d_out = (const char*)d_out;
+  a.do_row = do_row * size; a.do_head = do_head * size;
+  a.dq = (char*)d_q; a.dk = (char*)d_k; a.dv = (char*)d_v;
+  a.dq_row = dq_row * size; a.dq_head = dq_head * size;
+  a.dk_row = dk_row * size; a.dk_head = dk_head * size;
+  a.dv_row = dv_row * size; a.dv_head = dv_head * size;
+  a.d_slopes = d_slopes;
+  a.table = (float*)scratch;
+  a.rows_pad = docs::pad_rows(*d);
+  return d->kind == PREC_F32 ? docs::launch_grads_type<float>(a, d->cap > 0.f, st) : docs::launch_grads_type<bf16>(a, d->cap > 0.f, st);
+}
+
+}  // extern "C"

@@ -648,3 +648,43 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
         _lib.check(lib.fc_attention_docs(d, out.data_ptr(), *_strides(out), stats.data_ptr(), scratch.data_ptr(), scratch.numel(),
                                          _lib.current_stream()), "fc_attention_docs")
     return out, stats
+
+
+def attention_docs_backward(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, stats: torch.Tensor,
+                            q_offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None, causal: bool = False,
+                            prefix: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None, cap: float = 0.0,
+                            scale: Optional[float] = None, slope_grad: bool = False, d_q: Optional[torch.Tensor] = None,
+                            d_k: Optional[torch.Tensor] = None, d_v: Optional[torch.Tensor] = None) -> "tuple[torch.Tensor, ...]":
+    """Gradients of `attention_docs` (same operands and masks; `out` and `stats` are its results) from the gradient `d_out` of its
+    output: (d_q, d_k, d_v), and d_slopes float32 [heads] if `slope_grad`.  Gradients of shared key heads are summed over their query
+    heads; all sums have a fixed order.  Given d_q / d_k / d_v (strided rows and heads, e.g. the columns of a fused projection's
+    gradient) are written into, rows of no document left as they were; where none is given those rows get 0."""
+    given = [d_q, d_k, d_v]
+    fill = all(t is None for t in given)
+    _heads(q, "q", q.dtype)
+    for t, name in ((d_out, "d_out"), (out, "out")):
+        _heads(t, name, q.dtype)
+        if t.shape != q.shape:
+            raise ValueError(f"{name} must be {tuple(q.shape)}, got {tuple(t.shape)}")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (*q.shape[:2], 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be contiguous float32 {(*q.shape[:2], 2)}, got {stats.dtype} {tuple(stats.shape)}")
+    if slope_grad and slopes is None:
+        raise ValueError("slope_grad needs slopes")
+    for t, like, name in ((d_q, q, "d_q"), (d_k, k, "d_k"), (d_v, v, "d_v")):
+        if t is not None:
+            _written(t, name, like)
+    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill=fill)
+    make = torch.empty if fill and d.docs else torch.zeros
+    d_q, d_k, d_v = (make(like.shape, dtype=like.dtype, device=like.device) if t is None else t for t, like in zip(given, (q, k, v)))
+    _on_device(q.device, d_out=d_out, out=out, stats=stats, d_q=d_q, d_k=d_k, d_v=d_v)
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        d_slopes = torch.empty(q.shape[1], dtype=torch.float32, device=q.device) if slope_grad else None
+        if slope_grad and d.docs == 0:
+            d_slopes.zero_()
+        scratch = torch.empty(lib.fc_attention_docs_backward_scratch_bytes(d), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.fc_attention_docs_backward(d, out.data_ptr(), *_strides(out), stats.data_ptr(), d_out.data_ptr(), *_strides(d_out),
+                                                  d_q.data_ptr(), *_strides(d_q), d_k.data_ptr(), *_strides(d_k), d_v.data_ptr(),
+                                                  *_strides(d_v), _ptr(d_slopes), scratch.data_ptr(), scratch.numel(),
+                                                  _lib.current_stream()), "fc_attention_docs_backward")
+    return (d_q, d_k, d_v) + ((d_slopes,) if slope_grad else ())

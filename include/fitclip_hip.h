@@ -225,6 +225,14 @@ typedef struct {
 FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
                       size_t scratch_bytes, fc_stream stream);
+/* Gradients of fc_attention_docs from the gradient d_out of its result: d_q, d_k, d_v of q, k, v (same element kind) and, if d_slopes
+ * is given, of the slopes (dev f32 [q_heads]).  out and stats are the forward's.  Gradients of shared key heads are summed over their
+ * query heads; every sum has a fixed order (no atomics).  scratch: fc_attention_docs_backward_scratch_bytes. */
+FC_API size_t fc_attention_docs_backward_scratch_bytes(const fc_docs* d);
+FC_API int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_row, int64_t out_head, const float* stats,
+                               const void* d_out, int64_t do_row, int64_t do_head, void* d_q, int64_t dq_row, int64_t dq_head,
+                               void* d_k, int64_t dk_row, int64_t dk_head, void* d_v, int64_t dv_row, int64_t dv_head,
+                               float* d_slopes, void* scratch, size_t scratch_bytes, fc_stream stream);
 
 /* ---- WiSE (aligner/wise.py:16): out = (1 - weight_for_2) * a + weight_for_2 * b over n floats ------------------ */
 FC_API int fc_wise(const float* a, const float* b, double weight_for_2, float* out, size_t n, fc_stream stream);

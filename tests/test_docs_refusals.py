@@ -124,3 +124,39 @@ def test_the_c_rotary_refuses(change, match):
              interleaved=0, inverse=0, out=4096, out_row=128, out_head=64, rows=8, heads=2, dim=64, st=None) | change
     assert lib.fc_rotary(*a.values()) == -1
     assert match in lib.fc_last_error(), lib.fc_last_error()
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(d_out=torch.zeros(8, 2, 64)), ValueError, "d_out"),
+    (dict(out=torch.zeros(8, 4, 64, dtype=torch.bfloat16)), TypeError, "out"),
+    (dict(stats=torch.zeros(8, 4)), ValueError, "stats"),
+    (dict(stats=torch.zeros(8, 4, 2, dtype=torch.float64)), ValueError, "stats"),
+    (dict(slope_grad=True), ValueError, "slopes"),
+    (dict(d_k=torch.zeros(8, 4, 64)), ValueError, "d_k"),
+    (dict(d_v=torch.zeros(1, 2, 64).expand(8, 2, 64)), ValueError, "overlap"),
+    (dict(), _lib.FitclipHipError, "no CPU fallback"),
+])
+def test_gradients_refuse(change, error, match):
+    q, k, v = _qkv()
+    how = dict(d_out=torch.zeros(8, 4, 64), q=q, k=k, v=v, out=torch.zeros(8, 4, 64), stats=torch.zeros(8, 4, 2), q_offsets=OFF) | change
+    with pytest.raises(error, match=match):
+        ops.attention_docs_backward(**how)
+
+
+def test_the_c_gradients_refuse():
+    lib = _lib.load()
+
+    def call(d, out=4096, d_k=4096, dq_row=256, d_slopes=None, scratch=4096, n=1 << 30):
+        return lib.fc_attention_docs_backward(d, out, 256, 64, 4096, 4096, 256, 64, 4096, dq_row, 64, d_k, 128, 64, 4096, 128, 64, d_slopes, scratch, n, None)
+    d = _c_docs()
+    need = lib.fc_attention_docs_backward_scratch_bytes(d)
+    assert need > 0 and lib.fc_attention_docs_backward_scratch_bytes(_c_docs(kind=9)) == 0
+    assert call(d, out=None) == -1 and b"null" in lib.fc_last_error()
+    assert call(d, d_k=None) == -1 and b"null" in lib.fc_last_error()
+    assert call(d, dq_row=258) == -1 and b"16-byte" in lib.fc_last_error()
+    assert call(d, d_slopes=4096) == -1 and b"slopes" in lib.fc_last_error()
+    assert call(d, n=need - 1) == -3 and call(d, scratch=None) == -3
+    assert call(_c_docs(docs=0), scratch=None) == 0
+    bad = _c_docs()
+    bad.struct_size = 16
+    assert call(bad) == -1 and b"struct_size" in lib.fc_last_error()

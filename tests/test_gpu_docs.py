@@ -212,6 +212,207 @@ def test_attention_values_behind_a_mask_reach_nobody(dtype, bad, k_len):
         who.copy_(kept)
 
 
+# ---------------------------------------------------------------------------------------------------------------- gradients
+def _check_gradients(q, k, v, q_len, k_len=None, seed=50, ref=None, **how):
+    d_out = _rand(*q.shape, seed=seed, dtype=q.dtype)
+    q_off, k_off = R.offsets(q_len), None if k_len is None else R.offsets(k_len)
+    out, stats = ops.attention_docs(q, k, v, q_off, k_off, **how)
+    slopes = how.get("slopes")
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, k_off, slope_grad=slopes is not None, **how)
+    ref = ref or R.attention(q, k, v, q_len, k_len, d_out=d_out, **how)
+    keys = max(list(q_len if k_len is None else k_len) + [0])
+    ds = R.score_error(ref, keys, slopes, cap=how.get("cap", 0.0))
+    bounds = R.grad_bounds(ref, q, k, v, d_out, q.dtype, keys, ds, how.get("cap", 0.0), slopes)
+    for name, got in zip(("d_q", "d_k", "d_v", "d_slopes"), grads):
+        _within(name, got, ref[name], bounds[name])
+    again = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, k_off, slope_grad=slopes is not None, **how)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    return grads, ref, bounds
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len", [[1], [2], [31], [32], [33], [65], [127, 1], [0, 5, 0, 0, 3, 0], [1] * 70, [20, 0, 77, 4, 33, 1, 64]])
+def test_gradients_of_documents(dtype, causal, q_len):
+    q, k, v = _operands(sum(q_len), sum(q_len), 2, 2, dtype, seed=len(q_len), layout="fused")
+    grads, _, _ = _check_gradients(q, k, v, q_len, causal=causal)
+    if max(q_len) == 1:  # one key: its weight is 1 whatever the score
+        assert not grads[0].any() and not grads[1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(3, 1), (6, 2), (5, 5)])
+@pytest.mark.parametrize("layout", ["apart", "heads first"])
+def test_gradients_of_shared_heads(dtype, heads, kv_heads, layout):
+    q, k, v = _operands(64, 64, heads, kv_heads, dtype, seed=heads, layout=layout)
+    _check_gradients(q, k, v, [23, 1, 40], causal=True, slopes=torch.rand(heads, generator=torch.Generator().manual_seed(1)).to(DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 2.0, 30.0])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_gradients_of_masks_caps_and_biases(dtype, cap, slopes, prefix):
+    q_len = [45, 7, 0, 61, 12]
+    q, k, v = _operands(125, 125, 4, 2, dtype, seed=9, layout="fused")
+    pre = torch.tensor([20, 100, 3, 0, -4], dtype=torch.int32, device=DEV) if prefix else None
+    _check_gradients(q, k, v, q_len, causal=True, prefix=pre, cap=cap, slopes=torch.tensor([0.5, 0.0, 2.0, 0.01], device=DEV) if slopes else None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q_len,k_len", [([1], [900]), ([1, 1, 1], [40, 700, 1]), ([3, 0, 5], [70, 9, 333]), ([1], [0]), ([4, 2], [2, 9]),
+                                         ([40, 3], [7, 300]), ([100, 30], [1, 1]), ([0, 0], [5, 60])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_other_numbers_of_keys(dtype, q_len, k_len, causal):
+    q, k, v = _operands(sum(q_len), sum(k_len), 6, 2, dtype, seed=3)
+    _check_gradients(q, k, v, q_len, k_len, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_four_wave_tiles(dtype):
+    q_len = [300, 17, 129, 0, 64, 250]
+    rows, heads = sum(q_len), 64
+    q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
+    d_out = _rand(rows, heads, 64, seed=5, dtype=dtype)
+    for causal in (False, True):
+        out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal)
+        grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=causal)
+        some = [0, 63]
+        ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, d_out=d_out[:, some])
+        bounds = R.grad_bounds(ref, q[:, some], k[:, some], v[:, some], d_out[:, some], dtype, 300, R.score_error(ref, 300))
+        for name, got in zip(("d_q", "d_k", "d_v"), grads):
+            _within(name, got[:, some], ref[name], bounds[name])
+
+
+def test_gradients_by_differences():
+    """Central differences of the 64-bit forward against the kernels' gradients."""
+    q_len, how = [5, 14], dict(causal=True, cap=3.0, prefix=torch.tensor([2, 9], dtype=torch.int32, device=DEV),
+                               slopes=torch.tensor([0.3, 0.05], device=DEV))
+    q, k, v = _operands(19, 19, 2, 1, torch.float32, seed=21)
+    grads, ref, bounds = _check_gradients(q, k, v, q_len, seed=50, **how)
+    d_out = _rand(*q.shape, seed=50).double().cpu()
+    ops64 = {"d_q": q.double().cpu(), "d_k": k.double().cpu(), "d_v": v.double().cpu(), "d_slopes": how["slopes"].double().cpu()}
+    step = 1e-4
+
+    def loss(x):
+        return float((R.attention(x["d_q"], x["d_k"], x["d_v"], q_len, **(how | {"slopes": x["d_slopes"]}))["out"] * d_out).sum())
+    for name, got in zip(ops64, grads):
+        flat = got.double().cpu().reshape(-1)
+        for at in (0, flat.numel() // 2, flat.numel() - 1):
+            moved = []
+            for sign in (step, -step):
+                x = {n: t.clone() for n, t in ops64.items()}
+                x[name].view(-1)[at] += sign
+                moved.append(loss(x))
+            # truncation: step^2 times a third derivative of order 100; rounding of the 64-bit sums: 1e-13 / step
+            assert abs((moved[0] - moved[1]) / (2 * step) - float(flat[at])) <= float(bounds[name].reshape(-1)[at]) + 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_go_into_the_columns_of_a_fused_projection(dtype):
+    rows, heads = 90, 2
+    q, k, v = _operands(rows, rows, heads, heads, dtype, seed=5, layout="fused")
+    q_off, d_out = R.offsets([10, 31]), _rand(rows, heads, 64, seed=6, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, q_off)
+    own = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off)
+    assert all((g[41:] == 0).all() for g in own)
+    d_qkv = torch.full((rows, 3 * heads * 64), 7.0, dtype=dtype, device=DEV)
+    into = [t.view(rows, heads, 64) for t in d_qkv.split(heads * 64, 1)]
+    got = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, d_q=into[0], d_k=into[1], d_v=into[2])
+    assert all(a.data_ptr() == b.data_ptr() and torch.equal(a[:41], c[:41]) for a, b, c in zip(got, into, own))
+    assert (d_qkv[41:] == 7).all()
+    part = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, d_k=into[1])
+    assert (part[0][41:] == 0).all() and (part[1][41:] == 7).all() and (part[2][41:] == 0).all()
+    none = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets([]), slopes=torch.ones(heads, device=DEV), slope_grad=True)
+    assert not any(g.any() for g in none)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_of_what_nobody_sees(dtype, bad):
+    """NaN and infinities in rows and keys of other documents, of later keys and of no document reach no gradient that does not see them."""
+    q_len, rows = [30, 50], 85
+    q, k, v = _operands(rows, rows, 2, 1, dtype, seed=6)
+    d_out = _rand(rows, 2, 64, seed=7, dtype=dtype)
+    q_off = R.offsets(q_len)
+    out, stats = ops.attention_docs(q, k, v, q_off, causal=True)
+    clean = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, causal=True)
+    for who in (q, k, v, d_out):
+        kept = who.clone()
+        who[0] = bad    # the first document's first row / key: its whole document may be reached, the second one may not
+        who[80:] = bad  # of no document
+        o2, s2 = ops.attention_docs(q, k, v, q_off, causal=True)
+        got = ops.attention_docs_backward(d_out, q, k, v, o2, s2, q_off, causal=True)
+        for a, b in zip(got, clean):
+            assert torch.isfinite(a[30:]).all()
+            # the second pass adds in another order and keeps its weights in fp32
+            assert float((a[30:].double() - b[30:].double()).abs().max()) <= 8 * R.HALF[dtype] * float(b.double().abs().max()) + 1e-4
+        who.copy_(kept)
+    # a later row's dO reaches its own gradients and what it sees, no earlier row's d_q
+    d_out[29] = bad
+    got = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, causal=True)
+    assert torch.isfinite(got[0][:29]).all() and torch.isfinite(got[0][30:]).all() and not torch.isfinite(got[2][:30]).all()
+    assert all(torch.isfinite(g[30:]).all() for g in got)
+
+
+def test_a_block_of_video_tokens_forward_backward_and_captured():
+    """Rotary positions on q and k in place, attention over packed clips, its gradients, and the rotation taken back: against autograd in
+    64 bits, and replayed from a captured graph."""
+    frames, side, heads = [2, 5, 3], 3, 2
+    rows = sum(frames) * side * side
+    q_len = [f * side * side for f in frames]
+    place = torch.cat([torch.stack(torch.meshgrid(torch.arange(f), torch.arange(side), torch.arange(side), indexing="ij"), -1).view(-1, 3)
+                       for f in frames]).to(torch.int32).to(DEV)
+    inv_freq = (100.0 ** (-torch.arange(32) / 32)).to(DEV)
+    src = _rand(rows, 3 * heads * 64, seed=31)
+    d_out = _rand(rows, heads, 64, seed=32)
+    q_off = R.offsets(q_len)
+    D = heads * 64
+
+    def block(qkv):
+        qk = qkv[:, :2 * D].view(rows, 2 * heads, 64)
+        ops.rotary(qk, place, inv_freq, (8, 12, 12), out=qk)
+        q, k, v = (t.view(rows, heads, 64) for t in qkv.split(D, 1))
+        out, stats = ops.attention_docs(q, k, v, q_off, cap=20.0)
+        d_qkv = torch.empty_like(qkv)
+        d_q, d_k, d_v = (t.view(rows, heads, 64) for t in d_qkv.split(D, 1))
+        ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, cap=20.0, d_q=d_q, d_k=d_k, d_v=d_v)
+        d_qk = d_qkv[:, :2 * D].view(rows, 2 * heads, 64)
+        ops.rotary(d_qk, place, inv_freq, (8, 12, 12), inverse=True, out=d_qk)
+        return out, d_qkv
+
+    out, d_qkv = block(src.clone())
+    x = src.double().cpu()
+    turned = torch.cat([R.rotary(x[:, :2 * D].view(rows, 2 * heads, 64), place, inv_freq, (8, 12, 12)).reshape(rows, 2 * D), x[:, 2 * D:]], 1)
+    q, k, v = (t.reshape(rows, heads, 64) for t in turned.split(D, 1))
+    ref = R.attention(q, k, v, q_len, d_out=d_out, cap=20.0)
+    ds = R.score_error(ref, 45, cap=20.0) + 2.0 ** -24 * 64 * ref["big"]  # q and k carry the rotation's own error: 32 ulp of each
+    _within("out", out, ref["out"], R.out_bound(ref, v, torch.float32, 45, ds))
+    bounds = R.grad_bounds(ref, q, k, v, d_out, torch.float32, 45, ds, cap=20.0)
+    back = [R.rotary(ref[n], place, inv_freq, (8, 12, 12), inverse=True) for n in ("d_q", "d_k")]
+    for n, got, want in zip(("d_q", "d_k", "d_v"), d_qkv.split(D, 1), back + [ref["d_v"]]):
+        # turned back: a value takes both of its pair's errors, and the rotation's own
+        bound = 2 * bounds[n].max() + 32 * 2.0 ** -24 * want.abs().max()
+        _within(n, got.reshape(rows, heads, 64), want, bound)
+
+    side_stream = torch.cuda.Stream()
+    side_stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side_stream):
+        buf = src.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side_stream):
+            got = block(buf)
+        for turn in range(3):
+            buf.copy_(src)
+            for t in got:
+                t.zero_()
+            graph.replay()
+            eager = block(src.clone())
+            side_stream.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, eager)) and torch.equal(got[0], out) and torch.equal(got[1], d_qkv)
+    torch.cuda.current_stream().wait_stream(side_stream)
+
+
 def test_attention_on_another_stream_and_in_a_graph():
     q_len, k_len = [1, 1, 1], [300, 2000, 5]
     q, k, v = _operands(3, 2305, 6, 2, torch.bfloat16, seed=8)
