@@ -161,6 +161,37 @@ __device__ __forceinline__ void lds_dma(const char* src, char* dst) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
+// ROWS rows of 64 values, `stride` bytes apart from `base` on (wave-uniform; the rows behind the first n repeat row n - 1), into the LDS tile
+// at dst: 1 KiB pieces, dealt to the NW waves.  32-bit lane offsets on a uniform base; the lane number is hidden from the compiler so that
+// a dozen instructions per tile are spent instead of registers that live through the kernel.
+template <typename T, int ROWS, int NW>
+__device__ __forceinline__ void stage_rows(char* dst, const char* base, unsigned stride, int n, int wave, int lane) {
+  constexpr int PIECE = Tile<T>::kPiece, CH = 64 / PIECE, NP = ROWS / PIECE;
+  static_assert(NP % NW == 0, "every wave brings the same number of pieces");
+  asm volatile("" : "+v"(lane));
+  const unsigned in = lane / CH, pc = (lane % CH ^ Tile<T>::swizzle(in)) << 4;
+  const unsigned at = in * stride;
+#pragma unroll
+  for (int j = 0; j < NP / NW; ++j) {
+    const unsigned piece = wave + j * NW;
+    const unsigned turn = sizeof(T) == 2 ? (piece & 1) << 4 : (piece & 1) << 7 | (piece & 2) << 5;  // the row bits above the piece's
+    const unsigned off = n >= ROWS ? at + piece * PIECE * stride : min(piece * PIECE + in, (unsigned)(n - 1)) * stride;
+    lds_dma(base + (off + (pc ^ turn)), dst + piece * 1024);
+  }
+}
+
+// which of the lane's 16 scores in a tile of 32 keys (key 8 b + 4 hh + e of the tile) lie in [lo, hi) of the tile: bit 4 b + e
+__device__ __forceinline__ unsigned visible_bits(int lo, int hi, int hh) {
+  const int a = min(max(lo - 4 * hh, 0), 32), b = min(max(hi - 4 * hh, 0), 32);
+  const int ca = (a >> 3) * 4 + min(a & 7, 4), cb = (b >> 3) * 4 + min(b & 7, 4);
+  return ((1u << cb) - 1) & ~((1u << ca) - 1);
+}
+// x where bit i is set, else `other` (two instructions, no comparison)
+__device__ __forceinline__ float pick(unsigned bits, int i, float x, float other) {
+  const unsigned m = (unsigned)((int)(bits << (31 - i)) >> 31);
+  return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
+
 // a 64-value row in the registers of two lanes (lane r and r + 32), in the order of the row-operand reads below: bf16: 4 x 8 values
 // (d = 16 s + 8 hh ..), fp32: 8 x 4 values (d = 8 c + 4 hh ..)
 template <typename T> struct RowFrag;
@@ -280,33 +311,40 @@ __device__ __forceinline__ void cols_dot(const char* tile, const ColOff<float>& 
   }
 }
 
-// cols_dot value by value, for the (row, column) pairs that `sees(row)` says only: p = 0 does not keep an infinite or NaN value of a
-// masked row out of a matrix product
-template <typename T, typename Sees>
-__device__ __forceinline__ void cols_dot_careful(const char* tile, const f32x16& p, int lane, f32x16 (&out)[2], Sees sees) {
-  const int r = lane & 31, hh = lane >> 5;
-#pragma unroll 1
-  for (int w = 0; w < 32; ++w) {
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if ((w & ~4) == 8 * (i >> 2) + (i & 3)) x = p[i];
-    x = __shfl(x, r + ((w >> 2) & 1) * 32, 64);
-    const bool see = sees(w);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int byte = (32 * n + 8 * b + 4 * hh) * (int)sizeof(T);
-        typedef T vec __attribute__((ext_vector_type(4)));
-        const vec f = *reinterpret_cast<const vec*>(tile + w * Tile<T>::kRow + (((byte >> 4) ^ Tile<T>::swizzle(w)) << 4) + (byte & 15));
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (see) out[n][4 * b + e] = __builtin_fmaf(x, static_cast<float>(f[e]), out[n][4 * b + e]);
-        asm volatile("" ::: "memory");  // (one load at a time: this path is rare, its registers are everybody's)
-      }
-  }
+// score of a raw product in log2 units
+template <typename T, bool CAP, bool BIAS>
+__device__ __forceinline__ float score(const Args& a, float raw, float slope, float far) {
+  float x = CAP ? a.cap_out * tanh_f32<sizeof(T) == 4>(raw * a.cap_in) : raw * a.c;
+  if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
+  return x;
 }
+
+// ---- the way around NaN and infinities behind a mask.  A weight of 0 does not keep such a value out of a matrix product (0 * inf = NaN), so a
+// row (or key) whose result is not finite is done again by its wave, key by key, from what it sees alone.  That costs one test per row where
+// nothing is wrong, and the few registers of these loops.
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16> { typedef bf16x8 type; };
+template <> struct Chunk<float> { typedef f32x4 type; };
+
+__device__ __forceinline__ float lane_value(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
+
+// sum over d of row[d] x_d, x_d the value of lane d
+template <typename T>
+__device__ __forceinline__ float row_dot(const char* row, float x) {
+  constexpr int V = 16 / sizeof(T);
+  float s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 64 / V; ++c) {
+    const typename Chunk<T>::type v = *reinterpret_cast<const typename Chunk<T>::type*>(row + 16 * c);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s = __builtin_fmaf(static_cast<float>(v[e]), lane_value(x, c * V + e), s);
+  }
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ float value_at(const char* row, int d) { return static_cast<float>(*reinterpret_cast<const T*>(row + d * sizeof(T))); }
+template <typename T>
+__device__ __forceinline__ void put_at(char* row, int d, float x) { *reinterpret_cast<T*>(row + d * sizeof(T)) = static_cast<T>(x); }
 
 // NaN if a value is not finite, else 0
 __device__ __forceinline__ float not_finite(const f32x16 (&o)[2]) {
@@ -318,7 +356,7 @@ __device__ __forceinline__ float not_finite(const f32x16 (&o)[2]) {
   return x;
 }
 
-// o[n][..] = value (32 n + 8 b + 4 hh + e) of the lane's row, times `by` -> 32 rows of 64 values, through the wave's patch of LDS (32 rows)
+// o[n][..] = value (32 n + 8 b + 4 hh + e) of the lane's row, times `by` (0: exactly 0, whatever o holds) -> 32 rows of 64 values, through the wave's patch of LDS (32 rows)
 // and from there 16 bytes per lane; `at(w)` is row w's address, rows without their bit in `good` are left alone
 template <typename T, typename At>
 __device__ __forceinline__ void store_rows(char* patch, const f32x16 (&o)[2], float by, int lane, unsigned long long good, At at) {
@@ -328,7 +366,9 @@ __device__ __forceinline__ void store_rows(char* patch, const f32x16 (&o)[2], fl
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const f32x4 y = {o[n][4 * b] * by, o[n][4 * b + 1] * by, o[n][4 * b + 2] * by, o[n][4 * b + 3] * by};
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = by == 0.f ? 0.f : o[n][4 * b + e] * by;
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f32x4*>(patch + r * 256 + (((8 * n + 2 * b + hh) ^ (r & 15)) << 4)) = y;
       } else {

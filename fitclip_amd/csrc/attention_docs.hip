@@ -7,10 +7,6 @@
 //
 // Few rows over many keys (single tokens that are being written): the key range is cut into `splits` parts, each part leaves its
 // unnormalised O with (maximum, sum) in scratch, and a second kernel joins them in a fixed order.
-//
-// P = 0 does not keep an infinite or NaN value of a masked key out of a matrix product (0 * inf = NaN).  So a wave whose result is not
-// finite runs once more, and this time forms the products of the tiles that it sees in part value by value, for the rows that see the
-// key: values behind a mask never reach a row, at the cost of one test at the end.
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -21,11 +17,40 @@ namespace {
 
 template <typename T> constexpr int stage_bytes(int tk) { return 2 * tk * Tile<T>::kRow; }
 
+// One kernel row again, key by key (64 lanes = 64 keys for the scores, 64 dimensions for the sums), over keys [lo, hi).
+template <typename T, bool CAP, bool BIAS>
+__device__ void row_again(const Args& a, int head, int m, int lo, int hi, int pos, int split, bool sees, int lane) {
+  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+  const float q = value_at<T>(a.q + token * a.q_row + qh * a.q_head, lane), slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
+  const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
+  float top = -kInf, l = 0.f, o = 0.f;
+#pragma unroll 1
+  for (int j = lo; j < hi; j += 64) {
+    const int key = min(j + lane, hi - 1);
+    float x = score<T, CAP, BIAS>(a, row_dot<T>(kb + key * a.k_row, q), slope, fabsf((float)(pos - key)));
+    if (j + lane >= hi) x = -kInf;
+    const float mx = fmaxf(top, wave_max(x)), ref = mx == -kInf ? 0.f : mx;
+    const float p = __builtin_amdgcn_exp2f(x - ref), alpha = top == mx ? 1.f : __builtin_amdgcn_exp2f(top - ref);
+    top = mx;
+    l = l * alpha + wave_sum(p);
+    o *= alpha;
+#pragma unroll 1
+    for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(p, w), value_at<T>(vb + (long)(j + w) * a.v_row, lane), o);
+  }
+  if (a.splits > 1) {
+    const long at = ((long)split * a.kv_heads + head) * a.rows + m;
+    a.part[at * 64 + lane] = o;
+    if (lane == 0) *reinterpret_cast<f32x2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64 + at * 2) = f32x2{top, l};
+    return;
+  }
+  put_at<T>(a.out + token * a.out_row + qh * a.out_head, lane, sees ? o / l : 0.f);
+  if (lane == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{top, l};
+}
+
 template <typename T, int NW, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
-  constexpr int STAGE = stage_bytes<T>(TK), NP = 2 * TK / PIECE;  // 1 KiB pieces of a stage: K rows, then V rows
-  static_assert(NP % NW == 0, "every wave brings the same number of pieces");
+__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 3)))
+attention_docs_kernel(const Args a) {
+  constexpr int ROWB = Tile<T>::kRow, STAGE = stage_bytes<T>(TK);  // K rows, then V rows
   static_assert(NW * 32 * ROWB <= 2 * STAGE, "the output patches reuse the stages");
   constexpr int NT = TK / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -60,7 +85,12 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
     kend = __builtin_amdgcn_readfirstlane(kend);
   }
   const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
-  const int t_first = (int)((long)ntile * split / a.splits), t_last = (int)((long)ntile * (split + 1) / a.splits);
+  int t_first = 0, t_last = ntile;
+  if (a.splits > 1) {
+    const int part = (int)((unsigned)(ntile + a.splits - 1) / (unsigned)a.splits);
+    t_first = min(ntile, split * part);
+    t_last = min(ntile, t_first + part);
+  }
 
   const int m = min(m0 + r, a.rows - 1);
   const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
@@ -72,14 +102,9 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
   const char* vbase = a.v + head * a.v_head;
   auto stage = [&](int t) {
     char* dst = smem + (t & 1) * STAGE;
-    const int in = lane / (64 / PIECE), pc = lane % (64 / PIECE);
-#pragma unroll
-    for (int j = 0; j < NP / NW; ++j) {
-      const int piece = wave + j * NW, isv = piece >= NP / 2;
-      const int w = (isv ? piece - NP / 2 : piece) * PIECE + in;
-      const long key = min(kbeg + t * TK + w, kend - 1);  // rows behind the last key repeat it: they are masked
-      lds_dma((isv ? vbase + key * a.v_row : kbase + key * a.k_row) + ((pc ^ Tile<T>::swizzle(w)) << 4), dst + piece * 1024);
-    }
+    const long first = kbeg + t * TK;
+    stage_rows<T, TK, NW>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave, lane);
+    stage_rows<T, TK, NW>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave, lane);
   };
 
   RowOff<T> koff;
@@ -88,98 +113,88 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
   voff.init(lane);
 
   f32x16 o[2];
-  float mref, mtop, l;
-  bool careful = false;
-  while (true) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-    mref = mtop = -kInf;  // the maximum that the sums refer to (it follows the true one in steps of 2^8), and the true one
-    l = 0.f;
-    if (t_first < t_last) stage(t_first);
-    for (int t = t_first; t < t_last; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
-      if (t + 1 < t_last) stage(t + 1);
-      const int k0 = kbeg + t * TK;
-      if (k0 >= whi || k0 + TK <= wlo) continue;  // (wave-uniform)
-      const char* kt = smem + (t & 1) * STAGE;
-      const char* vt = kt + TK * ROWB;
-      const bool full = full_lo <= k0 && k0 + TK <= full_hi;
-      f32x16 s[NT];
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float mref = -kInf, mtop = -kInf, l = 0.f;  // the maximum that the sums refer to (it follows the true one in steps of 2^8), the true one
+  if (t_first < t_last) stage(t_first);
+  for (int t = t_first; t < t_last; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
+    if (t + 1 < t_last) stage(t + 1);
+    const int k0 = kbeg + t * TK;
+    if (k0 >= whi || k0 + TK <= wlo) continue;  // (wave-uniform)
+    const char* kt = smem + (t & 1) * STAGE;
+    const char* vt = kt + TK * ROWB;
+    const bool full = full_lo <= k0 && k0 + TK <= full_hi;
+    f32x16 s[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+      s[u] = rows_dot(kt + u * 32 * ROWB, koff, qf, s[u]);
+    }
+    // scores in log2 units
+    const float at = BIAS ? (float)(row.pos - k0 - 4 * hh) : 0.f;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int w = 32 * u + 8 * (i >> 2) + (i & 3);
+        float x = s[u][i];  // (neither cap nor bias: scaled in the exponent's fma)
+        if constexpr (CAP) x = a.cap_out * tanh_f32<sizeof(T) == 4>(x * a.cap_in);
+        else if constexpr (BIAS) x *= a.c;
+        if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(at - (float)w), x);
+        s[u][i] = x;
+      }
+    if (!full) {
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
+        const unsigned bits = visible_bits(row.lo - k0 - 32 * u, row.hi - k0 - 32 * u, hh);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-        s[u] = rows_dot(kt + u * 32 * ROWB, koff, qf, s[u]);
-      }
-      // scores in log2 units
-      const float at = BIAS ? (float)(row.pos - k0 - 4 * hh) : 0.f;
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int w = 32 * u + 8 * (i >> 2) + (i & 3);
-          float x = CAP ? a.cap_out * tanh_f32<sizeof(T) == 4>(s[u][i] * a.cap_in) : s[u][i] * a.c;
-          if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(at - (float)w), x);
-          s[u][i] = x;
-        }
-      const unsigned rel = (unsigned)(k0 + 4 * hh - row.lo), len = (unsigned)(row.hi - row.lo);
-      if (!full) {
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int w = 32 * u + 8 * (i >> 2) + (i & 3);
-            s[u][i] = rel + w < len ? s[u][i] : -kInf;
-          }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[u][i]), s[u][i + 1]);
-      mx = swap_max(mx);
-      mtop = fmaxf(mtop, mx);
-      if (__any(mtop > mref + 8.f)) {  // 2^8 of headroom costs nothing in fp32 and saves most of the rescaling
-        const float alpha = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);
-        l *= alpha;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[n][i] *= alpha;
-        mref = mtop;
-      }
-      const float mm = mref == -kInf ? 0.f : mref;
-#pragma unroll
-      for (int u = 0; u < NT; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - mm);
-          l += s[u][i];
-        }
-      if (careful && !full) {
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-          cols_dot_careful<T>(vt + u * 32 * ROWB, s[u], lane, o, [&](int w) { return rel - 4 * hh + 32 * u + w < len; });
-      } else {
-#pragma unroll
-        for (int u = 0; u < NT; ++u) cols_dot(vt + u * 32 * ROWB, voff, s[u], o);
+        for (int i = 0; i < 16; ++i) s[u][i] = pick(bits, i, s[u][i], -kInf);
       }
     }
-    if (careful) break;
-    const float probe = not_finite(o);
-    if (!__syncthreads_or(row.valid && probe != probe)) break;
-    careful = true;
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[u][i]), s[u][i + 1]);
+    mx = swap_max(mx);
+    constexpr bool kRaw = !CAP && !BIAS;
+    if constexpr (kRaw) mx *= a.c;
+    mtop = fmaxf(mtop, mx);
+    if (__any(mtop > mref + 8.f)) {  // 2^8 of headroom costs nothing in fp32 and saves most of the rescaling
+      const float alpha = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[n][i] *= alpha;
+      mref = mtop;
+    }
+    const float mm = mref == -kInf ? 0.f : mref;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[u][i] = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(s[u][i], a.c, -mm) : s[u][i] - mm);
+        l += s[u][i];
+      }
+#pragma unroll
+    for (int u = 0; u < NT; ++u) cols_dot(vt + u * 32 * ROWB, voff, s[u], o);
   }
   l = swap_sum(l);
   const float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
   l *= down;
 
+  const float probe = swap_sum(not_finite(o));
+  const bool again = row.valid && probe != probe;
+
   if (a.splits > 1) {
     const long at = ((long)split * a.kv_heads + head) * a.rows + m0 + r;
-    if (m0 + r < a.rows) {
+    if (m0 + r < a.rows && !again) {
       float* po = a.part + at * 64;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -190,36 +205,48 @@ __global__ void __launch_bounds__(NW * 64) attention_docs_kernel(const Args a) {
       // (sum -1: a row of no document)
       if (hh == 0) *reinterpret_cast<f32x2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64 + at * 2) = f32x2{mtop, row.valid ? l : -1.f};
     }
-    return;
+  } else {
+    const float inv = sees ? down / l : 0.f;
+    const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
+    if (hh == 0 && write)
+      *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
+    __syncthreads();  // (the patches reuse the stages)
+    store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
+      const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+      return a.out + tk * a.out_row + h * a.out_head;
+    });
   }
-
-  const float inv = sees ? down / l : 0.f;
-  if (hh == 0 && m0 + r < a.rows && (row.valid || a.fill))
-    *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
-  __syncthreads();  // (the patches reuse the stages)
-  store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(row.valid || (a.fill && m0 + r < a.rows)), [&](int w) {
-    const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
-    return a.out + tk * a.out_row + h * a.out_head;
-  });
+  unsigned bad = (unsigned)__ballot(again);
+  while (bad) {
+    const int w = __builtin_ctz(bad);
+    bad &= bad - 1;
+    const int lo = __builtin_amdgcn_readlane(row.lo, w), hi = __builtin_amdgcn_readlane(row.hi, w), pos = __builtin_amdgcn_readlane(row.pos, w);
+    row_again<T, CAP, BIAS>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lo < hi, lane);
+  }
 }
 
-// joins the parts of a key range: 16 lanes per kernel row, parts in order
+// joins the parts of a key range: a workgroup per kernel row, 16 parts at a time by 16 lanes each, then the 16 sums in order
 template <typename T>
 __global__ void __launch_bounds__(256) attention_docs_join_kernel(const Args a) {
-  const long idx = (long)blockIdx.x * 16 + (threadIdx.x >> 4), n = (long)a.kv_heads * a.rows;
-  const int ch = threadIdx.x & 15;
-  if (idx >= n) return;
+  __shared__ float sums[16][64 + 4];  // O, then the sum of the weights
+  __shared__ float tops[4];
+  const long idx = blockIdx.x, n = (long)a.kv_heads * a.rows;
+  const int tid = threadIdx.x, ch = tid & 15, g = tid >> 4;
   const int head = (int)(idx / a.rows), m = (int)(idx - (long)head * a.rows);
-  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.part + (long)a.splits * n * 64) + idx;
-  float top = -kInf;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * n][0]);
-  const bool valid = ml[0][1] >= 0.f || ml[0][1] != ml[0][1];
+  const float l0 = ml[0][1];
+  const bool valid = !(l0 < 0.f);
   if (!valid && !a.fill) return;
+  float top = -kInf;
+  for (int s = tid; s < a.splits; s += 256) top = fmaxf(top, ml[s * n][0]);
+  top = wave_max(top);
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const float ref = top == -kInf ? 0.f : top;
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = g; s < a.splits; s += 16) {
     const f32x2 v = ml[s * n];
     const float w = __builtin_amdgcn_exp2f(v[0] - ref);
     const f32x4 p = *reinterpret_cast<const f32x4*>(a.part + (s * n + idx) * 64 + ch * 4);
@@ -227,21 +254,21 @@ __global__ void __launch_bounds__(256) attention_docs_join_kernel(const Args a) 
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(p[e], w, o[e]);
   }
-  if (!valid) {
-    top = -kInf;
-    l = 0.f;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // (sum 0: the row sees nothing)
-  char* dst = a.out + token * a.out_row + qh * a.out_head;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4*>(dst + ch * 16) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  } else {
-    bf16x4 w;
+  *reinterpret_cast<f32x4*>(&sums[g][ch * 4]) = o;
+  if (ch == 0) sums[g][64] = l;
+  __syncthreads();
+  if (tid >= 64) return;
+  float x = 0.f;
+  l = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(o[e] * inv);
-    *reinterpret_cast<bf16x4*>(dst + ch * 8) = w;
+  for (int s = 0; s < 16; ++s) {
+    x += sums[s][tid];
+    l += sums[s][64];
   }
-  if (ch == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{top, l};
+  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+  const bool zero = !valid || l == 0.f;  // (sum 0: the row sees nothing)
+  put_at<T>(a.out + token * a.out_row + qh * a.out_head, tid, zero ? 0.f : x / l);
+  if (tid == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{valid ? top : -kInf, valid ? l : 0.f};
 }
 
 struct Plan {
@@ -260,7 +287,7 @@ Plan plan_forward(const fc_docs& d) {
   // keys that a tile walks over, from the mean lengths: the documents that 32 kernel rows touch
   const double mean_rows = std::max(1.0, (double)rows / d.docs), mean_keys = (double)d.k_rows / d.docs;
   const double keys = std::min((double)d.k_rows, (32.0 / mean_rows + 1.0) * mean_keys);
-  p.splits = (int)std::max(1L, std::min({4 * cus / std::max(1L, units), (long)(keys / 256.0), 512L}));
+  p.splits = (int)std::max(1L, std::min({2 * cus / std::max(1L, units), (long)(keys / 256.0), 512L}));
   return p;
 }
 
@@ -280,7 +307,7 @@ int launch_forward(const Args& a, hipStream_t st) {
   FC_CHECK_LAUNCH("fc_attention_docs");
   if (a.splits > 1) {
     const long n = (long)a.kv_heads * a.rows;
-    hipLaunchKernelGGL((attention_docs_join_kernel<T>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attention_docs_join_kernel<T>), dim3((unsigned)n), dim3(256), 0, st, a);
     FC_CHECK_LAUNCH("fc_attention_docs (join)");
   }
   return FC_OK;
@@ -318,6 +345,8 @@ int check_docs(const fc_docs* d, const char* what) {
   if ((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) ||
       ((d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head) * size & 15))
     return fail(FC_EINVAL, "%s: rows and heads must start on 16-byte boundaries", what);
+  if (d->k_row * size >= 1 << 25 || d->v_row * size >= 1 << 25)
+    return fail(FC_EINVAL, "%s: rows of k or v lie 32 MiB or more apart", what);
   return FC_OK;
 }
 

@@ -11,7 +11,6 @@
 //   keys: a wave owns 32 keys (K and V in registers) and walks over the kernel rows that see them - all heads of the group, so the gradients
 //   of shared heads need no further sum: S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
-// The products that weigh a masked row or key with 0 are guarded against NaN and infinities there as in the forward.
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -46,12 +45,88 @@ __device__ __forceinline__ float dot(const RowFrag<float>& x, const RowFrag<floa
   return s;
 }
 
+// dS behind P, dP, D and the raw product
+template <typename T, bool CAP>
+__device__ __forceinline__ float bent_by(const Args& a, float raw, float ds) {
+  if constexpr (CAP) {
+    const float t = tanh_f32<sizeof(T) == 4>(raw * a.cap_in);
+    ds *= 1.f - t * t;
+  }
+  return ds;
+}
+
+// d_q of one kernel row again, key by key (see attention_docs.h)
+template <typename T, bool CAP, bool BIAS>
+__device__ void row_grad_again(const Args& a, int head, int m, int lo, int hi, int pos, float top, float inv, float D, int lane) {
+  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+  const float q = value_at<T>(a.q + token * a.q_row + qh * a.q_head, lane), go = value_at<T>(a.d_out + token * a.do_row + qh * a.do_head, lane);
+  const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
+  const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
+  float o = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f;
+#pragma unroll 1
+  for (int j = lo; j < hi; j += 64) {
+    const int key = min(j + lane, hi - 1);
+    const float raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
+    float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - top) * inv;
+    const float g = hi - lo == 1 ? D : row_dot<T>(vb + key * a.v_row, go);
+    if (j + lane >= hi) p = 0.f;
+    pd = __builtin_fmaf(p, g, pd);
+    pf = __builtin_fmaf(p, far, pf);
+    pdf = __builtin_fmaf(p * g, far, pdf);
+    const float ds = bent_by<T, CAP>(a, raw, p * (g - D));
+#pragma unroll 1
+    for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
+  }
+  put_at<T>(a.dq + token * a.dq_row + qh * a.dq_head, lane, o * a.scale);
+  if constexpr (BIAS) {
+    pd = wave_sum(pd);
+    pf = wave_sum(pf);
+    pdf = wave_sum(pdf);
+    if (lane == 0) column(a, COL_DSLOPE, head)[m] = hi - lo > 1 ? pd * pf - pdf : 0.f;
+  }
+}
+
+// d_k and d_v of one key again, row by row (kernel rows r_lo .. r_hi - 1 hold those that see it)
+template <typename T, bool CAP, bool BIAS>
+__device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r_hi, int lane) {
+  const float k = value_at<T>(a.k + key * a.k_row + head * a.k_head, lane), v = value_at<T>(a.v + key * a.v_row + head * a.v_head, lane);
+  float dk = 0.f, dv = 0.f;
+#pragma unroll 1
+  for (int i = r_lo; i < r_hi; i += 64) {
+    const int m = min(i + lane, r_hi - 1);
+    const int lo = __float_as_int(column(a, COL_LO, head)[m]), hi = __float_as_int(column(a, COL_HI, head)[m]);
+    const bool see = i + lane < r_hi && (unsigned)(key - lo) < (unsigned)(hi - lo);
+    const unsigned long long seen = __ballot(see);
+    if (!seen) continue;
+    const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+    const float raw = row_dot<T>(a.q + token * a.q_row + qh * a.q_head, k);
+    const float g = row_dot<T>(a.d_out + token * a.do_row + qh * a.do_head, v);
+    float far = 0.f, slope = 0.f;
+    if constexpr (BIAS) {
+      far = fabsf((float)(__float_as_int(column(a, COL_POS, head)[m]) - key));
+      slope = column(a, COL_SLOPE, head)[m];
+    }
+    float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, head)[m]);
+    if constexpr (sizeof(T) == 4) p *= column(a, COL_INV, head)[m];
+    const float ds = hi - lo == 1 ? 0.f : bent_by<T, CAP>(a, raw, p * (g - column(a, COL_D, head)[m]));
+#pragma unroll 1
+    for (int w = 0; w < 64; ++w) {
+      if (!(seen >> w & 1)) continue;
+      const int mw = i + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+      dk = __builtin_fmaf(lane_value(ds, w), value_at<T>(a.q + tk * a.q_row + h * a.q_head, lane), dk);
+      dv = __builtin_fmaf(lane_value(p, w), value_at<T>(a.d_out + tk * a.do_row + h * a.do_head, lane), dv);
+    }
+  }
+  put_at<T>(a.dk + key * a.dk_row + head * a.dk_head, lane, dk * a.scale);
+  put_at<T>(a.dv + key * a.dv_row + head * a.dv_head, lane, dv);
+}
+
 // ------------------------------------------------------------------------------------------------------------------ rows
 template <typename T, int NW, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) docs_grad_rows_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
-  constexpr int STAGE = 2 * TK * ROWB, NP = 2 * TK / PIECE, NT = TK / 32;
-  static_assert(NP % NW == 0 && NW * 32 * ROWB <= 2 * STAGE, "pieces of a wave; patches");
+__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+docs_grad_rows_kernel(const Args a) {
+  constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;
+  static_assert(NW * 32 * ROWB <= 2 * STAGE, "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * NW];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
@@ -126,14 +201,9 @@ __global__ void __launch_bounds__(NW * 64) docs_grad_rows_kernel(const Args a) {
   const char* vbase = a.v + head * a.v_head;
   auto stage = [&](int t) {
     char* dst = smem + (t & 1) * STAGE;
-    const int in = lane / (64 / PIECE), pc = lane % (64 / PIECE);
-#pragma unroll
-    for (int j = 0; j < NP / NW; ++j) {
-      const int piece = wave + j * NW, isv = piece >= NP / 2;
-      const int w = (isv ? piece - NP / 2 : piece) * PIECE + in;
-      const long key = min(kbeg + t * TK + w, kend - 1);
-      lds_dma((isv ? vbase + key * a.v_row : kbase + key * a.k_row) + ((pc ^ Tile<T>::swizzle(w)) << 4), dst + piece * 1024);
-    }
+    const long first = kbeg + t * TK;
+    stage_rows<T, TK, NW>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave, lane);
+    stage_rows<T, TK, NW>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave, lane);
   };
   RowOff<T> roff;
   roff.init(r, hh);
@@ -141,92 +211,92 @@ __global__ void __launch_bounds__(NW * 64) docs_grad_rows_kernel(const Args a) {
   coff.init(lane);
 
   f32x16 o[2];
-  float pd, pf, pdf;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
-  bool careful = false;
-  while (true) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-    pd = pf = pdf = 0.f;
-    if (ntile) stage(0);
-    for (int t = 0; t < ntile; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (t + 1 < ntile) stage(t + 1);
-      const int k0 = kbeg + t * TK;
-      const char* kt = smem + (t & 1) * STAGE;
-      const char* vt = kt + TK * ROWB;
+    for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
+  float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
+  if (ntile) stage(0);
+  for (int t = 0; t < ntile; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t + 1 < ntile) stage(t + 1);
+    const int k0 = kbeg + t * TK;
+    const char* kt = smem + (t & 1) * STAGE;
+    const char* vt = kt + TK * ROWB;
+#pragma unroll 1
+    for (int u = 0; u < NT; ++u) {
+      const int ku = k0 + 32 * u;
+      if (ku >= whi || ku + 32 <= wlo) continue;  // (wave-uniform)
+      const bool full = full_lo <= ku && ku + 32 <= full_hi;
+      f32x16 s, dp;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const int ku = k0 + 32 * u;
-        if (ku >= whi || ku + 32 <= wlo) continue;  // (wave-uniform)
-        const bool full = full_lo <= ku && ku + 32 <= full_hi;
-        f32x16 s, dp;
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      s = rows_dot(kt + u * 32 * ROWB, roff, qf, s);
+      dp = rows_dot(vt + u * 32 * ROWB, roff, dof, dp);
+      __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
+      const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
+      const unsigned bits = full ? 0xffffu : visible_bits(row.lo - ku, row.hi - ku, hh);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-        s = rows_dot(kt + u * 32 * ROWB, roff, qf, s);
-        dp = rows_dot(vt + u * 32 * ROWB, roff, dof, dp);
-        const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
-        const unsigned rel = (unsigned)(ku + 4 * hh - row.lo), len = (unsigned)(row.hi - row.lo);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int w = 8 * (i >> 2) + (i & 3);
-          float bent = 0.f, x;
-          if constexpr (CAP) {
-            bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
-            x = a.cap_out * bent;
-          } else {
-            x = s[i] * a.c;
-          }
-          const float far = BIAS ? fabsf(at - (float)w) : 0.f;
-          if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
-          float p = __builtin_amdgcn_exp2f(x - top);
-          if constexpr (sizeof(T) == 4) p *= inv;
-          float g = dp[i];
-          if (!full) {
-            const bool see = rel + w < len;
-            p = see ? p : 0.f;
-            g = see ? (len == 1 ? D : g) : 0.f;  // one key: P = 1 whatever its score
-          }
-          if constexpr (BIAS) {
-            const float y = p * g;
-            pd += y;
-            pf = __builtin_fmaf(p, far, pf);
-            pdf = __builtin_fmaf(y, far, pdf);
-          }
-          float ds = p * (g - D);
-          if constexpr (CAP) ds *= 1.f - bent * bent;
-          if (!full) ds = rel + w < len ? ds : 0.f;
-          s[i] = ds;
+      for (int i = 0; i < 16; ++i) {
+        const int w = 8 * (i >> 2) + (i & 3);
+        float bent = 0.f, x;
+        if constexpr (CAP) {
+          bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
+          x = a.cap_out * bent;
+        } else {
+          x = s[i] * a.c;
         }
-        if (careful && !full)
-          cols_dot_careful<T>(kt + u * 32 * ROWB, s, lane, o, [&](int w) { return rel - 4 * hh + w < len; });
-        else
-          cols_dot(kt + u * 32 * ROWB, coff, s, o);
+        const float far = BIAS ? fabsf(at - (float)w) : 0.f;
+        if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
+        float p = __builtin_amdgcn_exp2f(x - top);
+        if constexpr (sizeof(T) == 4) p *= inv;
+        float g = dp[i];
+        if (!full) {
+          p = pick(bits, i, p, 0.f);
+          g = pick(bits, i, row.hi - row.lo == 1 ? D : g, 0.f);  // one key: P = 1 whatever its score
+        }
+        if constexpr (BIAS) {
+          const float y = p * g;
+          pd += y;
+          pf = __builtin_fmaf(p, far, pf);
+          pdf = __builtin_fmaf(y, far, pdf);
+        }
+        float ds = p * (g - D);
+        if constexpr (CAP) ds *= 1.f - bent * bent;
+        if (!full) ds = pick(bits, i, ds, 0.f);
+        s[i] = ds;
       }
+      __builtin_amdgcn_sched_barrier(0);
+      cols_dot(kt + u * 32 * ROWB, coff, s, o);
     }
-    if (careful) break;
-    const float probe = not_finite(o);
-    if (!__syncthreads_or(row.valid && probe != probe)) break;
-    careful = true;
   }
+  const float probe = swap_sum(not_finite(o));
+  const bool again = row.valid && probe != probe;
   if constexpr (BIAS) {
     pd = swap_sum(pd);
     pf = swap_sum(pf);
     pdf = swap_sum(pdf);
-    if (hh == 0 && m0 + r < a.rows_pad) column(a, COL_DSLOPE, head)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
+    if (hh == 0 && m0 + r < a.rows_pad && !again) column(a, COL_DSLOPE, head)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
   }
-  __syncthreads();
-  store_rows<T>(smem + wave * 32 * ROWB, o, a.scale, lane, __ballot(row.valid || (a.fill && m0 + r < a.rows)), [&](int w) {
+  __syncthreads();  // (the patches reuse the stages)
+  store_rows<T>(smem + wave * 32 * ROWB, o, row.valid ? a.scale : 0.f, lane, __ballot(row.valid ? !again : a.fill && m0 + r < a.rows), [&](int w) {
     const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
     return a.dq + tk * a.dq_row + h * a.dq_head;
   });
+  unsigned bad = (unsigned)__ballot(again);
+  while (bad) {
+    const int w = __builtin_ctz(bad);
+    bad &= bad - 1;
+    row_grad_again<T, CAP, BIAS>(a, head, m0 + w, __builtin_amdgcn_readlane(row.lo, w), __builtin_amdgcn_readlane(row.hi, w),
+                                 __builtin_amdgcn_readlane(row.pos, w), lane_value(top, w), lane_value(inv, w), lane_value(D, w), lane);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ keys
 template <typename T, int NW, int TQ, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) docs_grad_keys_kernel(const Args a) {
+__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+docs_grad_keys_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
   constexpr int OFF_DO = TQ * ROWB, OFF_TAB = 2 * TQ * ROWB;
   constexpr bool kInv = sizeof(T) == 4;
@@ -267,8 +337,10 @@ __global__ void __launch_bounds__(NW * 64) docs_grad_keys_kernel(const Args a) {
 
   auto stage = [&](int t) {
     char* dst = smem + (t & 1) * STAGE;
-    const int in = lane / (64 / PIECE), pc = lane % (64 / PIECE);
-#pragma unroll
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (addresses are formed here, not kept through the kernel)
+    const int in = ln / (64 / PIECE), pc = ln % (64 / PIECE);
+#pragma unroll 2
     for (int j = 0; j < (NP + NW - 1) / NW; ++j) {
       const int piece = wave + j * NW;
       if (piece < NROW) {
@@ -291,95 +363,90 @@ __global__ void __launch_bounds__(NW * 64) docs_grad_keys_kernel(const Args a) {
   coff.init(lane);
 
   f32x16 dk[2], dv[2];
-  bool careful = false;
-  while (true) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
-    if (t_first < t_last) stage(t_first);
-    for (int t = t_first; t < t_last; ++t) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (t + 1 < t_last) stage(t + 1);
-      const char* st = smem + (t & 1) * STAGE;
+    for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
+  if (t_first < t_last) stage(t_first);
+  for (int t = t_first; t < t_last; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t + 1 < t_last) stage(t + 1);
+    const char* st = smem + (t & 1) * STAGE;
+#pragma unroll 1
+    for (int u = 0; u < TQ / 32; ++u) {
+      const int block = t * (TQ / 32) + u;
+      if (block * 32 >= a.rows) continue;
+      const int32_t* bk = block_keys(a, head, block);
+      if (kw >= bk[1] || kw + 32 <= bk[0]) continue;  // (wave-uniform)
+      const bool full = bk[2] <= kw && kw + 32 <= bk[3];
+      const char* qt = st + u * 32 * ROWB;
+      const char* dt = qt + OFF_DO;
+      const char* tab = st + OFF_TAB + u * 128;
+      f32x16 s, dp;
 #pragma unroll
-      for (int u = 0; u < TQ / 32; ++u) {
-        const int block = t * (TQ / 32) + u;
-        if (block * 32 >= a.rows) continue;
-        const int32_t* bk = block_keys(a, head, block);
-        if (kw >= bk[1] || kw + 32 <= bk[0]) continue;  // (wave-uniform)
-        const bool full = bk[2] <= kw && kw + 32 <= bk[3];
-        const char* qt = st + u * 32 * ROWB;
-        const char* dt = qt + OFF_DO;
-        const char* tab = st + OFF_TAB + u * 128;
-        f32x16 s, dp;
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+      s = rows_dot(qt, roff, kf, s);
+      dp = rows_dot(dt, roff, vf, dp);
+      __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-        s = rows_dot(qt, roff, kf, s);
-        dp = rows_dot(dt, roff, vf, dp);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const char* at = tab + (8 * b + 4 * hh) * 4;
-          const f32x4 top = *reinterpret_cast<const f32x4*>(at + COL_MAX * COLB), D = *reinterpret_cast<const f32x4*>(at + COL_D * COLB);
-          f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, slope = {}, lo = {}, hi = {};
-          if constexpr (kInv) inv = *reinterpret_cast<const f32x4*>(at + COL_INV * COLB);
-          if constexpr (BIAS) {
-            pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
-            slope = *reinterpret_cast<const f32x4*>(at + COL_SLOPE * COLB);
-          }
-          if (!full) {
-            lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB);
-            hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * b + e;
-            float bent = 0.f, x;
-            if constexpr (CAP) {
-              bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
-              x = a.cap_out * bent;
-            } else {
-              x = s[i] * a.c;
-            }
-            if constexpr (BIAS) x = __builtin_fmaf(-slope[e], fabsf((float)(__float_as_int(pos[e]) - key)), x);
-            float p = __builtin_amdgcn_exp2f(x - top[e]);
-            if constexpr (kInv) p *= inv[e];
-            float ds = p * (dp[i] - D[e]);
-            if constexpr (CAP) ds *= 1.f - bent * bent;
-            if (!full) {
-              const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
-              p = rel < len ? p : 0.f;
-              ds = rel < len && len > 1 ? ds : 0.f;
-            }
-            s[i] = p;
-            dp[i] = ds;
-          }
+      for (int b = 0; b < 4; ++b) {
+        if constexpr (sizeof(T) == 4) asm volatile("" ::: "memory");  // (four rows of the table at a time)
+        const char* at = tab + (8 * b + 4 * hh) * 4;
+        const f32x4 top = *reinterpret_cast<const f32x4*>(at + COL_MAX * COLB), D = *reinterpret_cast<const f32x4*>(at + COL_D * COLB);
+        f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, slope = {}, lo = {}, hi = {};
+        if constexpr (kInv) inv = *reinterpret_cast<const f32x4*>(at + COL_INV * COLB);
+        if constexpr (BIAS) {
+          pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
+          slope = *reinterpret_cast<const f32x4*>(at + COL_SLOPE * COLB);
         }
-        if (careful && !full) {
-          const auto sees = [&](int w) {
-            const int lo = *reinterpret_cast<const int*>(tab + COL_LO * COLB + w * 4), hi = *reinterpret_cast<const int*>(tab + COL_HI * COLB + w * 4);
-            return (unsigned)(key - lo) < (unsigned)(hi - lo);
-          };
-          cols_dot_careful<T>(dt, s, lane, dv, sees);
-          cols_dot_careful<T>(qt, dp, lane, dk, sees);
-        } else {
-          cols_dot(dt, coff, s, dv);
-          cols_dot(qt, coff, dp, dk);
+        if (!full) {
+          lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB);
+          hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * b + e;
+          float bent = 0.f, x;
+          if constexpr (CAP) {
+            bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
+            x = a.cap_out * bent;
+          } else {
+            x = s[i] * a.c;
+          }
+          if constexpr (BIAS) x = __builtin_fmaf(-slope[e], fabsf((float)(__float_as_int(pos[e]) - key)), x);
+          float p = __builtin_amdgcn_exp2f(x - top[e]);
+          if constexpr (kInv) p *= inv[e];
+          float ds = p * (dp[i] - D[e]);
+          if constexpr (CAP) ds *= 1.f - bent * bent;
+          if (!full) {
+            const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
+            p = rel < len ? p : 0.f;
+            ds = rel < len && len > 1 ? ds : 0.f;
+          }
+          s[i] = p;
+          dp[i] = ds;
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      cols_dot(dt, coff, s, dv);
+      cols_dot(qt, coff, dp, dk);
     }
-    if (careful) break;
-    const float probe = not_finite(dk) + not_finite(dv);
-    if (!__syncthreads_or(key < a.k_rows && probe != probe)) break;
-    careful = true;
   }
   __syncthreads();
   const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
-  const unsigned long long good = __ballot(key < a.k_rows && (owned || a.fill));
+  const float probe = swap_sum(not_finite(dk) + not_finite(dv));
+  const bool again = owned && key < a.k_rows && probe != probe;
+  const unsigned long long good = __ballot(key < a.k_rows && (owned || a.fill) && !again);
   char* patch = smem + wave * 32 * ROWB;
-  store_rows<T>(patch, dk, a.scale, lane, good, [&](int w) { return a.dk + (long)(kw + w) * a.dk_row + head * a.dk_head; });
-  store_rows<T>(patch, dv, 1.f, lane, good, [&](int w) { return a.dv + (long)(kw + w) * a.dv_row + head * a.dv_head; });
+  store_rows<T>(patch, dk, owned ? a.scale : 0.f, lane, good, [&](int w) { return a.dk + (long)(kw + w) * a.dk_row + head * a.dk_head; });
+  store_rows<T>(patch, dv, owned ? 1.f : 0.f, lane, good, [&](int w) { return a.dv + (long)(kw + w) * a.dv_row + head * a.dv_head; });
+  unsigned bad = (unsigned)__ballot(again);
+  while (bad) {
+    const int w = __builtin_ctz(bad);
+    bad &= bad - 1;
+    key_grad_again<T, CAP, BIAS>(a, head, kw + w, r_lo, r_hi, lane);
+  }
 }
 
 // d_slopes[h] = sum over the rows of head h, in an order that depends on the number of rows alone
