@@ -162,23 +162,39 @@ __device__ __forceinline__ void lds_dma(const char* src, char* dst) {
 }
 
 // ROWS rows of 64 values, `stride` bytes apart from `base` on (wave-uniform; the rows behind the first n repeat row n - 1), into the LDS tile
-// at dst: 1 KiB pieces, dealt to the NW waves.  32-bit lane offsets on a uniform base; the lane number is hidden from the compiler so that
-// a dozen instructions per tile are spent instead of registers that live through the kernel.
-template <typename T, int ROWS, int NW>
-__device__ __forceinline__ void stage_rows(char* dst, const char* base, unsigned stride, int n, int wave, int lane) {
-  constexpr int PIECE = Tile<T>::kPiece, CH = 64 / PIECE, NP = ROWS / PIECE;
-  static_assert(NP % NW == 0, "every wave brings the same number of pieces");
-  asm volatile("" : "+v"(lane));
-  const unsigned in = lane / CH, pc = (lane % CH ^ Tile<T>::swizzle(in)) << 4;
-  const unsigned at = in * stride;
-#pragma unroll
-  for (int j = 0; j < NP / NW; ++j) {
-    const unsigned piece = wave + j * NW;
-    const unsigned turn = sizeof(T) == 2 ? (piece & 1) << 4 : (piece & 1) << 7 | (piece & 2) << 5;  // the row bits above the piece's
-    const unsigned off = n >= ROWS ? at + piece * PIECE * stride : min(piece * PIECE + in, (unsigned)(n - 1)) * stride;
-    lds_dma(base + (off + (pc ^ turn)), dst + piece * 1024);
+// at dst: 1 KiB pieces, dealt to the NW waves.  A piece's source is a uniform base plus a lane offset (row in the piece, swizzled chunk) that
+// is the same for every piece of the wave (NW = 4) or turned by a constant.
+template <typename T, int NW>
+struct Stager {
+  static constexpr int PIECE = Tile<T>::kPiece, CH = 64 / PIECE;
+  unsigned in, chunk, off;  // row and source chunk (in bytes) of the lane in the wave's first piece; both as one offset
+  __device__ __forceinline__ static unsigned turn(unsigned piece) {  // what the row bits above the piece's own do to the chunk
+    return sizeof(T) == 2 ? (piece & 1) << 4 : (piece & 1) << 7 | (piece & 2) << 5;
   }
-}
+  __device__ __forceinline__ void init(unsigned stride, int wave, int lane) {
+    in = lane / CH;
+    chunk = (lane % CH ^ Tile<T>::swizzle(in)) << 4 ^ turn(wave);
+    off = in * stride + chunk;
+  }
+  template <int ROWS>
+  __device__ __forceinline__ void rows(char* dst, const char* base, unsigned stride, int n, int wave) const {
+    constexpr int NP = ROWS / PIECE;
+    static_assert(NP % NW == 0 && (NW == 1 || NW % 4 == 0), "every wave brings the same number of pieces, all with the same turn");
+    dst += wave * 1024;
+    if (n >= ROWS) {
+      base += (unsigned)wave * PIECE * stride;
+      unsigned turned = chunk;
+      if constexpr (NW == 1) asm volatile("" : "+v"(turned));  // (formed here, not kept through the kernel)
+#pragma unroll
+      for (int j = 0; j < NP / NW; ++j)
+        lds_dma(base + (unsigned)(j * NW * PIECE) * stride + (NW == 1 ? off - chunk + (turned ^ turn(j)) : off), dst + j * NW * 1024);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NP / NW; ++j)
+        lds_dma(base + (min((wave + j * NW) * PIECE + in, (unsigned)(n - 1)) * stride + (NW == 1 ? chunk ^ turn(j) : chunk)), dst + j * NW * 1024);
+    }
+  }
+};
 
 // which of the lane's 16 scores in a tile of 32 keys (key 8 b + 4 hh + e of the tile) lie in [lo, hi) of the tile: bit 4 b + e
 __device__ __forceinline__ unsigned visible_bits(int lo, int hi, int hh) {
@@ -186,9 +202,9 @@ __device__ __forceinline__ unsigned visible_bits(int lo, int hi, int hh) {
   const int ca = (a >> 3) * 4 + min(a & 7, 4), cb = (b >> 3) * 4 + min(b & 7, 4);
   return ((1u << cb) - 1) & ~((1u << ca) - 1);
 }
-// x where bit i is set, else `other` (two instructions, no comparison)
+// x where bit i is set, else `other`: a bit field and a bitwise select (a comparison would cost its wait states on top)
 __device__ __forceinline__ float pick(unsigned bits, int i, float x, float other) {
-  const unsigned m = (unsigned)((int)(bits << (31 - i)) >> 31);
+  const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)bits, i, 1);
   return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
 }
 

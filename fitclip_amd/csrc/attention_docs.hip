@@ -100,11 +100,14 @@ attention_docs_kernel(const Args a) {
 
   const char* kbase = a.k + head * a.k_head;
   const char* vbase = a.v + head * a.v_head;
+  Stager<T, NW> kin, vin;
+  kin.init((unsigned)a.k_row, wave, lane);
+  vin.init((unsigned)a.v_row, wave, lane);
   auto stage = [&](int t) {
     char* dst = smem + (t & 1) * STAGE;
     const long first = kbeg + t * TK;
-    stage_rows<T, TK, NW>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave, lane);
-    stage_rows<T, TK, NW>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave, lane);
+    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave);
+    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave);
   };
 
   RowOff<T> koff;
@@ -149,6 +152,7 @@ attention_docs_kernel(const Args a) {
         s[u][i] = x;
       }
     if (!full) {
+      __builtin_amdgcn_sched_barrier(0);  // (the masks are formed here, not kept through the products)
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const unsigned bits = visible_bits(row.lo - k0 - 32 * u, row.hi - k0 - 32 * u, hh);

@@ -68,7 +68,7 @@ __device__ void row_grad_again(const Args& a, int head, int m, int lo, int hi, i
     const int key = min(j + lane, hi - 1);
     const float raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
     float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - top) * inv;
-    const float g = hi - lo == 1 ? D : row_dot<T>(vb + key * a.v_row, go);
+    const float g = row_dot<T>(vb + key * a.v_row, go);
     if (j + lane >= hi) p = 0.f;
     pd = __builtin_fmaf(p, g, pd);
     pf = __builtin_fmaf(p, far, pf);
@@ -77,7 +77,7 @@ __device__ void row_grad_again(const Args& a, int head, int m, int lo, int hi, i
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
   }
-  put_at<T>(a.dq + token * a.dq_row + qh * a.dq_head, lane, o * a.scale);
+  put_at<T>(a.dq + token * a.dq_row + qh * a.dq_head, lane, hi - lo > 1 ? o * a.scale : 0.f);
   if constexpr (BIAS) {
     pd = wave_sum(pd);
     pf = wave_sum(pf);
@@ -199,11 +199,14 @@ docs_grad_rows_kernel(const Args a) {
 
   const char* kbase = a.k + head * a.k_head;
   const char* vbase = a.v + head * a.v_head;
+  Stager<T, NW> kin, vin;
+  kin.init((unsigned)a.k_row, wave, lane);
+  vin.init((unsigned)a.v_row, wave, lane);
   auto stage = [&](int t) {
     char* dst = smem + (t & 1) * STAGE;
     const long first = kbeg + t * TK;
-    stage_rows<T, TK, NW>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave, lane);
-    stage_rows<T, TK, NW>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave, lane);
+    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave);
+    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave);
   };
   RowOff<T> roff;
   roff.init(r, hh);
@@ -251,11 +254,8 @@ docs_grad_rows_kernel(const Args a) {
         if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
         float p = __builtin_amdgcn_exp2f(x - top);
         if constexpr (sizeof(T) == 4) p *= inv;
-        float g = dp[i];
-        if (!full) {
-          p = pick(bits, i, p, 0.f);
-          g = pick(bits, i, row.hi - row.lo == 1 ? D : g, 0.f);  // one key: P = 1 whatever its score
-        }
+        if (!full) p = pick(bits, i, p, 0.f);  // (a NaN of a masked key then shows in the result: see row_grad_again)
+        const float g = dp[i];
         if constexpr (BIAS) {
           const float y = p * g;
           pd += y;
@@ -264,7 +264,6 @@ docs_grad_rows_kernel(const Args a) {
         }
         float ds = p * (g - D);
         if constexpr (CAP) ds *= 1.f - bent * bent;
-        if (!full) ds = pick(bits, i, ds, 0.f);
         s[i] = ds;
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -280,7 +279,8 @@ docs_grad_rows_kernel(const Args a) {
     if (hh == 0 && m0 + r < a.rows_pad && !again) column(a, COL_DSLOPE, head)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
   }
   __syncthreads();  // (the patches reuse the stages)
-  store_rows<T>(smem + wave * 32 * ROWB, o, row.valid ? a.scale : 0.f, lane, __ballot(row.valid ? !again : a.fill && m0 + r < a.rows), [&](int w) {
+  // (a row that sees one key: its weight is 1 whatever the score)
+  store_rows<T>(smem + wave * 32 * ROWB, o, row.hi - row.lo > 1 ? a.scale : 0.f, lane, __ballot(row.valid ? !again : a.fill && m0 + r < a.rows), [&](int w) {
     const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
     return a.dq + tk * a.dq_row + h * a.dq_head;
   });
@@ -421,8 +421,8 @@ docs_grad_keys_kernel(const Args a) {
           if constexpr (CAP) ds *= 1.f - bent * bent;
           if (!full) {
             const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
+            ds = rel < len && len > 1 ? ds : 0.f;  // (one key: its weight is 1 whatever the score)
             p = rel < len ? p : 0.f;
-            ds = rel < len && len > 1 ? ds : 0.f;
           }
           s[i] = p;
           dp[i] = ds;
