@@ -54,7 +54,8 @@ struct Args {
   float* stats;                                         // [q_rows][heads] (maximum in log2 units, sum of 2^(score - maximum))
   float* part;                                          // split over keys: [splits][kv_heads][rows][64] and behind it [..][2]
   int tiles, splits;
-  // gradients
+  // gradients: a kernel row is a row of ONE query head there (group 1), `share` query heads read a key head
+  int share;
   const char* d_out;
   long do_row, do_head;
   char *dq, *dk, *dv;
@@ -400,6 +401,63 @@ __device__ __forceinline__ void store_rows(char* patch, const f32x16 (&o)[2], fl
     const f32x4 y = *reinterpret_cast<const f32x4*>(patch + w * ROWB + ((ch ^ (sizeof(T) == 4 ? w & 15 : (w >> 1) & 7)) << 4));
     if (good >> w & 1) *reinterpret_cast<f32x4*>(at(w) + ch * 16) = y;
   }
+}
+
+// The KS waves of a workgroup hold shares of the same 32 rows: adds o * by over them, in order.  Wave w gets rows 8 w .. 8 w + 7 of the sum: lane l
+// row 8 w + l / 8, values 8 (l % 8) .. + 7.  `mine`: the wave's own 8 KiB of LDS, `stride` bytes apart from wave to wave.
+template <int KS>
+__device__ __forceinline__ void sum_waves(char* smem, int stride, const f32x16 (&o)[2], float by, int wave, int lane, f32x4 (&y)[2]) {
+  static_assert(KS == 4, "eight rows per wave");
+  const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *reinterpret_cast<f32x4*>(smem + wave * stride + r * 256 + (((8 * n + 2 * b + hh) ^ (r & 15)) << 4)) =
+          f32x4{o[n][4 * b] * by, o[n][4 * b + 1] * by, o[n][4 * b + 2] * by, o[n][4 * b + 3] * by};
+  __syncthreads();
+  const int row = 8 * wave + (lane >> 3);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    y[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < KS; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(smem + w * stride + row * 256 + (((2 * (lane & 7) + c) ^ (row & 15)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[c][e] += x[e];
+    }
+  }
+}
+// the eight values of sum_waves, times `by` (0: exactly 0), to the row at dst
+template <typename T>
+__device__ __forceinline__ void store_eight(char* dst, const f32x4 (&y)[2], float by, int lane) {
+  f32x4 z[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[c][e] = by == 0.f ? 0.f : y[c][e] * by;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(dst + 32 * (lane & 7)) = z[0];
+    *reinterpret_cast<f32x4*>(dst + 32 * (lane & 7) + 16) = z[1];
+  } else {
+    bf16x8 w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<bf16>(z[e >> 2][e & 3]);
+    *reinterpret_cast<bf16x8*>(dst + 16 * (lane & 7)) = w;
+  }
+}
+// which of the wave's eight rows hold a value that is not finite (bit k: row 8 w + k)
+__device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool counts) {
+  float x = 0.f;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x = __builtin_fmaf(y[c][e], 0.f, x);
+  const unsigned long long b = __ballot(counts && x != x);
+  unsigned rows = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) rows |= (unsigned)((b >> (8 * k) & 0xff) != 0) << k;
+  return rows;
 }
 
 #endif  // __HIPCC__

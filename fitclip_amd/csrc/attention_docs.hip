@@ -1,12 +1,14 @@
 // Attention over packed documents, forward (attention_docs.h: the formulas, the masks, the tiles).
 //
-// One workgroup: NW waves x 32 kernel rows of one key head; K and V stream through LDS in tiles of TK keys between the lowest and the
-// highest key that any of its rows sees.  S^T = K . Q^T puts a row's scores into two lanes (r, r + 32): its running maximum and sum need one
-// lane swap, and the exponentiated accumulator IS the operand of O^T = V^T . P^T.  A wave skips tiles that none of its rows sees and masks
-// only tiles that one of them sees in part.
+// S^T = K . Q^T puts a row's scores into two lanes (r, r + 32): its running maximum and sum need one lane swap, and the exponentiated
+// accumulator IS the operand of O^T = V^T . P^T.  K and V stream through LDS in tiles between the lowest and the highest key that a row of
+// the workgroup sees; a wave skips tiles that none of its 32 rows sees and masks only tiles that one of them sees in part.
 //
-// Few rows over many keys (single tokens that are being written): the key range is cut into `splits` parts, each part leaves its
-// unnormalised O with (maximum, sum) in scratch, and a second kernel joins them in a fixed order.
+// Two shapes of a workgroup of four waves.  Many rows: 4 x 32 rows share every tile of 64 keys (a quarter of the traffic from L2).  Fewer:
+// the four waves hold the SAME 32 rows, each takes every fourth tile of 32 keys into its own LDS, and their (maximum, sum, O) are joined at
+// the end - four times the waves and a quarter of the longest wave's work, with no barrier in the loop.
+// Few rows over many keys (single tokens that are being written): the key range is cut into `splits` parts on top of that, each part leaves
+// its unnormalised O with (maximum, sum) in scratch, and a second kernel joins them in a fixed order.
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -14,8 +16,6 @@
 namespace fc {
 namespace docs {
 namespace {
-
-template <typename T> constexpr int stage_bytes(int tk) { return 2 * tk * Tile<T>::kRow; }
 
 // One kernel row again, key by key (64 lanes = 64 keys for the scores, 64 dimensions for the sums), over keys [lo, hi).
 template <typename T, bool CAP, bool BIAS>
@@ -47,21 +47,21 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
   if (lane == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{top, l};
 }
 
-template <typename T, int NW, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 3)))
+template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? (KS > 1 ? 1 : 2) : KS > 1 ? 2 : 3)))
 attention_docs_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, STAGE = stage_bytes<T>(TK);  // K rows, then V rows
-  static_assert(NW * 32 * ROWB <= 2 * STAGE, "the output patches reuse the stages");
-  constexpr int NT = TK / 32;
+  constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
+  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int range[2 * NW];
+  __shared__ int range[2 * RW];
+  __shared__ float shares[KS > 1 ? KS : 1][2][32];
 
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // key head fastest (one XCD then works on few heads: K and V stay in its L2), later rows first (causal: they cost most)
   const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
   const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
-  const int m0 = (tile * NW + wave) * 32;
+  const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
   const Row row = find_row(a, m0, lane);
   const bool sees = row.lo < row.hi;
@@ -70,16 +70,16 @@ attention_docs_kernel(const Args a) {
   const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);
   const int full_hi = wave_min_i(row.valid ? (sees ? row.hi : -INT_MAX) : INT_MAX);
   int kbeg = wlo, kend = whi;
-  if constexpr (NW > 1) {
+  if constexpr (RW > 1) {
     if (lane == 0) {
       range[wave] = wlo;
-      range[NW + wave] = whi;
+      range[RW + wave] = whi;
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < RW; ++w) {
       kbeg = min(kbeg, range[w]);
-      kend = max(kend, range[NW + w]);
+      kend = max(kend, range[RW + w]);
     }
     kbeg = __builtin_amdgcn_readfirstlane(kbeg);
     kend = __builtin_amdgcn_readfirstlane(kend);
@@ -100,14 +100,17 @@ attention_docs_kernel(const Args a) {
 
   const char* kbase = a.k + head * a.k_head;
   const char* vbase = a.v + head * a.v_head;
-  Stager<T, NW> kin, vin;
-  kin.init((unsigned)a.k_row, wave, lane);
-  vin.init((unsigned)a.v_row, wave, lane);
-  auto stage = [&](int t) {
-    char* dst = smem + (t & 1) * STAGE;
+  constexpr int SW = KS > 1 ? 1 : RW;  // waves that bring a tile together
+  const int sw = KS > 1 ? 0 : wave;
+  Stager<T, SW> kin, vin;
+  kin.init((unsigned)a.k_row, sw, lane);
+  vin.init((unsigned)a.v_row, sw, lane);
+  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  auto stage = [&](int t, int buf) {
+    char* dst = stages + buf * STAGE;
     const long first = kbeg + t * TK;
-    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave);
-    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave);
+    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, sw);
+    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, sw);
   };
 
   RowOff<T> koff;
@@ -121,14 +124,15 @@ attention_docs_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
   float mref = -kInf, mtop = -kInf, l = 0.f;  // the maximum that the sums refer to (it follows the true one in steps of 2^8), the true one
-  if (t_first < t_last) stage(t_first);
-  for (int t = t_first; t < t_last; ++t) {
+  int t = t_first + (KS > 1 ? wave : 0), buf = 0;
+  if (t < t_last) stage(t, 0);
+  for (; t < t_last; t += KS, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
-    if (t + 1 < t_last) stage(t + 1);
+    if constexpr (KS == 1) __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
+    if (t + KS < t_last) stage(t + KS, buf ^ 1);
     const int k0 = kbeg + t * TK;
     if (k0 >= whi || k0 + TK <= wlo) continue;  // (wave-uniform)
-    const char* kt = smem + (t & 1) * STAGE;
+    const char* kt = stages + buf * STAGE;
     const char* vt = kt + TK * ROWB;
     const bool full = full_lo <= k0 && k0 + TK <= full_hi;
     f32x16 s[NT];
@@ -190,39 +194,76 @@ attention_docs_kernel(const Args a) {
     for (int u = 0; u < NT; ++u) cols_dot(vt + u * 32 * ROWB, voff, s[u], o);
   }
   l = swap_sum(l);
-  const float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
+  float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
   l *= down;
+  float2* const part_ml = reinterpret_cast<float2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64);
+  unsigned bad;  // rows to be done again: bit k = row bad0 + k
+  int bad0 = 0;
 
-  const float probe = swap_sum(not_finite(o));
-  const bool again = row.valid && probe != probe;
-
-  if (a.splits > 1) {
-    const long at = ((long)split * a.kv_heads + head) * a.rows + m0 + r;
-    if (m0 + r < a.rows && !again) {
-      float* po = a.part + at * 64;
+  if constexpr (KS == 1) {
+    const float probe = swap_sum(not_finite(o));
+    const bool again = row.valid && probe != probe;
+    if (a.splits > 1) {
+      const long at = ((long)split * a.kv_heads + head) * a.rows + m0 + r;
+      if (m0 + r < a.rows && !again) {
+        float* po = a.part + at * 64;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          *reinterpret_cast<f32x4*>(po + 32 * n + 8 * b + 4 * hh) =
-              f32x4{o[n][4 * b] * down, o[n][4 * b + 1] * down, o[n][4 * b + 2] * down, o[n][4 * b + 3] * down};
-      // (sum -1: a row of no document)
-      if (hh == 0) *reinterpret_cast<f32x2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64 + at * 2) = f32x2{mtop, row.valid ? l : -1.f};
+          for (int b = 0; b < 4; ++b)
+            *reinterpret_cast<f32x4*>(po + 32 * n + 8 * b + 4 * hh) =
+                f32x4{o[n][4 * b] * down, o[n][4 * b + 1] * down, o[n][4 * b + 2] * down, o[n][4 * b + 3] * down};
+        if (hh == 0) part_ml[at] = float2{mtop, row.valid ? l : -1.f};  // (sum -1: a row of no document)
+      }
+    } else {
+      const float inv = sees ? down / l : 0.f;
+      const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
+      if (hh == 0 && write)
+        *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
+      __syncthreads();  // (the patches reuse the stages)
+      store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
+        const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+        return a.out + tk * a.out_row + h * a.out_head;
+      });
     }
+    bad = (unsigned)__ballot(again);
   } else {
-    const float inv = sees ? down / l : 0.f;
-    const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
-    if (hh == 0 && write)
-      *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
-    __syncthreads();  // (the patches reuse the stages)
-    store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
-      const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
-      return a.out + tk * a.out_row + h * a.out_head;
-    });
+    if (hh == 0) {
+      shares[wave][0][r] = mtop;
+      shares[wave][1][r] = l;
+    }
+    __syncthreads();
+    float top = -kInf, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < KS; ++w) top = fmaxf(top, shares[w][0][r]);
+    const float ref = top == -kInf ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < KS; ++w) sum = __builtin_fmaf(shares[w][1][r], __builtin_amdgcn_exp2f(shares[w][0][r] - ref), sum);
+    down *= __builtin_amdgcn_exp2f(mtop - ref);
+    f32x4 y[2];
+    sum_waves<KS>(smem, 2 * STAGE, o, down, wave, lane, y);
+    bad0 = 8 * wave;
+    const int rr = bad0 + (lane >> 3), mr = m0 + rr;
+    const bool valid = __shfl((int)row.valid, rr, 64), see = __shfl((int)sees, rr, 64);
+    top = __shfl(top, rr, 64);
+    sum = __shfl(sum, rr, 64);
+    bad = bad_of_eight(y, valid);
+    const bool again = bad >> (lane >> 3) & 1, write = mr < a.rows && !again && (valid || a.fill || a.splits > 1);
+    if (a.splits > 1) {
+      const long at = ((long)split * a.kv_heads + head) * a.rows + mr;
+      if (write) {
+        store_eight<float>(reinterpret_cast<char*>(a.part + at * 64), y, 1.f, lane);
+        if ((lane & 7) == 0) part_ml[at] = float2{top, valid ? sum : -1.f};
+      }
+    } else if (write) {
+      const int tk = a.group.div(mr), h = head * (int)a.group.d + (mr - tk * (int)a.group.d);
+      store_eight<T>(a.out + tk * a.out_row + h * a.out_head, y, see ? 1.f / sum : 0.f, lane);
+      if ((lane & 7) == 0)
+        *reinterpret_cast<f32x2*>(a.stats + ((long)tk * a.kv_heads * (int)a.group.d + h) * 2) = f32x2{valid ? top : -kInf, valid ? sum : 0.f};
+    }
   }
-  unsigned bad = (unsigned)__ballot(again);
   while (bad) {
-    const int w = __builtin_ctz(bad);
+    const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
     const int lo = __builtin_amdgcn_readlane(row.lo, w), hi = __builtin_amdgcn_readlane(row.hi, w), pos = __builtin_amdgcn_readlane(row.pos, w);
     row_again<T, CAP, BIAS>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lo < hi, lane);
@@ -276,22 +317,21 @@ __global__ void __launch_bounds__(256) attention_docs_join_kernel(const Args a) 
 }
 
 struct Plan {
-  int waves, tiles, splits;
+  bool shared;  // four waves x 32 rows share tiles of keys; otherwise four waves share 32 rows and each takes every fourth tile of keys
+  int tiles, splits;
 };
 
-// Four waves (128 rows) share a tile of keys when that still gives every compute unit a workgroup; one wave alone otherwise.  Single
-// waves that are too few as well split the keys, as far as a part keeps 256 of them.
 Plan plan_forward(const fc_docs& d) {
   const long group = d.q_heads / d.kv_heads, rows = d.q_rows * group, cus = device_cus();
-  Plan p{4, (int)((rows + 127) / 128), 1};
-  if ((long)p.tiles * d.kv_heads >= cus) return p;
-  p.waves = 1;
+  Plan p{true, (int)((rows + 127) / 128), 1};
+  if ((long)p.tiles * d.kv_heads >= 2 * cus) return p;
+  p.shared = false;
   p.tiles = (int)((rows + 31) / 32);
   const long units = (long)p.tiles * d.kv_heads;
   // keys that a tile walks over, from the mean lengths: the documents that 32 kernel rows touch
   const double mean_rows = std::max(1.0, (double)rows / d.docs), mean_keys = (double)d.k_rows / d.docs;
   const double keys = std::min((double)d.k_rows, (32.0 / mean_rows + 1.0) * mean_keys);
-  p.splits = (int)std::max(1L, std::min({2 * cus / std::max(1L, units), (long)(keys / 256.0), 512L}));
+  p.splits = (int)std::max(1L, std::min({2 * cus / std::max(1L, units), (long)(keys / 512.0), 512L}));
   return p;
 }
 
@@ -299,15 +339,15 @@ size_t part_bytes(const fc_docs& d, const Plan& p) {
   return p.splits == 1 ? 0 : (size_t)p.splits * (d.q_heads * d.q_rows) * 66 * sizeof(float);
 }
 
-template <typename T, int NW, int TK, bool CAP, bool BIAS>
+template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
 int launch_forward(const Args& a, hipStream_t st) {
-  constexpr int lds = 2 * stage_bytes<T>(TK);
-  auto kern = attention_docs_kernel<T, NW, TK, CAP, BIAS>;
+  constexpr int lds = 2 * KS * 2 * TK * Tile<T>::kRow;
+  auto kern = attention_docs_kernel<T, RW, KS, TK, CAP, BIAS>;
   if (lds > 60 * 1024 && raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds) != hipSuccess)
     return fail(FC_ELAUNCH, "fc_attention_docs: cannot raise dynamic LDS");
   const long blocks = (long)a.tiles * a.splits * a.kv_heads;
   if (blocks > 0x7fffffffL) return fail(FC_EINVAL, "fc_attention_docs: grid of %ld workgroups", blocks);
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(NW * 64), lds, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(RW * KS * 64), lds, st, a);
   FC_CHECK_LAUNCH("fc_attention_docs");
   if (a.splits > 1) {
     const long n = (long)a.kv_heads * a.rows;
@@ -318,14 +358,14 @@ int launch_forward(const Args& a, hipStream_t st) {
 }
 
 template <typename T, bool CAP, bool BIAS>
-int launch_waves(const Args& a, int waves, hipStream_t st) {
-  return waves == 4 ? launch_forward<T, 4, 64, CAP, BIAS>(a, st) : launch_forward<T, 1, 32, CAP, BIAS>(a, st);
+int launch_waves(const Args& a, bool shared, hipStream_t st) {
+  return shared ? launch_forward<T, 4, 1, 64, CAP, BIAS>(a, st) : launch_forward<T, 1, 4, 32, CAP, BIAS>(a, st);
 }
 
 template <typename T>
-int launch_type(const Args& a, bool cap, int waves, hipStream_t st) {
-  if (a.slopes) return cap ? launch_waves<T, true, true>(a, waves, st) : launch_waves<T, false, true>(a, waves, st);
-  return cap ? launch_waves<T, true, false>(a, waves, st) : launch_waves<T, false, false>(a, waves, st);
+int launch_type(const Args& a, bool cap, bool shared, hipStream_t st) {
+  if (a.slopes) return cap ? launch_waves<T, true, true>(a, shared, st) : launch_waves<T, false, true>(a, shared, st);
+  return cap ? launch_waves<T, true, false>(a, shared, st) : launch_waves<T, false, false>(a, shared, st);
 }
 
 }  // namespace
@@ -349,8 +389,8 @@ int check_docs(const fc_docs* d, const char* what) {
   if ((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) ||
       ((d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head) * size & 15))
     return fail(FC_EINVAL, "%s: rows and heads must start on 16-byte boundaries", what);
-  if (d->k_row * size >= 1 << 25 || d->v_row * size >= 1 << 25)
-    return fail(FC_EINVAL, "%s: rows of k or v lie 32 MiB or more apart", what);
+  if (d->q_row * size >= 1 << 25 || d->k_row * size >= 1 << 25 || d->v_row * size >= 1 << 25)
+    return fail(FC_EINVAL, "%s: rows of q, k or v lie 32 MiB or more apart", what);
   return FC_OK;
 }
 
@@ -412,7 +452,7 @@ int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_
   a.part = (float*)scratch;
   a.tiles = p.tiles;
   a.splits = p.splits;
-  return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.waves, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.waves, st);
+  return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.shared, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.shared, st);
 }
 
 }  // extern "C"

@@ -6,11 +6,14 @@
 //   d slope_h = - sum dS |p_i - j| = - (sum_j P dP |p - j| - (sum_j P dP) (sum_j P |p - j|)) per row: every factor in fp32 (the D of a
 //   bf16 output is rounded)
 //
-// Two kernels, no atomics: every sum has one owner and a fixed order.
-//   rows: as the forward (a wave owns 32 kernel rows and walks over keys): dQ, and the row table that the other kernel reads.
-//   keys: a wave owns 32 keys (K and V in registers) and walks over the kernel rows that see them - all heads of the group, so the gradients
-//   of shared heads need no further sum: S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
+// Two kernels, no atomics: every sum has one owner and a fixed order.  A kernel row is a row of ONE query head here: 32 rows of a head lie at
+// one stride, and all sources are a uniform base plus a lane offset.
+//   rows: as the forward (32 rows per wave, tiles of keys): dQ, and the row table that the other kernel reads.
+//   keys: 32 keys per wave (K and V in registers), tiles of the rows that see them, one query head of the group after the other - the
+//   gradients of shared heads need no further sum.  S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
+// Both have the forward's two shapes: four waves x 32 rows (keys) that share tiles, or four waves that take turns over the tiles of the
+// same 32 and add up at the end - where there are few of them, and each has a long way.
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -19,13 +22,13 @@ namespace fc {
 namespace docs {
 namespace {
 
-// Row table in scratch, one array of rows_pad numbers per quantity and key head: what a kernel row needs to have its weights formed again
-enum Column : int { COL_MAX = 0, COL_D = 1, COL_LO = 2, COL_HI = 3, COL_INV = 4, COL_POS = 5, COL_SLOPE = 6, COL_DSLOPE = 7, COLS = 8 };
+// Row table in scratch, one array of rows_pad numbers per quantity and query head: what a row needs to have its weights formed again
+enum Column : int { COL_MAX = 0, COL_D = 1, COL_LO = 2, COL_HI = 3, COL_INV = 4, COL_POS = 5, COL_DSLOPE = 6, COLS = 7 };
 // (maximum; bf16: maximum + log2 sum, and no COL_INV; fp32: 1 / sum apart, so that the forward's P is formed exactly again)
-// and behind the columns four ints per 32 kernel rows and key head: lowest and highest key that one of them sees; the keys from .. to that ALL see
-__device__ __forceinline__ float* column(const Args& a, int c, int head) { return a.table + ((long)c * a.kv_heads + head) * a.rows_pad; }
-__device__ __forceinline__ int32_t* block_keys(const Args& a, int head, int block) {
-  return reinterpret_cast<int32_t*>(a.table + (long)COLS * a.kv_heads * a.rows_pad) + ((long)head * (a.rows_pad / 32) + block) * 4;
+// and behind the columns four ints per 32 rows: lowest and highest key that one of them sees; the keys from .. to that ALL of them see
+__device__ __forceinline__ float* column(const Args& a, int c, int qh) { return a.table + ((long)c * a.kv_heads * a.share + qh) * a.rows_pad; }
+__device__ __forceinline__ int32_t* block_keys(const Args& a, int block) {
+  return reinterpret_cast<int32_t*>(a.table + (long)COLS * a.kv_heads * a.share * a.rows_pad) + (long)block * 4;
 }
 
 __device__ __forceinline__ float dot(const RowFrag<bf16>& x, const RowFrag<bf16>& y) {
@@ -55,11 +58,11 @@ __device__ __forceinline__ float bent_by(const Args& a, float raw, float ds) {
   return ds;
 }
 
-// d_q of one kernel row again, key by key (see attention_docs.h)
+// d_q of one row again, key by key (see attention_docs.h)
 template <typename T, bool CAP, bool BIAS>
-__device__ void row_grad_again(const Args& a, int head, int m, int lo, int hi, int pos, float top, float inv, float D, int lane) {
-  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-  const float q = value_at<T>(a.q + token * a.q_row + qh * a.q_head, lane), go = value_at<T>(a.d_out + token * a.do_row + qh * a.do_head, lane);
+__device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int pos, float top, float inv, float D, int lane) {
+  const int head = qh / a.share;
+  const float q = value_at<T>(a.q + m * a.q_row + qh * a.q_head, lane), go = value_at<T>(a.d_out + m * a.do_row + qh * a.do_head, lane);
   const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
   const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
   float o = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f;
@@ -77,44 +80,42 @@ __device__ void row_grad_again(const Args& a, int head, int m, int lo, int hi, i
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
   }
-  put_at<T>(a.dq + token * a.dq_row + qh * a.dq_head, lane, hi - lo > 1 ? o * a.scale : 0.f);
+  put_at<T>(a.dq + m * a.dq_row + qh * a.dq_head, lane, hi - lo > 1 ? o * a.scale : 0.f);
   if constexpr (BIAS) {
     pd = wave_sum(pd);
     pf = wave_sum(pf);
     pdf = wave_sum(pdf);
-    if (lane == 0) column(a, COL_DSLOPE, head)[m] = hi - lo > 1 ? pd * pf - pdf : 0.f;
+    if (lane == 0) column(a, COL_DSLOPE, qh)[m] = hi - lo > 1 ? pd * pf - pdf : 0.f;
   }
 }
 
-// d_k and d_v of one key again, row by row (kernel rows r_lo .. r_hi - 1 hold those that see it)
+// d_k and d_v of one key again, row by row (rows r_lo .. r_hi - 1 hold those that see it)
 template <typename T, bool CAP, bool BIAS>
 __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r_hi, int lane) {
   const float k = value_at<T>(a.k + key * a.k_row + head * a.k_head, lane), v = value_at<T>(a.v + key * a.v_row + head * a.v_head, lane);
   float dk = 0.f, dv = 0.f;
 #pragma unroll 1
-  for (int i = r_lo; i < r_hi; i += 64) {
-    const int m = min(i + lane, r_hi - 1);
-    const int lo = __float_as_int(column(a, COL_LO, head)[m]), hi = __float_as_int(column(a, COL_HI, head)[m]);
-    const bool see = i + lane < r_hi && (unsigned)(key - lo) < (unsigned)(hi - lo);
-    const unsigned long long seen = __ballot(see);
-    if (!seen) continue;
-    const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-    const float raw = row_dot<T>(a.q + token * a.q_row + qh * a.q_head, k);
-    const float g = row_dot<T>(a.d_out + token * a.do_row + qh * a.do_head, v);
-    float far = 0.f, slope = 0.f;
-    if constexpr (BIAS) {
-      far = fabsf((float)(__float_as_int(column(a, COL_POS, head)[m]) - key));
-      slope = column(a, COL_SLOPE, head)[m];
-    }
-    float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, head)[m]);
-    if constexpr (sizeof(T) == 4) p *= column(a, COL_INV, head)[m];
-    const float ds = hi - lo == 1 ? 0.f : bent_by<T, CAP>(a, raw, p * (g - column(a, COL_D, head)[m]));
+  for (int qh = head * a.share; qh < (head + 1) * a.share; ++qh) {
+    const char *qb = a.q + qh * a.q_head, *db = a.d_out + qh * a.do_head;
+    const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
 #pragma unroll 1
-    for (int w = 0; w < 64; ++w) {
-      if (!(seen >> w & 1)) continue;
-      const int mw = i + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
-      dk = __builtin_fmaf(lane_value(ds, w), value_at<T>(a.q + tk * a.q_row + h * a.q_head, lane), dk);
-      dv = __builtin_fmaf(lane_value(p, w), value_at<T>(a.d_out + tk * a.do_row + h * a.do_head, lane), dv);
+    for (int i = r_lo; i < r_hi; i += 64) {
+      const int m = min(i + lane, r_hi - 1);
+      const int lo = __float_as_int(column(a, COL_LO, qh)[m]), hi = __float_as_int(column(a, COL_HI, qh)[m]);
+      const bool see = i + lane < r_hi && (unsigned)(key - lo) < (unsigned)(hi - lo);
+      const unsigned long long seen = __ballot(see);
+      if (!seen) continue;
+      const float raw = row_dot<T>(qb + m * a.q_row, k), g = row_dot<T>(db + m * a.do_row, v);
+      const float far = BIAS ? fabsf((float)(__float_as_int(column(a, COL_POS, qh)[m]) - key)) : 0.f;
+      float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, qh)[m]);
+      if constexpr (sizeof(T) == 4) p *= column(a, COL_INV, qh)[m];
+      const float ds = hi - lo == 1 ? 0.f : bent_by<T, CAP>(a, raw, p * (g - column(a, COL_D, qh)[m]));
+#pragma unroll 1
+      for (int w = 0; w < 64; ++w) {
+        if (!(seen >> w & 1)) continue;
+        dk = __builtin_fmaf(lane_value(ds, w), value_at<T>(qb + (long)(i + w) * a.q_row, lane), dk);
+        dv = __builtin_fmaf(lane_value(p, w), value_at<T>(db + (long)(i + w) * a.do_row, lane), dv);
+      }
     }
   }
   put_at<T>(a.dk + key * a.dk_row + head * a.dk_head, lane, dk * a.scale);
@@ -122,17 +123,18 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
 }
 
 // ------------------------------------------------------------------------------------------------------------------ rows
-template <typename T, int NW, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && KS > 1 ? 1 : 2)))
 docs_grad_rows_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;
-  static_assert(NW * 32 * ROWB <= 2 * STAGE, "the output patches reuse the stages");
+  constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
+  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int range[2 * NW];
+  __shared__ int range[2 * RW];
+  __shared__ float shares[KS > 1 ? KS : 1][3][32];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = blockIdx.x % a.kv_heads, tile = a.tiles - 1 - blockIdx.x / a.kv_heads;
-  const int m0 = (tile * NW + wave) * 32;
+  const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, tile = a.tiles - 1 - blockIdx.x / heads;
+  const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
   const Row row = find_row(a, m0, lane);
   const bool sees = row.lo < row.hi;
@@ -140,16 +142,16 @@ docs_grad_rows_kernel(const Args a) {
   const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);
   const int full_hi = wave_min_i(row.valid ? (sees ? row.hi : -INT_MAX) : INT_MAX);
   int kbeg = wlo, kend = whi;
-  if constexpr (NW > 1) {
+  if constexpr (RW > 1) {
     if (lane == 0) {
       range[wave] = wlo;
-      range[NW + wave] = whi;
+      range[RW + wave] = whi;
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < RW; ++w) {
       kbeg = min(kbeg, range[w]);
-      kend = max(kend, range[NW + w]);
+      kend = max(kend, range[RW + w]);
     }
     kbeg = __builtin_amdgcn_readfirstlane(kbeg);
     kend = __builtin_amdgcn_readfirstlane(kend);
@@ -157,17 +159,16 @@ docs_grad_rows_kernel(const Args a) {
   const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
 
   const int m = min(m0 + r, a.rows - 1);
-  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
   RowFrag<T> qf, dof;
-  qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
-  dof.load(a.d_out + token * a.do_row + qh * a.do_head, hh);
+  qf.load(a.q + m * a.q_row + qh * a.q_head, hh);
+  dof.load(a.d_out + m * a.do_row + qh * a.do_head, hh);
   float D;
   {
     RowFrag<T> of;
-    of.load(a.out + token * a.out_row + qh * a.out_head, hh);
+    of.load(a.out + m * a.out_row + qh * a.out_head, hh);
     D = swap_sum(dot(of, dof));
   }
-  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2);
+  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * heads + qh) * 2);
   // a row that sees nothing weighs nothing: its maximum is taken as +inf
   float top = sees ? st[0] : kInf, inv = sees ? 1.f / st[1] : 0.f;
   if constexpr (sizeof(T) == 2) {
@@ -176,37 +177,38 @@ docs_grad_rows_kernel(const Args a) {
   }
   if (!sees) D = 0.f;
   const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
-  if (hh == 0 && m0 + r < a.rows_pad) {
-    const int at = m0 + r;
-    column(a, COL_MAX, head)[at] = top;
-    column(a, COL_D, head)[at] = D;
-    column(a, COL_LO, head)[at] = __int_as_float(row.lo);
-    column(a, COL_HI, head)[at] = __int_as_float(row.hi);
-    if constexpr (sizeof(T) == 4) column(a, COL_INV, head)[at] = inv;
-    if constexpr (BIAS) {
-      column(a, COL_POS, head)[at] = __int_as_float(row.pos);
-      column(a, COL_SLOPE, head)[at] = slope;
+  if (KS == 1 || wave == 0) {
+    if (hh == 0) {  // (m0 + r < rows_pad)
+      column(a, COL_MAX, qh)[m0 + r] = top;
+      column(a, COL_D, qh)[m0 + r] = D;
+      column(a, COL_LO, qh)[m0 + r] = __int_as_float(row.lo);
+      column(a, COL_HI, qh)[m0 + r] = __int_as_float(row.hi);
+      if constexpr (sizeof(T) == 4) column(a, COL_INV, qh)[m0 + r] = inv;
+      if constexpr (BIAS) column(a, COL_POS, qh)[m0 + r] = __int_as_float(row.pos);
     }
-  }
-  const int all_lo = wave_max_i(sees ? row.lo : INT_MAX), all_hi = wave_min_i(sees ? row.hi : -INT_MAX);
-  if (lane == 0) {
-    int32_t* b = block_keys(a, head, m0 / 32);
-    b[0] = wlo;
-    b[1] = whi;
-    b[2] = all_lo;  // (here a row of no document asks for the mask too: its Q and dO may hold anything)
-    b[3] = all_hi;
+    const int all_lo = wave_max_i(sees ? row.lo : INT_MAX), all_hi = wave_min_i(sees ? row.hi : -INT_MAX);
+    if (lane == 0 && qh == 0) {
+      int32_t* b = block_keys(a, m0 / 32);
+      b[0] = wlo;
+      b[1] = whi;
+      b[2] = all_lo;  // (here a row of no document asks for the mask too: its Q and dO may hold anything)
+      b[3] = all_hi;
+    }
   }
 
   const char* kbase = a.k + head * a.k_head;
   const char* vbase = a.v + head * a.v_head;
-  Stager<T, NW> kin, vin;
-  kin.init((unsigned)a.k_row, wave, lane);
-  vin.init((unsigned)a.v_row, wave, lane);
-  auto stage = [&](int t) {
-    char* dst = smem + (t & 1) * STAGE;
+  constexpr int SW = KS > 1 ? 1 : RW;  // waves that bring a tile together
+  const int sw = KS > 1 ? 0 : wave;
+  Stager<T, SW> kin, vin;
+  kin.init((unsigned)a.k_row, sw, lane);
+  vin.init((unsigned)a.v_row, sw, lane);
+  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  auto stage = [&](int t, int buf) {
+    char* dst = stages + buf * STAGE;
     const long first = kbeg + t * TK;
-    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, wave);
-    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, wave);
+    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, sw);
+    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, sw);
   };
   RowOff<T> roff;
   roff.init(r, hh);
@@ -219,13 +221,14 @@ docs_grad_rows_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
   float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
-  if (ntile) stage(0);
-  for (int t = 0; t < ntile; ++t) {
+  int t = KS > 1 ? wave : 0, buf = 0;
+  if (t < ntile) stage(t, 0);
+  for (; t < ntile; t += KS, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < ntile) stage(t + 1);
+    if constexpr (KS == 1) __syncthreads();
+    if (t + KS < ntile) stage(t + KS, buf ^ 1);
     const int k0 = kbeg + t * TK;
-    const char* kt = smem + (t & 1) * STAGE;
+    const char* kt = stages + buf * STAGE;
     const char* vt = kt + TK * ROWB;
 #pragma unroll 1
     for (int u = 0; u < NT; ++u) {
@@ -270,51 +273,83 @@ docs_grad_rows_kernel(const Args a) {
       cols_dot(kt + u * 32 * ROWB, coff, s, o);
     }
   }
-  const float probe = swap_sum(not_finite(o));
-  const bool again = row.valid && probe != probe;
   if constexpr (BIAS) {
     pd = swap_sum(pd);
     pf = swap_sum(pf);
     pdf = swap_sum(pdf);
-    if (hh == 0 && m0 + r < a.rows_pad && !again) column(a, COL_DSLOPE, head)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
   }
-  __syncthreads();  // (the patches reuse the stages)
-  // (a row that sees one key: its weight is 1 whatever the score)
-  store_rows<T>(smem + wave * 32 * ROWB, o, row.hi - row.lo > 1 ? a.scale : 0.f, lane, __ballot(row.valid ? !again : a.fill && m0 + r < a.rows), [&](int w) {
-    const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
-    return a.dq + tk * a.dq_row + h * a.dq_head;
-  });
-  unsigned bad = (unsigned)__ballot(again);
+  unsigned bad;  // rows to be done again: bit k = row bad0 + k
+  int bad0 = 0;
+  if constexpr (KS == 1) {
+    const float probe = swap_sum(not_finite(o));
+    const bool again = row.valid && probe != probe;
+    if (BIAS && hh == 0 && !again) column(a, COL_DSLOPE, qh)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
+    __syncthreads();  // (the patches reuse the stages)
+    // (a row that sees one key: its weight is 1 whatever the score)
+    store_rows<T>(smem + wave * 32 * ROWB, o, row.hi - row.lo > 1 ? a.scale : 0.f, lane, __ballot(row.valid ? !again : a.fill && m0 + r < a.rows),
+                  [&](int w) { return a.dq + (long)(m0 + w) * a.dq_row + qh * a.dq_head; });
+    bad = (unsigned)__ballot(again);
+  } else {
+    if constexpr (BIAS) {
+      if (hh == 0) {
+        shares[wave][0][r] = pd;
+        shares[wave][1][r] = pf;
+        shares[wave][2][r] = pdf;
+      }
+    }
+    f32x4 y[2];
+    sum_waves<KS>(smem, 2 * STAGE, o, 1.f, wave, lane, y);  // (with a barrier inside)
+    bad0 = 8 * wave;
+    const int rr = bad0 + (lane >> 3), mr = m0 + rr;
+    const bool valid = __shfl((int)row.valid, rr, 64), many = __shfl(row.hi - row.lo, rr, 64) > 1;
+    bad = bad_of_eight(y, valid);
+    const bool again = bad >> (lane >> 3) & 1;
+    if (mr < a.rows && !again) {
+      if (valid || a.fill) store_eight<T>(a.dq + (long)mr * a.dq_row + qh * a.dq_head, y, many ? a.scale : 0.f, lane);
+      if constexpr (BIAS) {
+        if ((lane & 7) == 0) {
+          pd = pf = pdf = 0.f;
+#pragma unroll
+          for (int w = 0; w < KS; ++w) {
+            pd += shares[w][0][rr];
+            pf += shares[w][1][rr];
+            pdf += shares[w][2][rr];
+          }
+          column(a, COL_DSLOPE, qh)[mr] = many ? pd * pf - pdf : 0.f;
+        }
+      }
+    }
+  }
   while (bad) {
-    const int w = __builtin_ctz(bad);
+    const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
-    row_grad_again<T, CAP, BIAS>(a, head, m0 + w, __builtin_amdgcn_readlane(row.lo, w), __builtin_amdgcn_readlane(row.hi, w),
+    row_grad_again<T, CAP, BIAS>(a, qh, m0 + w, __builtin_amdgcn_readlane(row.lo, w), __builtin_amdgcn_readlane(row.hi, w),
                                  __builtin_amdgcn_readlane(row.pos, w), lane_value(top, w), lane_value(inv, w), lane_value(D, w), lane);
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ keys
-template <typename T, int NW, int TQ, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+template <typename T, int KW, int KS, int TQ, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(KW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && KS > 1 ? 1 : 2)))
 docs_grad_keys_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, PIECE = Tile<T>::kPiece;
+  constexpr int ROWB = Tile<T>::kRow;
   constexpr int OFF_DO = TQ * ROWB, OFF_TAB = 2 * TQ * ROWB;
   constexpr bool kInv = sizeof(T) == 4;
-  constexpr int NTAB = BIAS ? 7 : kInv ? 5 : 4;           // columns of the row table that come along (in the order of Column)
-  constexpr int COLB = 256;                               // a column's share of a stage: 64 numbers, of which TQ count
-  constexpr int STAGE = OFF_TAB + 7 * COLB;
-  constexpr int NROW = 2 * TQ / PIECE, NP = NROW + NTAB;  // pieces: 1 KiB of Q, then of dO; 64 numbers of a column
-  static_assert(NW * 32 * ROWB <= 2 * STAGE, "patches");
+  constexpr int NTAB = BIAS ? 6 : kInv ? 5 : 4;           // columns of the row table that come along (in the order of Column)
+  constexpr int COLB = TQ * 4;                            // a column's share of a stage
+  constexpr int OFF_KEYS = OFF_TAB + 6 * COLB;            // the blocks' four ints
+  constexpr int STAGE = OFF_KEYS + 64;
+  static_assert((KS == 1 && KW * 32 * ROWB <= 2 * STAGE) || (KW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;  // (earlier keys first: causal, they cost most)
-  const int k0 = tile * NW * 32, kw = k0 + wave * 32;
+  const int k0 = tile * KW * 32, kw = k0 + (KS > 1 ? 0 : wave * 32);
 
-  // kernel rows of the documents that own keys k0 .. k0 + 32 NW - 1; causal: in the first of them from the first row that sees k0
+  // rows of the documents that own keys k0 .. k0 + 32 KW - 1; causal: in the first of them from the first row that sees k0
   int r_lo, r_hi;
   {
-    const int last = min(k0 + NW * 32, a.k_rows) - 1;
+    const int last = min(k0 + KW * 32, a.k_rows) - 1;
     const int d0 = min(max(wave_count_le(a.k_off, a.docs + 1, k0, lane) - 1, 0), a.docs - 1);
     const int d1 = min(max(wave_count_le(a.k_off, a.docs + 1, last, lane) - 1, d0), a.docs - 1);
     const int qs = min(max(a.q_off[d0], 0), a.q_rows), qe = min(max(a.q_off[d0 + 1], qs), a.q_rows);
@@ -324,10 +359,10 @@ docs_grad_keys_kernel(const Args a) {
       const int j = k0 - ks;
       if (!(a.prefix && a.prefix[d0] > j)) skip = min(max(j - (ke - ks) + (qe - qs), 0), qe - qs);
     }
-    r_lo = (qs + skip) * (int)a.group.d;
-    r_hi = min(max(a.q_off[d1 + 1], 0), a.q_rows) * (int)a.group.d;
+    r_lo = qs + skip;
+    r_hi = min(max(a.q_off[d1 + 1], 0), a.q_rows);
   }
-  const int t_first = r_lo / TQ, t_last = r_hi > r_lo ? (r_hi + TQ - 1) / TQ : t_first;
+  const int t_first = r_lo / TQ, steps = r_hi > r_lo ? (r_hi + TQ - 1) / TQ - t_first : 0;  // tiles of rows, for each query head of the group
 
   const int key = kw + r;
   const long kc = min(key, a.k_rows - 1);
@@ -335,26 +370,27 @@ docs_grad_keys_kernel(const Args a) {
   kf.load(a.k + kc * a.k_row + head * a.k_head, hh);
   vf.load(a.v + kc * a.v_row + head * a.v_head, hh);
 
-  auto stage = [&](int t) {
-    char* dst = smem + (t & 1) * STAGE;
-    int ln = lane;
-    asm volatile("" : "+v"(ln));  // (addresses are formed here, not kept through the kernel)
-    const int in = ln / (64 / PIECE), pc = ln % (64 / PIECE);
-#pragma unroll 2
-    for (int j = 0; j < (NP + NW - 1) / NW; ++j) {
-      const int piece = wave + j * NW;
-      if (piece < NROW) {
-        const int isd = piece >= NROW / 2, w = (isd ? piece - NROW / 2 : piece) * PIECE + in;
-        const int m = min(t * TQ + w, a.rows - 1);
-        const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-        lds_dma((isd ? a.d_out + token * a.do_row + qh * a.do_head : a.q + token * a.q_row + qh * a.q_head) +
-                    ((pc ^ Tile<T>::swizzle(w)) << 4), dst + piece * 1024);
-      } else if (piece < NP) {
-        const int c = piece - NROW;
-        if (c != COL_INV || kInv)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(column(a, c, head) + (long)t * TQ + lane),
+  constexpr int SW = KS > 1 ? 1 : KW;  // waves that bring a tile together
+  const int sw = KS > 1 ? 0 : wave;
+  Stager<T, SW> qin, din;
+  qin.init((unsigned)a.q_row, sw, lane);
+  din.init((unsigned)a.do_row, sw, lane);
+  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  auto stage = [&](int qh, int t, int buf) {
+    char* dst = stages + buf * STAGE;
+    const long first = (long)t * TQ;
+    const int n = a.rows - t * TQ;
+    qin.template rows<TQ>(dst, a.q + first * a.q_row + qh * a.q_head, (unsigned)a.q_row, n, sw);
+    din.template rows<TQ>(dst + OFF_DO, a.d_out + first * a.do_row + qh * a.do_head, (unsigned)a.do_row, n, sw);
+    if (lane < TQ) {  // (a column is rows_pad long: whole tiles)
+#pragma unroll
+      for (int c = 0; c < NTAB; ++c)
+        if ((SW == 1 || c % SW == sw) && (c != COL_INV || kInv))
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(column(a, c, qh) + first + lane),
                                            (__attribute__((address_space(3))) void*)(dst + OFF_TAB + c * COLB), 4, 0, 0);
-      }
+      if (lane < 4 * (TQ / 32) && (SW == 1 || sw == SW - 1))
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(block_keys(a, t * (TQ / 32)) + lane),
+                                         (__attribute__((address_space(3))) void*)(dst + OFF_KEYS), 4, 0, 0);
     }
   };
   RowOff<T> roff;
@@ -367,19 +403,34 @@ docs_grad_keys_kernel(const Args a) {
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
-  if (t_first < t_last) stage(t_first);
-  for (int t = t_first; t < t_last; ++t) {
+  int g = 0, t = KS > 1 ? wave : 0, buf = 0;  // query head of the group, tile of rows
+  const int all = steps ? a.share : 0;
+  auto settle = [&](int& g, int& t) {
+    while (t >= steps && g < all) {
+      t -= steps;
+      ++g;
+    }
+  };
+  settle(g, t);
+  if (g < all) stage(head * a.share + g, t_first + t, 0);
+  while (g < all) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < t_last) stage(t + 1);
-    const char* st = smem + (t & 1) * STAGE;
+    if constexpr (KS == 1) __syncthreads();
+    const int now = t_first + t;
+    const float slope = BIAS ? a.slopes[head * a.share + g] * kLog2e : 0.f;
+    t += KS;
+    settle(g, t);
+    if (g < all) stage(head * a.share + g, t_first + t, buf ^ 1);
+    const char* st = stages + buf * STAGE;
+    buf ^= 1;
 #pragma unroll 1
     for (int u = 0; u < TQ / 32; ++u) {
-      const int block = t * (TQ / 32) + u;
-      if (block * 32 >= a.rows) continue;
-      const int32_t* bk = block_keys(a, head, block);
-      if (kw >= bk[1] || kw + 32 <= bk[0]) continue;  // (wave-uniform)
-      const bool full = bk[2] <= kw && kw + 32 <= bk[3];
+      if ((now * (TQ / 32) + u) * 32 >= a.rows) continue;
+      const int bl = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16));
+      const int bh = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 4));
+      if (kw >= bh || kw + 32 <= bl) continue;  // (wave-uniform)
+      const bool full = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 8)) <= kw &&
+                        kw + 32 <= __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 12));
       const char* qt = st + u * 32 * ROWB;
       const char* dt = qt + OFF_DO;
       const char* tab = st + OFF_TAB + u * 128;
@@ -394,12 +445,9 @@ docs_grad_keys_kernel(const Args a) {
         if constexpr (sizeof(T) == 4) asm volatile("" ::: "memory");  // (four rows of the table at a time)
         const char* at = tab + (8 * b + 4 * hh) * 4;
         const f32x4 top = *reinterpret_cast<const f32x4*>(at + COL_MAX * COLB), D = *reinterpret_cast<const f32x4*>(at + COL_D * COLB);
-        f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, slope = {}, lo = {}, hi = {};
+        f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, lo = {}, hi = {};
         if constexpr (kInv) inv = *reinterpret_cast<const f32x4*>(at + COL_INV * COLB);
-        if constexpr (BIAS) {
-          pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
-          slope = *reinterpret_cast<const f32x4*>(at + COL_SLOPE * COLB);
-        }
+        if constexpr (BIAS) pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
         if (!full) {
           lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB);
           hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
@@ -414,7 +462,7 @@ docs_grad_keys_kernel(const Args a) {
           } else {
             x = s[i] * a.c;
           }
-          if constexpr (BIAS) x = __builtin_fmaf(-slope[e], fabsf((float)(__float_as_int(pos[e]) - key)), x);
+          if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf((float)(__float_as_int(pos[e]) - key)), x);
           float p = __builtin_amdgcn_exp2f(x - top[e]);
           if constexpr (kInv) p *= inv[e];
           float ds = p * (dp[i] - D[e]);
@@ -433,44 +481,57 @@ docs_grad_keys_kernel(const Args a) {
       cols_dot(qt, coff, dp, dk);
     }
   }
-  __syncthreads();
   const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
-  const float probe = swap_sum(not_finite(dk) + not_finite(dv));
-  const bool again = owned && key < a.k_rows && probe != probe;
-  const unsigned long long good = __ballot(key < a.k_rows && (owned || a.fill) && !again);
-  char* patch = smem + wave * 32 * ROWB;
-  store_rows<T>(patch, dk, owned ? a.scale : 0.f, lane, good, [&](int w) { return a.dk + (long)(kw + w) * a.dk_row + head * a.dk_head; });
-  store_rows<T>(patch, dv, owned ? 1.f : 0.f, lane, good, [&](int w) { return a.dv + (long)(kw + w) * a.dv_row + head * a.dv_head; });
-  unsigned bad = (unsigned)__ballot(again);
+  unsigned bad;  // keys to be done again: bit k = key kw + bad0 + k
+  int bad0 = 0;
+  if constexpr (KS == 1) {
+    __syncthreads();  // (the patches reuse the stages)
+    const float probe = swap_sum(not_finite(dk) + not_finite(dv));
+    const bool again = owned && key < a.k_rows && probe != probe;
+    const unsigned long long good = __ballot(key < a.k_rows && (owned || a.fill) && !again);
+    char* patch = smem + wave * 32 * ROWB;
+    store_rows<T>(patch, dk, owned ? a.scale : 0.f, lane, good, [&](int w) { return a.dk + (long)(kw + w) * a.dk_row + head * a.dk_head; });
+    store_rows<T>(patch, dv, owned ? 1.f : 0.f, lane, good, [&](int w) { return a.dv + (long)(kw + w) * a.dv_row + head * a.dv_head; });
+    bad = (unsigned)__ballot(again);
+  } else {
+    bad0 = 8 * wave;
+    const int rr = bad0 + (lane >> 3);
+    const bool mine = __shfl((int)owned, rr, 64), in = kw + rr < a.k_rows;
+    f32x4 y[2], z[2];
+    sum_waves<KS>(smem, 2 * STAGE, dk, 1.f, wave, lane, y);
+    __syncthreads();
+    sum_waves<KS>(smem, 2 * STAGE, dv, 1.f, wave, lane, z);
+    bad = bad_of_eight(y, mine && in) | bad_of_eight(z, mine && in);
+    if (in && (mine || a.fill) && !(bad >> (lane >> 3) & 1)) {
+      store_eight<T>(a.dk + (long)(kw + rr) * a.dk_row + head * a.dk_head, y, mine ? a.scale : 0.f, lane);
+      store_eight<T>(a.dv + (long)(kw + rr) * a.dv_row + head * a.dv_head, z, mine ? 1.f : 0.f, lane);
+    }
+  }
   while (bad) {
-    const int w = __builtin_ctz(bad);
+    const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
     key_grad_again<T, CAP, BIAS>(a, head, kw + w, r_lo, r_hi, lane);
   }
 }
 
 // d_slopes[h] = sum over the rows of head h, in an order that depends on the number of rows alone
-__global__ void __launch_bounds__(256) docs_grad_slopes_kernel(const Args a) {
-  const int head = blockIdx.x / (int)a.group.d, g = blockIdx.x - head * (int)a.group.d;
-  const float* v = column(a, COL_DSLOPE, head);
+__global__ void __launch_bounds__(1024) docs_grad_slopes_kernel(const Args a) {
+  const float* v = column(a, COL_DSLOPE, blockIdx.x);
   double s = 0.0;
-  for (int t = threadIdx.x; t < a.q_rows; t += 256) s += (double)v[(long)t * (int)a.group.d + g];
-  __shared__ double part[256];
+  for (int t = threadIdx.x; t < a.q_rows; t += 1024) s += (double)v[t];
+  __shared__ double part[1024];
   part[threadIdx.x] = s;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
+  for (int o = 512; o > 0; o >>= 1) {
     if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
     __syncthreads();
   }
   if (threadIdx.x == 0) a.d_slopes[blockIdx.x] = (float)part[0];
 }
 
-int pad_rows(const fc_docs& d) { return (int)((d.q_rows * (d.q_heads / d.kv_heads) + 127) / 128 * 128) + 64; }  // (a column is read 64 numbers at a time)
+int pad_rows(const fc_docs& d) { return (int)((d.q_rows + 127) / 128 * 128); }
 
-size_t grad_bytes(const fc_docs& d) {
-  const size_t n = (size_t)pad_rows(d) * d.kv_heads;
-  return n * COLS * 4 + n / 32 * 16;
-}
+size_t grad_bytes(const fc_docs& d) { return (size_t)pad_rows(d) * d.q_heads * COLS * 4 + (size_t)pad_rows(d) / 32 * 16; }
 
 template <typename K>
 int launch_docs(K kern, long blocks, int waves, int lds, const Args& a, const char* what, hipStream_t st) {
@@ -485,25 +546,25 @@ int launch_docs(K kern, long blocks, int waves, int lds, const Args& a, const ch
 
 template <typename T, bool CAP, bool BIAS>
 int launch_grads(Args a, hipStream_t st) {
-  const long cus = device_cus();
+  constexpr int row = Tile<T>::kRow;
+  const char *rows = "fc_attention_docs_backward (rows)", *keys = "fc_attention_docs_backward (keys)";
+  const long cus = device_cus(), heads = (long)a.kv_heads * a.share;
   int rc;
-  // four waves share a tile where that still gives every compute unit a workgroup, as in the forward
   a.tiles = (a.rows + 127) / 128;
-  if ((long)a.tiles * a.kv_heads >= cus) {
-    rc = launch_docs(docs_grad_rows_kernel<T, 4, 64, CAP, BIAS>, (long)a.tiles * a.kv_heads, 4, 4 * 64 * Tile<T>::kRow, a, "fc_attention_docs_backward (rows)", st);
+  if (a.tiles * heads >= 2 * cus) {
+    rc = launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
   } else {
     a.tiles = (a.rows + 31) / 32;
-    rc = launch_docs(docs_grad_rows_kernel<T, 1, 32, CAP, BIAS>, (long)a.tiles * a.kv_heads, 1, 4 * 32 * Tile<T>::kRow, a, "fc_attention_docs_backward (rows)", st);
+    rc = launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS>, a.tiles * heads, 4, 8 * 64 * row, a, rows, st);
   }
   if (rc != FC_OK) return rc;
-  constexpr int row = Tile<T>::kRow;
   const long four = (a.k_rows + 127) / 128 * (long)a.kv_heads;
-  if (four >= cus)
-    rc = launch_docs(docs_grad_keys_kernel<T, 4, 64, CAP, BIAS>, four, 4, 2 * (128 * row + 7 * 256), a, "fc_attention_docs_backward (keys)", st);
+  if (four >= 2 * cus)
+    rc = launch_docs(docs_grad_keys_kernel<T, 4, 1, 64, CAP, BIAS>, four, 4, 2 * (128 * row + 6 * 256 + 64), a, keys, st);
   else
-    rc = launch_docs(docs_grad_keys_kernel<T, 1, 32, CAP, BIAS>, (a.k_rows + 31) / 32 * (long)a.kv_heads, 1, 2 * (64 * row + 7 * 256), a, "fc_attention_docs_backward (keys)", st);
+    rc = launch_docs(docs_grad_keys_kernel<T, 1, 4, 32, CAP, BIAS>, (a.k_rows + 31) / 32 * (long)a.kv_heads, 4, 8 * (64 * row + 6 * 128 + 64), a, keys, st);
   if (rc != FC_OK || !a.d_slopes) return rc;
-  return launch_docs(docs_grad_slopes_kernel, (long)a.kv_heads * a.group.d, 4, 0, a, "fc_attention_docs_backward (slopes)", st);
+  return launch_docs(docs_grad_slopes_kernel, heads, 16, 0, a, "fc_attention_docs_backward (slopes)", st);
 }
 
 template <typename T>
@@ -539,6 +600,8 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
       !docs::rows_aligned(d_q, dq_row, dq_head, d->kind) || !docs::rows_aligned(d_k, dk_row, dk_head, d->kind) ||
       !docs::rows_aligned(d_v, dv_row, dv_head, d->kind) || ((uintptr_t)stats & 7))
     return fail(FC_EINVAL, "fc_attention_docs_backward: rows and heads must start on 16-byte boundaries");
+  if (do_row * (d->kind == PREC_F32 ? 4 : 2) >= 1 << 25)
+    return fail(FC_EINVAL, "fc_attention_docs_backward: rows of d_out lie 32 MiB or more apart");
   const size_t need = docs::grad_bytes(*d);
   if (need && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 15)))
     return fail(FC_ENOMEM, "fc_attention_docs_backward: scratch of %zu bytes (16-byte aligned) needed, %zu given", need, scratch ? scratch_bytes : 0);
@@ -553,6 +616,9 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
   a.dq_row = dq_row * size; a.dq_head = dq_head * size;
   a.dk_row = dk_row * size; a.dk_head = dk_head * size;
   a.dv_row = dv_row * size; a.dv_head = dv_head * size;
+  a.share = (int)a.group.d;
+  a.group = docs::FastDiv(1);
+  a.rows = a.q_rows;
   a.d_slopes = d_slopes;
   a.table = (float*)scratch;
   a.rows_pad = docs::pad_rows(*d);

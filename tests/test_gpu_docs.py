@@ -156,11 +156,11 @@ def test_attention_four_wave_tiles(dtype):
     """Enough rows that 128 of them share a tile of keys, in documents that end inside tiles."""
     q_len = [300, 17, 129, 0, 64, 250]
     rows = sum(q_len)
-    heads = 64  # 6 tiles of 128 rows x 64 heads: more than one workgroup per compute unit
+    heads = 96  # 6 tiles of 128 rows x 96 heads: more than two workgroups per compute unit
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     for causal in (False, True):
         out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal, cap=20.0)
-        some = [0, 31, 63]  # (the reference is slow: three heads of them)
+        some = [0, 31, 95]  # (the reference is slow: three heads of them)
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, cap=20.0)
         ds = R.score_error(ref, 300, cap=20.0)
         _within("out", out[:, some], ref["out"], R.out_bound(ref, v, dtype, 300, ds))
@@ -271,13 +271,13 @@ def test_gradients_of_other_numbers_of_keys(dtype, q_len, k_len, causal):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gradients_four_wave_tiles(dtype):
     q_len = [300, 17, 129, 0, 64, 250]
-    rows, heads = sum(q_len), 64
+    rows, heads = sum(q_len), 96
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     d_out = _rand(rows, heads, 64, seed=5, dtype=dtype)
     for causal in (False, True):
         out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal)
         grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=causal)
-        some = [0, 63]
+        some = [0, 95]
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, d_out=d_out[:, some])
         bounds = R.grad_bounds(ref, q[:, some], k[:, some], v[:, some], d_out[:, some], dtype, 300, R.score_error(ref, 300))
         for name, got in zip(("d_q", "d_k", "d_v"), grads):
