@@ -164,35 +164,44 @@ __device__ __forceinline__ void lds_dma(const char* src, char* dst) {
 
 // ROWS rows of 64 values, `stride` bytes apart from `base` on (wave-uniform; the rows behind the first n repeat row n - 1), into the LDS tile
 // at dst: 1 KiB pieces, dealt to the NW waves.  A piece's source is a uniform base plus a lane offset (row in the piece, swizzled chunk) that
-// is the same for every piece of the wave (NW = 4) or turned by a constant.
+// is the same for every piece of the wave, or turned by a constant.
 template <typename T, int NW>
 struct Stager {
   static constexpr int PIECE = Tile<T>::kPiece, CH = 64 / PIECE;
-  unsigned in, chunk, off;  // row and source chunk (in bytes) of the lane in the wave's first piece; both as one offset
+  unsigned off;  // row of the lane in the wave's first piece, and its swizzled chunk, as an offset
+  int lane;
   __device__ __forceinline__ static unsigned turn(unsigned piece) {  // what the row bits above the piece's own do to the chunk
     return sizeof(T) == 2 ? (piece & 1) << 4 : (piece & 1) << 7 | (piece & 2) << 5;
   }
-  __device__ __forceinline__ void init(unsigned stride, int wave, int lane) {
-    in = lane / CH;
-    chunk = (lane % CH ^ Tile<T>::swizzle(in)) << 4 ^ turn(wave);
-    off = in * stride + chunk;
+  __device__ __forceinline__ static unsigned chunk(unsigned lane, unsigned piece) { return (lane % CH ^ Tile<T>::swizzle(lane / CH)) << 4 ^ turn(piece); }
+  __device__ __forceinline__ void init(unsigned stride, int wave, int l) {
+    lane = l;
+    off = l / CH * stride + chunk(l, wave);
   }
   template <int ROWS>
   __device__ __forceinline__ void rows(char* dst, const char* base, unsigned stride, int n, int wave) const {
     constexpr int NP = ROWS / PIECE;
-    static_assert(NP % NW == 0 && (NW == 1 || NW % 4 == 0), "every wave brings the same number of pieces, all with the same turn");
+    static_assert(NP % NW == 0, "every wave brings the same number of pieces");
+    constexpr bool kSame = NW % (sizeof(T) == 2 ? 2 : 4) == 0;  // all of a wave's pieces have the same turn
     dst += wave * 1024;
+    unsigned l = lane;
     if (n >= ROWS) {
       base += (unsigned)wave * PIECE * stride;
-      unsigned turned = chunk;
-      if constexpr (NW == 1) asm volatile("" : "+v"(turned));  // (formed here, not kept through the kernel)
+      if constexpr (!kSame) {
+        asm volatile("" : "+v"(l));  // (formed here, not kept through the kernel)
+        const unsigned in = l / CH * stride;
 #pragma unroll
-      for (int j = 0; j < NP / NW; ++j)
-        lds_dma(base + (unsigned)(j * NW * PIECE) * stride + (NW == 1 ? off - chunk + (turned ^ turn(j)) : off), dst + j * NW * 1024);
+        for (int j = 0; j < NP / NW; ++j)
+          lds_dma(base + (unsigned)(j * NW * PIECE) * stride + (in + chunk(l, wave + j * NW)), dst + j * NW * 1024);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NP / NW; ++j) lds_dma(base + (unsigned)(j * NW * PIECE) * stride + off, dst + j * NW * 1024);
+      }
     } else {
+      asm volatile("" : "+v"(l));
 #pragma unroll
       for (int j = 0; j < NP / NW; ++j)
-        lds_dma(base + (min((wave + j * NW) * PIECE + in, (unsigned)(n - 1)) * stride + (NW == 1 ? chunk ^ turn(j) : chunk)), dst + j * NW * 1024);
+        lds_dma(base + (min((wave + j * NW) * PIECE + l / CH, (unsigned)(n - 1)) * stride + chunk(l, wave + j * NW)), dst + j * NW * 1024);
     }
   }
 };
@@ -237,27 +246,33 @@ template <> struct RowOff<bf16> {
   }
 };
 template <> struct RowOff<float> {
-  int o[8];
-  __device__ __forceinline__ void init(int r, int hh) {
-#pragma unroll
-    for (int c = 0; c < 8; ++c) o[c] = r * 256 + (((2 * c + hh) ^ Tile<float>::swizzle(r)) << 4);
-  }
+  int o;  // chunk hh; chunk 2 c + hh is the same address with bits c << 5 turned (formed at the read: eight registers less)
+  __device__ __forceinline__ void init(int r, int hh) { o = r * 256 + ((hh ^ Tile<float>::swizzle(r)) << 4); }
 };
 
-// acc[row of the LDS tile][column = the lane's fragment] += tile row . fragment, 32 rows starting at `tile`
-__device__ __forceinline__ f32x16 rows_dot(const char* tile, const RowOff<bf16>& off, const RowFrag<bf16>& f, f32x16 acc) {
+// 32 rows of an LDS tile as the first operand: every read is issued before the first product wants one (left alone, hipcc reads, waits and
+// multiplies by turns, and the LDS latency shows wherever a SIMD has few waves)
+__device__ __forceinline__ void read_rows(const char* tile, const RowOff<bf16>& off, RowFrag<bf16>& f) {
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(tile + off.o[s]), f.v[s], acc, 0, 0, 0);
+  for (int s = 0; s < 4; ++s) f.v[s] = *reinterpret_cast<const bf16x8*>(tile + off.o[s]);
+}
+__device__ __forceinline__ void read_rows(const char* tile, const RowOff<float>& off, RowFrag<float>& f) {
+  int o = off.o;
+  asm volatile("" : "+v"(o));
+#pragma unroll
+  for (int c = 0; c < 8; ++c) f.v[c] = *reinterpret_cast<const f32x4*>(tile + (o ^ c << 5));
+}
+// acc[row of the tile][column = the lane's fragment] += tile row . fragment
+__device__ __forceinline__ f32x16 rows_dot(const RowFrag<bf16>& rows, const RowFrag<bf16>& f, f32x16 acc) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows.v[s], f.v[s], acc, 0, 0, 0);
   return acc;
 }
-__device__ __forceinline__ f32x16 rows_dot(const char* tile, const RowOff<float>& off, const RowFrag<float>& f, f32x16 acc) {
+__device__ __forceinline__ f32x16 rows_dot(const RowFrag<float>& rows, const RowFrag<float>& f, f32x16 acc) {
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const f32x4 k = *reinterpret_cast<const f32x4*>(tile + off.o[c]);
+  for (int c = 0; c < 8; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], f.v[c][e], acc, 0, 0, 0);
-  }
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(rows.v[c][e], f.v[c][e], acc, 0, 0, 0);
   return acc;
 }
 
@@ -274,14 +289,10 @@ template <> struct ColOff<bf16> {
   }
 };
 template <> struct ColOff<float> {
-  int o[2][4];
+  int o;  // n = 0, row 4 hh of an 8-row block; row + e and half n turn bits of the chunk, as the block's parity does (swizzle bit 2)
   __device__ __forceinline__ void init(int lane) {
     const int r = lane & 31, hh = lane >> 5;
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)  // row 4 hh + e of an 8-row block (its parity, swizzle bit 2, is added by the reader)
-        o[n][e] = (4 * hh + e) * 256 + (((8 * n + (r >> 2)) ^ (hh << 3 | e)) << 4) + (r & 3) * 4;
+    o = 4 * hh * 256 + (((r >> 2) ^ hh << 3) << 4) + (r & 3) * 4;
   }
 };
 
@@ -290,42 +301,46 @@ __device__ __forceinline__ s16x4 read_tr(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
 }
 
-// weights: a 32 x 32 accumulator tile (rows = the 32 rows of the LDS tile) as the second operand of a product over those rows
-struct WeightsB { bf16x8 v[2]; };
-__device__ __forceinline__ void to_weights(const f32x16& p, WeightsB& w) {
+// columns of 32 rows of an LDS tile as the first operand of a product over those rows
+template <typename T> struct ColFrag;
+template <> struct ColFrag<bf16> { bf16x8 v[2][2]; };  // [16 rows][32 columns]
+template <> struct ColFrag<float> { float v[16][2]; };
+__device__ __forceinline__ void read_cols(const char* tile, const ColOff<bf16>& off, ColFrag<bf16>& f) {
 #pragma unroll
   for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w.v[s][j] = static_cast<bf16>(p[8 * s + j]);  // blocks b = 2 s, 2 s + 1 of four rows each
-}
-
-// out[32 n + column][lane's column of p] += sum over the 32 LDS rows of tile[row][32 n + ..] p[row][..]
-__device__ __forceinline__ void cols_dot(const char* tile, const ColOff<bf16>& off, const f32x16& p, f32x16 (&out)[2]) {
-  WeightsB w;
-  to_weights(p, w);
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       // rows 16 s + 4 hh .. and 16 s + 8 + 4 hh ..: the odd 8-row block has row bit 3 set, which moves chunk bit 0
       const s16x4 a = read_tr(tile + off.o[n] + s * 2048), b = read_tr(tile + (off.o[n] ^ 16) + s * 2048 + 1024);
-      const bf16x8 f = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-      out[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, w.v[s], out[n], 0, 0, 0);
+      f.v[s][n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
+}
+__device__ __forceinline__ void read_cols(const char* tile, const ColOff<float>& off, ColFrag<float>& f) {
+  int o = off.o;
+  asm volatile("" : "+v"(o));
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) f.v[4 * b + e][n] = *reinterpret_cast<const float*>(tile + (o ^ (n << 7 | e << 4 | (b & 1) << 6)) + e * 256 + b * 2048);
+}
+// out[32 n + column][lane's column of p] += sum over the 32 rows of cols[row][32 n + ..] p[row][..]; p: an accumulator tile, as it lies
+__device__ __forceinline__ void cols_dot(const ColFrag<bf16>& f, const f32x16& p, f32x16 (&out)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    bf16x8 w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = static_cast<bf16>(p[8 * s + j]);  // blocks b = 2 s, 2 s + 1 of four rows each
+#pragma unroll
+    for (int n = 0; n < 2; ++n) out[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v[s][n], w, out[n], 0, 0, 0);
   }
 }
-__device__ __forceinline__ void cols_dot(const char* tile, const ColOff<float>& off, const f32x16& p, f32x16 (&out)[2]) {
+__device__ __forceinline__ void cols_dot(const ColFrag<float>& f, const f32x16& p, f32x16 (&out)[2]) {
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
+  for (int i = 0; i < 16; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float f = *reinterpret_cast<const float*>(tile + (off.o[n][e] ^ ((b & 1) << 6)) + b * 2048);
-        out[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f, p[4 * b + e], out[n], 0, 0, 0);
-      }
-    }
-  }
+    for (int n = 0; n < 2; ++n) out[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f.v[i][n], p[i], out[n], 0, 0, 0);
 }
 
 // score of a raw product in log2 units

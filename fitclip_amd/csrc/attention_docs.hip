@@ -92,11 +92,13 @@ attention_docs_kernel(const Args a) {
     t_last = min(ntile, t_first + part);
   }
 
-  const int m = min(m0 + r, a.rows - 1);
-  const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
   RowFrag<T> qf;
-  qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
-  const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
+  float slope = 0.f;
+  {
+    const int m = min(m0 + r, a.rows - 1), token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+    qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
+    if constexpr (BIAS) slope = a.slopes[qh] * kLog2e;
+  }
 
   const char* kbase = a.k + head * a.k_head;
   const char* vbase = a.v + head * a.v_head;
@@ -136,12 +138,20 @@ attention_docs_kernel(const Args a) {
     const char* vt = kt + TK * ROWB;
     const bool full = full_lo <= k0 && k0 + TK <= full_hi;
     f32x16 s[NT];
+    RowFrag<T> kf[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) read_rows(kt + u * 32 * ROWB, koff, kf[u]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-      s[u] = rows_dot(kt + u * 32 * ROWB, koff, qf, s[u]);
+      s[u] = rows_dot(kf[u], qf, s[u]);
     }
+    ColFrag<T> vf[NT];  // (on their way under the softmax)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+    __builtin_amdgcn_sched_barrier(0);
     // scores in log2 units
     const float at = BIAS ? (float)(row.pos - k0 - 4 * hh) : 0.f;
 #pragma unroll
@@ -191,7 +201,7 @@ attention_docs_kernel(const Args a) {
         l += s[u][i];
       }
 #pragma unroll
-    for (int u = 0; u < NT; ++u) cols_dot(vt + u * 32 * ROWB, voff, s[u], o);
+    for (int u = 0; u < NT; ++u) cols_dot(vf[u], s[u], o);
   }
   l = swap_sum(l);
   float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
@@ -218,8 +228,12 @@ attention_docs_kernel(const Args a) {
     } else {
       const float inv = sees ? down / l : 0.f;
       const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
-      if (hh == 0 && write)
+      if (hh == 0 && write) {
+        int m = m0 + r;
+        asm volatile("" : "+v"(m));  // (token and head are formed here again, not kept through the loop)
+        const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
         *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
+      }
       __syncthreads();  // (the patches reuse the stages)
       store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
         const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);

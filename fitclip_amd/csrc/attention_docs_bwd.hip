@@ -238,8 +238,14 @@ docs_grad_rows_kernel(const Args a) {
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-      s = rows_dot(kt + u * 32 * ROWB, roff, qf, s);
-      dp = rows_dot(vt + u * 32 * ROWB, roff, dof, dp);
+      RowFrag<T> kf, vf;
+      read_rows(kt + u * 32 * ROWB, roff, kf);
+      read_rows(vt + u * 32 * ROWB, roff, vf);
+      __builtin_amdgcn_sched_barrier(0);
+      s = rows_dot(kf, qf, s);
+      dp = rows_dot(vf, dof, dp);
+      ColFrag<T> kc;  // (on their way under the next step)
+      read_cols(kt + u * 32 * ROWB, coff, kc);
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
       const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
       const unsigned bits = full ? 0xffffu : visible_bits(row.lo - ku, row.hi - ku, hh);
@@ -270,7 +276,7 @@ docs_grad_rows_kernel(const Args a) {
         s[i] = ds;
       }
       __builtin_amdgcn_sched_barrier(0);
-      cols_dot(kt + u * 32 * ROWB, coff, s, o);
+      cols_dot(kc, s, o);
     }
   }
   if constexpr (BIAS) {
@@ -437,8 +443,17 @@ docs_grad_keys_kernel(const Args a) {
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-      s = rows_dot(qt, roff, kf, s);
-      dp = rows_dot(dt, roff, vf, dp);
+      {
+        RowFrag<T> rows;
+        read_rows(qt, roff, rows);
+        __builtin_amdgcn_sched_barrier(0);
+        s = rows_dot(rows, kf, s);
+        read_rows(dt, roff, rows);
+        __builtin_amdgcn_sched_barrier(0);
+        dp = rows_dot(rows, vf, dp);
+      }
+      ColFrag<T> cols;
+      if constexpr (sizeof(T) == 2) read_cols(dt, coff, cols);  // (on their way under the next step; fp32: no registers for that)
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -477,8 +492,14 @@ docs_grad_keys_kernel(const Args a) {
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      cols_dot(dt, coff, s, dv);
-      cols_dot(qt, coff, dp, dk);
+      if constexpr (sizeof(T) == 4) {
+        read_cols(dt, coff, cols);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      cols_dot(cols, s, dv);
+      read_cols(qt, coff, cols);
+      __builtin_amdgcn_sched_barrier(0);
+      cols_dot(cols, dp, dk);
     }
   }
   const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
