@@ -477,6 +477,12 @@ __device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool count
 
 #endif  // __HIPCC__
 
+// From how many workgroups of 128 rows (keys) on four waves share tiles instead of taking turns over them.  Sharing has a quarter of the
+// traffic, turns have work in smaller pieces; both measured on 12 heads of 1, 2, 3, 6, 12 x 3136 tokens (1.2 to 14 workgroups per compute
+// unit), forward, us: bf16 sharing 61 127 147 246 447, turns 62 113 155 297 576; fp32 (whose products take ten times as long) sharing
+// 354 802 1004 1617, turns 291 570 799 1585, and over 4 x 8192 tokens, 8 per compute unit, 4206 and 4555.
+inline long sharing_from(int kind) { return (kind == PREC_F32 ? 8L : 3L) * device_cus(); }
+
 int check_docs(const fc_docs* d, const char* what);
 bool rows_aligned(const void* p, int64_t row, int64_t head, int kind);
 Args make_args(const fc_docs& d);

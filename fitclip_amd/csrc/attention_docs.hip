@@ -48,10 +48,11 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 }
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? (KS > 1 ? 1 : 2) : KS > 1 ? 2 : 3)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 3)))
 attention_docs_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
-  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
+  constexpr int BUFS = KS > 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
+  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * RW];
   __shared__ float shares[KS > 1 ? KS : 1][2][32];
@@ -107,7 +108,7 @@ attention_docs_kernel(const Args a) {
   Stager<T, SW> kin, vin;
   kin.init((unsigned)a.k_row, sw, lane);
   vin.init((unsigned)a.v_row, sw, lane);
-  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  char* const stages = smem + (KS > 1 ? wave * STAGE : 0);
   auto stage = [&](int t, int buf) {
     char* dst = stages + buf * STAGE;
     const long first = kbeg + t * TK;
@@ -128,12 +129,17 @@ attention_docs_kernel(const Args a) {
   float mref = -kInf, mtop = -kInf, l = 0.f;  // the maximum that the sums refer to (it follows the true one in steps of 2^8), the true one
   int t = t_first + (KS > 1 ? wave : 0), buf = 0;
   if (t < t_last) stage(t, 0);
-  for (; t < t_last; t += KS, buf ^= 1) {
+  for (; t < t_last; t += KS, buf ^= BUFS - 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (KS == 1) __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
-    if (t + KS < t_last) stage(t + KS, buf ^ 1);
+    if constexpr (KS == 1) {
+      __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
+      if (t + KS < t_last) stage(t + KS, buf ^ 1);
+    }
     const int k0 = kbeg + t * TK;
-    if (k0 >= whi || k0 + TK <= wlo) continue;  // (wave-uniform)
+    if (k0 >= whi || k0 + TK <= wlo) {  // (wave-uniform)
+      if (KS > 1 && t + KS < t_last) stage(t + KS, 0);
+      continue;
+    }
     const char* kt = stages + buf * STAGE;
     const char* vt = kt + TK * ROWB;
     const bool full = full_lo <= k0 && k0 + TK <= full_hi;
@@ -141,6 +147,13 @@ attention_docs_kernel(const Args a) {
     RowFrag<T> kf[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) read_rows(kt + u * 32 * ROWB, koff, kf[u]);
+    ColFrag<T> vf[NT];
+    if constexpr (KS > 1) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (t + KS < t_last) stage(t + KS, 0);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -148,9 +161,10 @@ attention_docs_kernel(const Args a) {
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
       s[u] = rows_dot(kf[u], qf, s[u]);
     }
-    ColFrag<T> vf[NT];  // (on their way under the softmax)
+    if constexpr (KS == 1) {  // (on their way under the softmax)
 #pragma unroll
-    for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+      for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     // scores in log2 units
     const float at = BIAS ? (float)(row.pos - k0 - 4 * hh) : 0.f;
@@ -255,7 +269,7 @@ attention_docs_kernel(const Args a) {
     for (int w = 0; w < KS; ++w) sum = __builtin_fmaf(shares[w][1][r], __builtin_amdgcn_exp2f(shares[w][0][r] - ref), sum);
     down *= __builtin_amdgcn_exp2f(mtop - ref);
     f32x4 y[2];
-    sum_waves<KS>(smem, 2 * STAGE, o, down, wave, lane, y);
+    sum_waves<KS>(smem, STAGE, o, down, wave, lane, y);
     bad0 = 8 * wave;
     const int rr = bad0 + (lane >> 3), mr = m0 + rr;
     const bool valid = __shfl((int)row.valid, rr, 64), see = __shfl((int)sees, rr, 64);
@@ -338,7 +352,7 @@ struct Plan {
 Plan plan_forward(const fc_docs& d) {
   const long group = d.q_heads / d.kv_heads, rows = d.q_rows * group, cus = device_cus();
   Plan p{true, (int)((rows + 127) / 128), 1};
-  if ((long)p.tiles * d.kv_heads >= 2 * cus) return p;
+  if ((long)p.tiles * d.kv_heads >= sharing_from(d.kind)) return p;
   p.shared = false;
   p.tiles = (int)((rows + 31) / 32);
   const long units = (long)p.tiles * d.kv_heads;
@@ -355,7 +369,7 @@ size_t part_bytes(const fc_docs& d, const Plan& p) {
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
 int launch_forward(const Args& a, hipStream_t st) {
-  constexpr int lds = 2 * KS * 2 * TK * Tile<T>::kRow;
+  constexpr int lds = (KS > 1 ? KS : 2) * 2 * TK * Tile<T>::kRow;
   auto kern = attention_docs_kernel<T, RW, KS, TK, CAP, BIAS>;
   if (lds > 60 * 1024 && raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds) != hipSuccess)
     return fail(FC_ELAUNCH, "fc_attention_docs: cannot raise dynamic LDS");

@@ -89,6 +89,22 @@ __device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int
   }
 }
 
+// the rows of the documents that own keys k0 .. k0 + n - 1; causal: in the first of them from the first row that sees k0
+__device__ __forceinline__ void rows_of_keys(const Args& a, int k0, int n, int lane, int& r_lo, int& r_hi) {
+  const int last = min(k0 + n, a.k_rows) - 1;
+  const int d0 = min(max(wave_count_le(a.k_off, a.docs + 1, k0, lane) - 1, 0), a.docs - 1);
+  const int d1 = min(max(wave_count_le(a.k_off, a.docs + 1, last, lane) - 1, d0), a.docs - 1);
+  const int qs = min(max(a.q_off[d0], 0), a.q_rows), qe = min(max(a.q_off[d0 + 1], qs), a.q_rows);
+  int skip = 0;
+  if (a.causal) {
+    const int ks = min(max(a.k_off[d0], 0), a.k_rows), ke = min(max(a.k_off[d0 + 1], ks), a.k_rows);
+    const int j = k0 - ks;
+    if (!(a.prefix && a.prefix[d0] > j)) skip = min(max(j - (ke - ks) + (qe - qs), 0), qe - qs);
+  }
+  r_lo = qs + skip;
+  r_hi = min(max(a.q_off[d1 + 1], 0), a.q_rows);
+}
+
 // d_k and d_v of one key again, row by row (rows r_lo .. r_hi - 1 hold those that see it)
 template <typename T, bool CAP, bool BIAS>
 __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r_hi, int lane) {
@@ -124,10 +140,11 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
 
 // ------------------------------------------------------------------------------------------------------------------ rows
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && KS > 1 ? 1 : 2)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(2)))
 docs_grad_rows_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
-  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
+  constexpr int BUFS = KS > 1 ? 1 : 2;  // (as in the forward)
+  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && STAGE >= 8192 && NT == 1), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * RW];
   __shared__ float shares[KS > 1 ? KS : 1][3][32];
@@ -203,7 +220,7 @@ docs_grad_rows_kernel(const Args a) {
   Stager<T, SW> kin, vin;
   kin.init((unsigned)a.k_row, sw, lane);
   vin.init((unsigned)a.v_row, sw, lane);
-  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  char* const stages = smem + (KS > 1 ? wave * STAGE : 0);
   auto stage = [&](int t, int buf) {
     char* dst = stages + buf * STAGE;
     const long first = kbeg + t * TK;
@@ -223,17 +240,22 @@ docs_grad_rows_kernel(const Args a) {
   float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
   int t = KS > 1 ? wave : 0, buf = 0;
   if (t < ntile) stage(t, 0);
-  for (; t < ntile; t += KS, buf ^= 1) {
+  for (; t < ntile; t += KS, buf ^= BUFS - 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (KS == 1) __syncthreads();
-    if (t + KS < ntile) stage(t + KS, buf ^ 1);
+    if constexpr (KS == 1) {
+      __syncthreads();
+      if (t + KS < ntile) stage(t + KS, buf ^ 1);
+    }
     const int k0 = kbeg + t * TK;
     const char* kt = stages + buf * STAGE;
     const char* vt = kt + TK * ROWB;
 #pragma unroll 1
     for (int u = 0; u < NT; ++u) {
       const int ku = k0 + 32 * u;
-      if (ku >= whi || ku + 32 <= wlo) continue;  // (wave-uniform)
+      if (ku >= whi || ku + 32 <= wlo) {  // (wave-uniform)
+        if (KS > 1 && t + KS < ntile) stage(t + KS, 0);
+        continue;
+      }
       const bool full = full_lo <= ku && ku + 32 <= full_hi;
       f32x16 s, dp;
 #pragma unroll
@@ -246,6 +268,10 @@ docs_grad_rows_kernel(const Args a) {
       dp = rows_dot(vf, dof, dp);
       ColFrag<T> kc;  // (on their way under the next step)
       read_cols(kt + u * 32 * ROWB, coff, kc);
+      if constexpr (KS > 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + KS < ntile) stage(t + KS, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
       const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
       const unsigned bits = full ? 0xffffu : visible_bits(row.lo - ku, row.hi - ku, hh);
@@ -304,7 +330,7 @@ docs_grad_rows_kernel(const Args a) {
       }
     }
     f32x4 y[2];
-    sum_waves<KS>(smem, 2 * STAGE, o, 1.f, wave, lane, y);  // (with a barrier inside)
+    sum_waves<KS>(smem, STAGE, o, 1.f, wave, lane, y);  // (with a barrier inside)
     bad0 = 8 * wave;
     const int rr = bad0 + (lane >> 3), mr = m0 + rr;
     const bool valid = __shfl((int)row.valid, rr, 64), many = __shfl(row.hi - row.lo, rr, 64) > 1;
@@ -336,7 +362,7 @@ docs_grad_rows_kernel(const Args a) {
 
 // ------------------------------------------------------------------------------------------------------------------ keys
 template <typename T, int KW, int KS, int TQ, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(KW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && KS > 1 ? 1 : 2)))
+__global__ void __launch_bounds__(KW * KS * 64) __attribute__((amdgpu_waves_per_eu(2)))
 docs_grad_keys_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow;
   constexpr int OFF_DO = TQ * ROWB, OFF_TAB = 2 * TQ * ROWB;
@@ -345,29 +371,17 @@ docs_grad_keys_kernel(const Args a) {
   constexpr int COLB = TQ * 4;                            // a column's share of a stage
   constexpr int OFF_KEYS = OFF_TAB + 6 * COLB;            // the blocks' four ints
   constexpr int STAGE = OFF_KEYS + 64;
-  static_assert((KS == 1 && KW * 32 * ROWB <= 2 * STAGE) || (KW == 1 && 2 * STAGE >= 8192), "the output patches reuse the stages");
+  constexpr int BUFS = KS > 1 && sizeof(T) == 4 ? 1 : 2;  // (fp32, a wave alone: one, or a second workgroup would not fit the CU)
+  static_assert((KS == 1 && KW * 32 * ROWB <= 2 * STAGE) || (KW == 1 && STAGE >= 8192 && TQ == 32), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;  // (earlier keys first: causal, they cost most)
+  const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
+  const int tile = rest % a.tiles, split = rest / a.tiles;  // (earlier keys first: causal, they cost most)
   const int k0 = tile * KW * 32, kw = k0 + (KS > 1 ? 0 : wave * 32);
 
-  // rows of the documents that own keys k0 .. k0 + 32 KW - 1; causal: in the first of them from the first row that sees k0
   int r_lo, r_hi;
-  {
-    const int last = min(k0 + KW * 32, a.k_rows) - 1;
-    const int d0 = min(max(wave_count_le(a.k_off, a.docs + 1, k0, lane) - 1, 0), a.docs - 1);
-    const int d1 = min(max(wave_count_le(a.k_off, a.docs + 1, last, lane) - 1, d0), a.docs - 1);
-    const int qs = min(max(a.q_off[d0], 0), a.q_rows), qe = min(max(a.q_off[d0 + 1], qs), a.q_rows);
-    int skip = 0;
-    if (a.causal) {
-      const int ks = min(max(a.k_off[d0], 0), a.k_rows), ke = min(max(a.k_off[d0 + 1], ks), a.k_rows);
-      const int j = k0 - ks;
-      if (!(a.prefix && a.prefix[d0] > j)) skip = min(max(j - (ke - ks) + (qe - qs), 0), qe - qs);
-    }
-    r_lo = qs + skip;
-    r_hi = min(max(a.q_off[d1 + 1], 0), a.q_rows);
-  }
+  rows_of_keys(a, k0, KW * 32, lane, r_lo, r_hi);
   const int t_first = r_lo / TQ, steps = r_hi > r_lo ? (r_hi + TQ - 1) / TQ - t_first : 0;  // tiles of rows, for each query head of the group
 
   const int key = kw + r;
@@ -381,7 +395,7 @@ docs_grad_keys_kernel(const Args a) {
   Stager<T, SW> qin, din;
   qin.init((unsigned)a.q_row, sw, lane);
   din.init((unsigned)a.do_row, sw, lane);
-  char* const stages = smem + (KS > 1 ? wave * 2 * STAGE : 0);
+  char* const stages = smem + (KS > 1 ? wave * BUFS * STAGE : 0);
   auto stage = [&](int qh, int t, int buf) {
     char* dst = stages + buf * STAGE;
     const long first = (long)t * TQ;
@@ -410,12 +424,20 @@ docs_grad_keys_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
   int g = 0, t = KS > 1 ? wave : 0, buf = 0;  // query head of the group, tile of rows
+  int left = steps * a.share;                 // tiles of this part of the rows, from here on
+  if (a.splits > 1) {
+    const int part = (int)((unsigned)(left + a.splits - 1) / (unsigned)a.splits);
+    t += split * part;
+    left = min(part, left - split * part);
+  }
+  left -= KS > 1 ? wave : 0;
   const int all = steps ? a.share : 0;
   auto settle = [&](int& g, int& t) {
     while (t >= steps && g < all) {
       t -= steps;
       ++g;
     }
+    if (left <= 0) g = all;
   };
   settle(g, t);
   if (g < all) stage(head * a.share + g, t_first + t, 0);
@@ -425,16 +447,26 @@ docs_grad_keys_kernel(const Args a) {
     const int now = t_first + t;
     const float slope = BIAS ? a.slopes[head * a.share + g] * kLog2e : 0.f;
     t += KS;
+    left -= KS;
     settle(g, t);
-    if (g < all) stage(head * a.share + g, t_first + t, buf ^ 1);
+    if (BUFS == 2 && g < all) stage(head * a.share + g, t_first + t, buf ^ 1);
+    const auto next = [&] {  // a wave alone: what it needs of this tile is in registers
+      if constexpr (BUFS == 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (g < all) stage(head * a.share + g, t_first + t, 0);
+      }
+    };
     const char* st = stages + buf * STAGE;
-    buf ^= 1;
+    buf ^= BUFS - 1;
 #pragma unroll 1
     for (int u = 0; u < TQ / 32; ++u) {
-      if ((now * (TQ / 32) + u) * 32 >= a.rows) continue;
+      if ((now * (TQ / 32) + u) * 32 >= a.rows) continue;  // (TQ 64 only: a tile has rows)
       const int bl = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16));
       const int bh = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 4));
-      if (kw >= bh || kw + 32 <= bl) continue;  // (wave-uniform)
+      if (kw >= bh || kw + 32 <= bl) {  // (wave-uniform)
+        next();
+        continue;
+      }
       const bool full = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 8)) <= kw &&
                         kw + 32 <= __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(st + OFF_KEYS + u * 16 + 12));
       const char* qt = st + u * 32 * ROWB;
@@ -498,13 +530,15 @@ docs_grad_keys_kernel(const Args a) {
       }
       cols_dot(cols, s, dv);
       read_cols(qt, coff, cols);
+      next();
       __builtin_amdgcn_sched_barrier(0);
       cols_dot(cols, dp, dk);
     }
   }
   const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
-  unsigned bad;  // keys to be done again: bit k = key kw + bad0 + k
+  unsigned bad = 0;  // keys to be done again: bit k = key kw + bad0 + k
   int bad0 = 0;
+  float* const part = a.part + ((long)split * a.kv_heads + head) * a.k_rows * 128;  // d_k and d_v of a part of the rows, 64 values each
   if constexpr (KS == 1) {
     __syncthreads();  // (the patches reuse the stages)
     const float probe = swap_sum(not_finite(dk) + not_finite(dv));
@@ -519,9 +553,16 @@ docs_grad_keys_kernel(const Args a) {
     const int rr = bad0 + (lane >> 3);
     const bool mine = __shfl((int)owned, rr, 64), in = kw + rr < a.k_rows;
     f32x4 y[2], z[2];
-    sum_waves<KS>(smem, 2 * STAGE, dk, 1.f, wave, lane, y);
+    sum_waves<KS>(smem, BUFS * STAGE, dk, 1.f, wave, lane, y);
     __syncthreads();
-    sum_waves<KS>(smem, 2 * STAGE, dv, 1.f, wave, lane, z);
+    sum_waves<KS>(smem, BUFS * STAGE, dv, 1.f, wave, lane, z);
+    if (a.splits > 1) {
+      if (in) {
+        store_eight<float>(reinterpret_cast<char*>(part + (long)(kw + rr) * 128), y, 1.f, lane);
+        store_eight<float>(reinterpret_cast<char*>(part + (long)(kw + rr) * 128 + 64), z, 1.f, lane);
+      }
+      return;
+    }
     bad = bad_of_eight(y, mine && in) | bad_of_eight(z, mine && in);
     if (in && (mine || a.fill) && !(bad >> (lane >> 3) & 1)) {
       store_eight<T>(a.dk + (long)(kw + rr) * a.dk_row + head * a.dk_head, y, mine ? a.scale : 0.f, lane);
@@ -533,6 +574,30 @@ docs_grad_keys_kernel(const Args a) {
     bad &= bad - 1;
     key_grad_again<T, CAP, BIAS>(a, head, kw + w, r_lo, r_hi, lane);
   }
+}
+
+// adds the parts up, in order: a wave per key and key head, a lane per dimension
+template <typename T, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256) docs_grad_join_kernel(const Args a) {
+  const int lane = threadIdx.x & 63, head = blockIdx.x % a.kv_heads;
+  const int key = (blockIdx.x / a.kv_heads) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (key >= a.k_rows) return;
+  const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
+  if (!owned && !a.fill) return;
+  float dk = 0.f, dv = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part + (((long)s * a.kv_heads + head) * a.k_rows + key) * 128 + lane;
+    dk += p[0];
+    dv += p[64];
+  }
+  if (owned && __any((dk + dv) * 0.f != 0.f)) {
+    int r_lo, r_hi;
+    rows_of_keys(a, key, 1, lane, r_lo, r_hi);
+    key_grad_again<T, CAP, BIAS>(a, head, key, r_lo, r_hi, lane);
+    return;
+  }
+  put_at<T>(a.dk + key * a.dk_row + head * a.dk_head, lane, owned ? dk * a.scale : 0.f);
+  put_at<T>(a.dv + key * a.dv_row + head * a.dv_head, lane, owned ? dv : 0.f);
 }
 
 // d_slopes[h] = sum over the rows of head h, in an order that depends on the number of rows alone
@@ -552,7 +617,30 @@ __global__ void __launch_bounds__(1024) docs_grad_slopes_kernel(const Args a) {
 
 int pad_rows(const fc_docs& d) { return (int)((d.q_rows + 127) / 128 * 128); }
 
-size_t grad_bytes(const fc_docs& d) { return (size_t)pad_rows(d) * d.q_heads * COLS * 4 + (size_t)pad_rows(d) / 32 * 16; }
+size_t table_bytes(const fc_docs& d) { return (size_t)pad_rows(d) * d.q_heads * COLS * 4 + (size_t)pad_rows(d) / 32 * 16; }
+
+// Workgroups of the keys kernel: four waves x 32 keys that share tiles of rows, or four waves that take turns over the rows of 32 keys; where
+// that leaves compute units without work, the rows of a key are cut into parts on top of it
+struct KeyPlan {
+  bool shared;
+  int tiles, splits;
+};
+KeyPlan plan_keys(const fc_docs& d) {
+  const long cus = device_cus();
+  KeyPlan p{true, (int)((d.k_rows + 127) / 128), 1};
+  if ((long)p.tiles * d.kv_heads >= sharing_from(d.kind)) return p;
+  p.shared = false;
+  p.tiles = (int)((d.k_rows + 31) / 32);
+  const long units = std::max(1L, (long)p.tiles * d.kv_heads);
+  const double rows = (double)d.q_rows / std::max(1, d.docs) * (d.q_heads / d.kv_heads);  // mean way of a key through the rows
+  p.splits = (int)std::max(1L, std::min({4 * cus / units, (long)(rows / 256.0), 64L}));
+  return p;
+}
+
+size_t grad_bytes(const fc_docs& d) {
+  const KeyPlan p = plan_keys(d);
+  return table_bytes(d) + (p.splits > 1 ? (size_t)p.splits * d.kv_heads * d.k_rows * 128 * sizeof(float) : 0);
+}
 
 template <typename K>
 int launch_docs(K kern, long blocks, int waves, int lds, const Args& a, const char* what, hipStream_t st) {
@@ -566,32 +654,36 @@ int launch_docs(K kern, long blocks, int waves, int lds, const Args& a, const ch
 }
 
 template <typename T, bool CAP, bool BIAS>
-int launch_grads(Args a, hipStream_t st) {
+int launch_grads(Args a, const KeyPlan& p, hipStream_t st) {
   constexpr int row = Tile<T>::kRow;
   const char *rows = "fc_attention_docs_backward (rows)", *keys = "fc_attention_docs_backward (keys)";
-  const long cus = device_cus(), heads = (long)a.kv_heads * a.share;
+  const long heads = (long)a.kv_heads * a.share;
   int rc;
   a.tiles = (a.rows + 127) / 128;
-  if (a.tiles * heads >= 2 * cus) {
+  if (a.tiles * heads >= sharing_from(sizeof(T) == 4 ? PREC_F32 : PREC_BF16)) {
     rc = launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
   } else {
     a.tiles = (a.rows + 31) / 32;
-    rc = launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS>, a.tiles * heads, 4, 8 * 64 * row, a, rows, st);
+    rc = launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS>, a.tiles * heads, 4, 4 * 64 * row, a, rows, st);
   }
   if (rc != FC_OK) return rc;
-  const long four = (a.k_rows + 127) / 128 * (long)a.kv_heads;
-  if (four >= 2 * cus)
-    rc = launch_docs(docs_grad_keys_kernel<T, 4, 1, 64, CAP, BIAS>, four, 4, 2 * (128 * row + 6 * 256 + 64), a, keys, st);
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  const long units = (long)p.tiles * p.splits * a.kv_heads;
+  if (p.shared)
+    rc = launch_docs(docs_grad_keys_kernel<T, 4, 1, 64, CAP, BIAS>, units, 4, 2 * (128 * row + 6 * 256 + 64), a, keys, st);
   else
-    rc = launch_docs(docs_grad_keys_kernel<T, 1, 4, 32, CAP, BIAS>, (a.k_rows + 31) / 32 * (long)a.kv_heads, 4, 8 * (64 * row + 6 * 128 + 64), a, keys, st);
+    rc = launch_docs(docs_grad_keys_kernel<T, 1, 4, 32, CAP, BIAS>, units, 4, (sizeof(T) == 4 ? 4 : 8) * (64 * row + 6 * 128 + 64), a, keys, st);
+  if (rc == FC_OK && p.splits > 1)
+    rc = launch_docs(docs_grad_join_kernel<T, CAP, BIAS>, ((long)a.k_rows + 3) / 4 * a.kv_heads, 4, 0, a, "fc_attention_docs_backward (join)", st);
   if (rc != FC_OK || !a.d_slopes) return rc;
   return launch_docs(docs_grad_slopes_kernel, heads, 16, 0, a, "fc_attention_docs_backward (slopes)", st);
 }
 
 template <typename T>
-int launch_grads_type(const Args& a, bool cap, hipStream_t st) {
-  if (a.slopes) return cap ? launch_grads<T, true, true>(a, st) : launch_grads<T, false, true>(a, st);
-  return cap ? launch_grads<T, true, false>(a, st) : launch_grads<T, false, false>(a, st);
+int launch_grads_type(const Args& a, const KeyPlan& p, bool cap, hipStream_t st) {
+  if (a.slopes) return cap ? launch_grads<T, true, true>(a, p, st) : launch_grads<T, false, true>(a, p, st);
+  return cap ? launch_grads<T, true, false>(a, p, st) : launch_grads<T, false, false>(a, p, st);
 }
 
 }  // namespace
@@ -642,8 +734,10 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
   a.rows = a.q_rows;
   a.d_slopes = d_slopes;
   a.table = (float*)scratch;
+  const docs::KeyPlan p = docs::plan_keys(*d);
+  a.part = reinterpret_cast<float*>((char*)scratch + docs::table_bytes(*d));
   a.rows_pad = docs::pad_rows(*d);
-  return d->kind == PREC_F32 ? docs::launch_grads_type<float>(a, d->cap > 0.f, st) : docs::launch_grads_type<bf16>(a, d->cap > 0.f, st);
+  return d->kind == PREC_F32 ? docs::launch_grads_type<float>(a, p, d->cap > 0.f, st) : docs::launch_grads_type<bf16>(a, p, d->cap > 0.f, st);
 }
 
 }  // extern "C"

@@ -151,16 +151,16 @@ def test_attention_of_few_rows_over_many_keys(dtype, q_len, k_len, causal):
     _check_forward(q, k, v, q_len, k_len, causal=causal)
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-def test_attention_four_wave_tiles(dtype):
+@pytest.mark.parametrize("dtype,heads", [(torch.float32, 352), (torch.bfloat16, 144)])
+def test_attention_four_wave_tiles(dtype, heads):
     """Enough rows that 128 of them share a tile of keys, in documents that end inside tiles."""
     q_len = [300, 17, 129, 0, 64, 250]
     rows = sum(q_len)
-    heads = 96  # 6 tiles of 128 rows x 96 heads: more than two workgroups per compute unit
+    # 6 tiles of 128 rows a head: more than eight (bf16: three) workgroups per compute unit
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     for causal in (False, True):
         out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal, cap=20.0)
-        some = [0, 31, 95]  # (the reference is slow: three heads of them)
+        some = [0, 31, heads - 1]  # (the reference is slow: three heads of them)
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, cap=20.0)
         ds = R.score_error(ref, 300, cap=20.0)
         _within("out", out[:, some], ref["out"], R.out_bound(ref, v, dtype, 300, ds))
@@ -268,20 +268,43 @@ def test_gradients_of_other_numbers_of_keys(dtype, q_len, k_len, causal):
     _check_gradients(q, k, v, q_len, k_len, causal=causal)
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-def test_gradients_four_wave_tiles(dtype):
+@pytest.mark.parametrize("dtype,heads", [(torch.float32, 352), (torch.bfloat16, 144)])
+def test_gradients_four_wave_tiles(dtype, heads):
     q_len = [300, 17, 129, 0, 64, 250]
-    rows, heads = sum(q_len), 96
+    rows = sum(q_len)
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     d_out = _rand(rows, heads, 64, seed=5, dtype=dtype)
     for causal in (False, True):
         out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal)
         grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=causal)
-        some = [0, 95]
+        some = [0, heads - 1]
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, d_out=d_out[:, some])
         bounds = R.grad_bounds(ref, q[:, some], k[:, some], v[:, some], d_out[:, some], dtype, 300, R.score_error(ref, 300))
         for name, got in zip(("d_q", "d_k", "d_v"), grads):
             _within(name, got[:, some], ref[name], bounds[name])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [False, True])
+def test_gradients_of_few_keys_with_many_rows(dtype, bad):
+    """One key head of six query heads: the rows of a key are cut into parts."""
+    q_len, heads = [300, 1, 219], 6
+    rows = sum(q_len)
+    q, k, v = _operands(rows, rows, heads, 1, dtype, seed=13, layout="fused")
+    how = dict(causal=True, cap=9.0, slopes=torch.full((heads,), 0.02, device=DEV))
+    if not bad:
+        _check_gradients(q, k, v, q_len, **how)
+        return
+    q_off, d_out = R.offsets(q_len), _rand(rows, heads, 64, seed=14, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, q_off, **how)
+    clean = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, **how)
+    d_out[299] = math.nan  # the first document's last row: sees all of its keys, and no other
+    got = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, **how)
+    assert not torch.isfinite(got[2][:300]).any() and torch.isfinite(got[0][:299]).all()
+    for a, b in zip(got, clean):
+        assert torch.isfinite(a[300:]).all()
+        # done again key by key, with weights in fp32
+        assert float((a[300:].double() - b[300:].double()).abs().max()) <= 8 * R.HALF[dtype] * float(b.double().abs().max()) + 1e-4
 
 
 def test_gradients_by_differences():
