@@ -46,8 +46,8 @@ struct Args {
   int docs, kv_heads, rows, q_rows, k_rows;             // rows = kernel rows = q_rows * group
   FastDiv group;
   int causal, fill;
-  float c;                                              // scale log2 e (no cap): score in log2 units = raw * c
-  float cap_in, cap_out;                                // scale / cap, cap log2 e: score = cap_out tanh(raw cap_in)
+  float c;                                              // scale log2 e: score in log2 units = raw * c
+  float cap_in;                                         // scale / cap: behind a cap, score = c tanh(raw cap_in) with c = cap log2 e
   // forward
   char* out;
   long out_row, out_head;
@@ -130,20 +130,33 @@ __device__ __forceinline__ Row find_row(const Args& a, int m0, int lane) {
   return r;
 }
 
-// tanh: exact to 1.2e-7 (fp32 scores) or to 3e-7 of 1 in three instructions less (bf16 scores, whose own rounding is 2^-9)
-template <bool EXACT>
+// tanh(u) = u + u^3 P(u^2) for |u| < 9 / 16 (least squares on Chebyshev nodes, 7e-8), 1 - 2 / (1 + e^2u) beyond (1.2e-7): the quotient alone
+// would lose the small scores that a cap hardly bends
+constexpr float kTanhSmall = 0.5625f;
+__device__ __forceinline__ float tanh_small(float u) {
+  const float w = u * u;
+  float p = -0.006178273353725672f;
+  p = __builtin_fmaf(p, w, 0.021006036549806595f);
+  p = __builtin_fmaf(p, w, -0.05383696034550667f);
+  p = __builtin_fmaf(p, w, 0.13332445919513702f);
+  p = __builtin_fmaf(p, w, -0.3333331346511841f);
+  return __builtin_fmaf(u * w, p, u);
+}
 __device__ __forceinline__ float tanh_f32(float u) {
-  if constexpr (EXACT) {
-    const float au = fabsf(u), w = u * u;
-    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(au * (2.f * kLog2e)) + 1.f);
-    float p = -0.006178273353725672f;  // tanh(u) = u + u^3 P(u^2) for |u| <= 9 / 16: least squares on Chebyshev nodes, 7e-8
-    p = __builtin_fmaf(p, w, 0.021006036549806595f);
-    p = __builtin_fmaf(p, w, -0.05383696034550667f);
-    p = __builtin_fmaf(p, w, 0.13332445919513702f);
-    p = __builtin_fmaf(p, w, -0.3333331346511841f);
-    return au < 0.5625f ? __builtin_fmaf(u * w, p, u) : copysignf(big, u);
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(u) * (2.f * kLog2e)) + 1.f);
+  return fabsf(u) < kTanhSmall ? tanh_small(u) : copysignf(big, u);
+}
+// s <- tanh(s * by); scores of more than half the cap are rare, so the wave looks for one before it pays for them
+__device__ __forceinline__ void bend(f32x16& s, float by) {
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, fabsf(s[i])), fabsf(s[i + 1]));
+  if (__any(mx * by >= kTanhSmall)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = tanh_f32(s[i] * by);
   } else {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * (2.f * kLog2e)) + 1.f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = tanh_small(s[i] * by);
   }
 }
 
@@ -344,9 +357,9 @@ __device__ __forceinline__ void cols_dot(const ColFrag<float>& f, const f32x16& 
 }
 
 // score of a raw product in log2 units
-template <typename T, bool CAP, bool BIAS>
+template <bool CAP, bool BIAS>
 __device__ __forceinline__ float score(const Args& a, float raw, float slope, float far) {
-  float x = CAP ? a.cap_out * tanh_f32<sizeof(T) == 4>(raw * a.cap_in) : raw * a.c;
+  float x = CAP ? a.c * tanh_f32(raw * a.cap_in) : raw * a.c;
   if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
   return x;
 }

@@ -27,7 +27,7 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 #pragma unroll 1
   for (int j = lo; j < hi; j += 64) {
     const int key = min(j + lane, hi - 1);
-    float x = score<T, CAP, BIAS>(a, row_dot<T>(kb + key * a.k_row, q), slope, fabsf((float)(pos - key)));
+    float x = score<CAP, BIAS>(a, row_dot<T>(kb + key * a.k_row, q), slope, fabsf((float)(pos - key)));
     if (j + lane >= hi) x = -kInf;
     const float mx = fmaxf(top, wave_max(x)), ref = mx == -kInf ? 0.f : mx;
     const float p = __builtin_amdgcn_exp2f(x - ref), alpha = top == mx ? 1.f : __builtin_amdgcn_exp2f(top - ref);
@@ -161,24 +161,23 @@ attention_docs_kernel(const Args a) {
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
       s[u] = rows_dot(kf[u], qf, s[u]);
     }
-    if constexpr (KS == 1) {  // (on their way under the softmax)
+    if constexpr (KS == 1 && !CAP) {  // (on their way under the softmax; a cap has no registers for that)
 #pragma unroll
       for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // scores in log2 units
-    const float at = BIAS ? (float)(row.pos - k0 - 4 * hh) : 0.f;
+    // scores in log2 units; without a bias they are scaled in the exponent's fma
+    if constexpr (CAP) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
+      for (int u = 0; u < NT; ++u) bend(s[u], a.cap_in);
+    }
+    if constexpr (BIAS) {
+      const float at = (float)(row.pos - k0 - 4 * hh);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int w = 32 * u + 8 * (i >> 2) + (i & 3);
-        float x = s[u][i];  // (neither cap nor bias: scaled in the exponent's fma)
-        if constexpr (CAP) x = a.cap_out * tanh_f32<sizeof(T) == 4>(x * a.cap_in);
-        else if constexpr (BIAS) x *= a.c;
-        if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf(at - (float)w), x);
-        s[u][i] = x;
-      }
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = __builtin_fmaf(-slope, fabsf(at - (float)(32 * u + 8 * (i >> 2) + (i & 3))), s[u][i] * a.c);
+    }
     if (!full) {
       __builtin_amdgcn_sched_barrier(0);  // (the masks are formed here, not kept through the products)
 #pragma unroll
@@ -188,14 +187,17 @@ attention_docs_kernel(const Args a) {
         for (int i = 0; i < 16; ++i) s[u][i] = pick(bits, i, s[u][i], -kInf);
       }
     }
+    if constexpr (KS == 1 && CAP) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+    }
     float mx = s[0][0];
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[u][i]), s[u][i + 1]);
     mx = swap_max(mx);
-    constexpr bool kRaw = !CAP && !BIAS;
-    if constexpr (kRaw) mx *= a.c;
+    if constexpr (!BIAS) mx *= a.c;
     mtop = fmaxf(mtop, mx);
     if (__any(mtop > mref + 8.f)) {  // 2^8 of headroom costs nothing in fp32 and saves most of the rescaling
       const float alpha = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);
@@ -211,7 +213,7 @@ attention_docs_kernel(const Args a) {
     for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[u][i] = __builtin_amdgcn_exp2f(kRaw ? __builtin_fmaf(s[u][i], a.c, -mm) : s[u][i] - mm);
+        s[u][i] = __builtin_amdgcn_exp2f(BIAS ? s[u][i] - mm : __builtin_fmaf(s[u][i], a.c, -mm));
         l += s[u][i];
       }
 #pragma unroll
@@ -439,9 +441,8 @@ Args make_args(const fc_docs& d) {
   a.group = FastDiv((unsigned)(d.q_heads / d.kv_heads));
   a.rows = (int)(d.q_rows * (d.q_heads / d.kv_heads));
   a.causal = d.causal; a.fill = d.fill;
-  a.c = (float)((double)d.scale * 1.4426950408889634);
+  a.c = (float)((double)(d.cap > 0.f ? d.cap : d.scale) * 1.4426950408889634);
   a.cap_in = d.cap > 0.f ? (float)((double)d.scale / d.cap) : 0.f;
-  a.cap_out = (float)((double)d.cap * 1.4426950408889634);
   a.scale = d.scale;
   a.splits = 1;
   return a;

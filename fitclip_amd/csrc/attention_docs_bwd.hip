@@ -49,10 +49,10 @@ __device__ __forceinline__ float dot(const RowFrag<float>& x, const RowFrag<floa
 }
 
 // dS behind P, dP, D and the raw product
-template <typename T, bool CAP>
+template <bool CAP>
 __device__ __forceinline__ float bent_by(const Args& a, float raw, float ds) {
   if constexpr (CAP) {
-    const float t = tanh_f32<sizeof(T) == 4>(raw * a.cap_in);
+    const float t = tanh_f32(raw * a.cap_in);
     ds *= 1.f - t * t;
   }
   return ds;
@@ -70,13 +70,13 @@ __device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int
   for (int j = lo; j < hi; j += 64) {
     const int key = min(j + lane, hi - 1);
     const float raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
-    float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - top) * inv;
+    float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - top) * inv;
     const float g = row_dot<T>(vb + key * a.v_row, go);
     if (j + lane >= hi) p = 0.f;
     pd = __builtin_fmaf(p, g, pd);
     pf = __builtin_fmaf(p, far, pf);
     pdf = __builtin_fmaf(p * g, far, pdf);
-    const float ds = bent_by<T, CAP>(a, raw, p * (g - D));
+    const float ds = bent_by<CAP>(a, raw, p * (g - D));
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
   }
@@ -123,9 +123,9 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
       if (!seen) continue;
       const float raw = row_dot<T>(qb + m * a.q_row, k), g = row_dot<T>(db + m * a.do_row, v);
       const float far = BIAS ? fabsf((float)(__float_as_int(column(a, COL_POS, qh)[m]) - key)) : 0.f;
-      float p = __builtin_amdgcn_exp2f(score<T, CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, qh)[m]);
+      float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, qh)[m]);
       if constexpr (sizeof(T) == 4) p *= column(a, COL_INV, qh)[m];
-      const float ds = hi - lo == 1 ? 0.f : bent_by<T, CAP>(a, raw, p * (g - column(a, COL_D, qh)[m]));
+      const float ds = hi - lo == 1 ? 0.f : bent_by<CAP>(a, raw, p * (g - column(a, COL_D, qh)[m]));
 #pragma unroll 1
       for (int w = 0; w < 64; ++w) {
         if (!(seen >> w & 1)) continue;
@@ -274,32 +274,29 @@ docs_grad_rows_kernel(const Args a) {
       }
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
       const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
-      const unsigned bits = full ? 0xffffu : visible_bits(row.lo - ku, row.hi - ku, hh);
+      if constexpr (CAP) bend(s, a.cap_in);
+      f32x16 p;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int w = 8 * (i >> 2) + (i & 3);
-        float bent = 0.f, x;
-        if constexpr (CAP) {
-          bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
-          x = a.cap_out * bent;
-        } else {
-          x = s[i] * a.c;
-        }
-        const float far = BIAS ? fabsf(at - (float)w) : 0.f;
-        if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
-        float p = __builtin_amdgcn_exp2f(x - top);
-        if constexpr (sizeof(T) == 4) p *= inv;
-        if (!full) p = pick(bits, i, p, 0.f);  // (a NaN of a masked key then shows in the result: see row_grad_again)
-        const float g = dp[i];
+        const float far = fabsf(at - (float)(8 * (i >> 2) + (i & 3)));
+        p[i] = __builtin_amdgcn_exp2f(BIAS ? __builtin_fmaf(-slope, far, s[i] * a.c) - top : __builtin_fmaf(s[i], a.c, -top));
+        if constexpr (sizeof(T) == 4) p[i] *= inv;
+      }
+      if (!full) {  // (a NaN of a masked key then shows in the result: see row_grad_again)
+        const unsigned bits = visible_bits(row.lo - ku, row.hi - ku, hh);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = pick(bits, i, p[i], 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
         if constexpr (BIAS) {
-          const float y = p * g;
+          const float far = fabsf(at - (float)(8 * (i >> 2) + (i & 3))), y = p[i] * dp[i];
           pd += y;
-          pf = __builtin_fmaf(p, far, pf);
+          pf = __builtin_fmaf(p[i], far, pf);
           pdf = __builtin_fmaf(y, far, pdf);
         }
-        float ds = p * (g - D);
-        if constexpr (CAP) ds *= 1.f - bent * bent;
-        s[i] = ds;
+        const float ds = p[i] * (dp[i] - D);
+        s[i] = CAP ? ds * __builtin_fmaf(-s[i], s[i], 1.f) : ds;
       }
       __builtin_amdgcn_sched_barrier(0);
       cols_dot(kc, s, o);
@@ -487,40 +484,41 @@ docs_grad_keys_kernel(const Args a) {
       ColFrag<T> cols;
       if constexpr (sizeof(T) == 2) read_cols(dt, coff, cols);  // (on their way under the next step; fp32: no registers for that)
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
+      if constexpr (CAP) bend(s, a.cap_in);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if constexpr (sizeof(T) == 4) asm volatile("" ::: "memory");  // (four rows of the table at a time)
         const char* at = tab + (8 * b + 4 * hh) * 4;
         const f32x4 top = *reinterpret_cast<const f32x4*>(at + COL_MAX * COLB), D = *reinterpret_cast<const f32x4*>(at + COL_D * COLB);
-        f32x4 inv = {1.f, 1.f, 1.f, 1.f}, pos = {}, lo = {}, hi = {};
+        f32x4 inv, pos;
         if constexpr (kInv) inv = *reinterpret_cast<const f32x4*>(at + COL_INV * COLB);
         if constexpr (BIAS) pos = *reinterpret_cast<const f32x4*>(at + COL_POS * COLB);
-        if (!full) {
-          lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB);
-          hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
-        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = 4 * b + e;
-          float bent = 0.f, x;
-          if constexpr (CAP) {
-            bent = tanh_f32<sizeof(T) == 4>(s[i] * a.cap_in);
-            x = a.cap_out * bent;
-          } else {
-            x = s[i] * a.c;
-          }
-          if constexpr (BIAS) x = __builtin_fmaf(-slope, fabsf((float)(__float_as_int(pos[e]) - key)), x);
-          float p = __builtin_amdgcn_exp2f(x - top[e]);
+          float p;
+          if constexpr (BIAS)
+            p = __builtin_amdgcn_exp2f(__builtin_fmaf(-slope, fabsf((float)(__float_as_int(pos[e]) - key)), s[i] * a.c) - top[e]);
+          else
+            p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -top[e]));
           if constexpr (kInv) p *= inv[e];
-          float ds = p * (dp[i] - D[e]);
-          if constexpr (CAP) ds *= 1.f - bent * bent;
-          if (!full) {
-            const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
-            ds = rel < len && len > 1 ? ds : 0.f;  // (one key: its weight is 1 whatever the score)
-            p = rel < len ? p : 0.f;
-          }
+          dp[i] = p * (dp[i] - D[e]);
+          if constexpr (CAP) dp[i] *= __builtin_fmaf(-s[i], s[i], 1.f);
           s[i] = p;
-          dp[i] = ds;
+        }
+      }
+      if (!full) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const char* at = tab + (8 * b + 4 * hh) * 4;
+          const f32x4 lo = *reinterpret_cast<const f32x4*>(at + COL_LO * COLB), hi = *reinterpret_cast<const f32x4*>(at + COL_HI * COLB);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 4 * b + e;
+            const unsigned rel = (unsigned)(key - __float_as_int(lo[e])), len = (unsigned)(__float_as_int(hi[e]) - __float_as_int(lo[e]));
+            s[i] = rel < len ? s[i] : 0.f;
+            dp[i] = rel < len && len > 1 ? dp[i] : 0.f;  // (one key: its weight is 1 whatever the score)
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);
