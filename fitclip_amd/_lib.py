@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 from typing import Optional
 
@@ -54,6 +55,14 @@ class fc_docs(C.Structure):
 
     def __init__(self, **kw):
         super().__init__(struct_size=C.sizeof(type(self)), **kw)
+
+    @classmethod
+    def of(cls, *values) -> "fc_docs":
+        """The struct from its fields behind `struct_size`, in order (a pointer that is None: 0): a third of the keywords' time."""
+        return cls.from_buffer_copy(_DOCS.pack(_DOCS.size, *values))
+
+
+_DOCS = struct.Struct("@7i2f2q3P6q4P")
 
 
 _vp, _i32, _i64, _sz, _f32, _f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_float, C.c_double
@@ -169,6 +178,12 @@ def check(rc: int, what: str = "") -> None:
 def current_stream() -> int:
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def stream_of(index: int) -> int:
+    """`current_stream` of device `index` without the Stream object around it (a tenth of its time)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def require_gpu() -> None:

@@ -516,7 +516,24 @@ def _heads(t: torch.Tensor, name: str, dtype: torch.dtype, dim: Optional[int] = 
 
 
 def _strides(t: torch.Tensor) -> "tuple[int, int]":
-    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+    rows, heads, _ = t.shape
+    row, head, _ = t.stride()
+    return (row if rows > 1 else 0), (head if heads > 1 else 0)
+
+
+class _On:
+    """`torch.cuda.device`, at no cost where the device is the current one already."""
+
+    def __init__(self, index: int) -> None:
+        self.guard = None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+    def __enter__(self) -> None:
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *error) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*error)
 
 
 def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
@@ -532,14 +549,14 @@ def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _on_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
     for name, t in tensors.items():
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if t.get_device() < 0:
             raise _lib.FitclipHipError(f"{name} must live on the ROCm device (got {t.device}); there is no CPU fallback")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
 
 
 def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, n: Optional[int] = None) -> None:
@@ -579,17 +596,19 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
         _written(out, "out", x)
         if out.data_ptr() == x.data_ptr() and _strides(out) != _strides(x):
             raise ValueError("in place needs the same strides")
-    _on_device(x.device, x=x, positions=positions, inv_freq=inv_freq, out=out)
+    index = x.get_device()
+    _on_device(index, x=x, positions=positions, inv_freq=inv_freq, out=out)
     if out is None:
         out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().fc_rotary(_KIND[x.dtype], x.data_ptr(), *_strides(x), positions.data_ptr(), axes, inv_freq.data_ptr(),
+    (x_row, x_head), (out_row, out_head) = _strides(x), _strides(out)
+    with _On(index):
+        _lib.check(_lib.load().fc_rotary(_KIND[x.dtype], x.data_ptr(), x_row, x_head, positions.data_ptr(), axes, inv_freq.data_ptr(),
                                          (_lib._i32 * axes)(*sections), pairs, int(interleaved), int(inverse), out.data_ptr(),
-                                         *_strides(out), rows, heads, dim, _lib.current_stream()), "fc_rotary")
+                                         out_row, out_head, rows, heads, dim, _lib.stream_of(index)), "fc_rotary")
     return out
 
 
-def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill) -> "_lib.fc_docs":
+def _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale) -> None:
     _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have the same shape")
@@ -598,25 +617,39 @@ def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fil
     _vector(q_offsets, "q_offsets", torch.int32)
     if not q_offsets.numel():
         raise ValueError("q_offsets must hold docs + 1 numbers")
-    if k_offsets is None:
-        if k.shape[0] != q.shape[0]:
-            raise ValueError("k_offsets is needed where keys and queries differ in number")
-        k_offsets = q_offsets
+    if k_offsets is None and k.shape[0] != q.shape[0]:
+        raise ValueError("k_offsets is needed where keys and queries differ in number")
     docs = q_offsets.numel() - 1
     _vector(k_offsets, "k_offsets", torch.int32, docs + 1)
     _vector(prefix, "prefix", torch.int32, docs)
     _vector(slopes, "slopes", torch.float32, q.shape[1])
     if prefix is not None and not causal:
         raise ValueError("a prefix mask needs causal=True")
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
     if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
         raise ValueError(f"scale must be positive and cap 0 (none) or positive, got {scale} and {cap}")
-    _on_device(q.device, q=q, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, prefix=prefix, slopes=slopes)
-    (q_row, q_head), (k_row, k_head), (v_row, v_head) = _strides(q), _strides(k), _strides(v)
-    return _lib.fc_docs(kind=_KIND[q.dtype], docs=docs, q_heads=q.shape[1], kv_heads=k.shape[1], causal=int(causal), fill=int(fill),
-                        scale=scale, cap=float(cap), q_rows=q.shape[0], k_rows=k.shape[0], q=q.data_ptr(), k=k.data_ptr(),
-                        v=v.data_ptr(), q_row=q_row, q_head=q_head, k_row=k_row, k_head=k_head, v_row=v_row, v_head=v_head,
-                        q_offsets=q_offsets.data_ptr(), k_offsets=k_offsets.data_ptr(), prefix=_ptr(prefix), slopes=_ptr(slopes))
+    _on_device(q.get_device(), q=q, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, prefix=prefix, slopes=slopes)
+
+
+def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill) -> "_lib.fc_docs":
+    scale = 0.125 if scale is None else scale  # 64 ** -0.5
+    q_shape, k_shape, index, kind = q.shape, k.shape, q.get_device(), _KIND.get(q.dtype)
+    q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+    # the operands as they should be, looked over in a few microseconds; anything else is named by _check_docs
+    if not (len(q_shape) == 3 == len(k_shape) and k_shape == v.shape and q_shape[2] == 64 == k_shape[2] and kind is not None
+            and q.dtype is k.dtype is v.dtype and q_stride[2] == 1 == k_stride[2] == v_stride[2] and q_shape[0] and k_shape[0]
+            and k_shape[1] and q_shape[1] and not q_shape[1] % k_shape[1] and index >= 0 and index == k.get_device() == v.get_device()
+            and index == q_offsets.get_device() and q_offsets.dtype is torch.int32 and q_offsets.dim() == 1 and q_offsets.numel()
+            and q_offsets.is_contiguous() and k_offsets is None and k_shape[0] == q_shape[0] and prefix is None and slopes is None
+            and scale > 0 and cap == 0 and scale < float("inf")):
+        _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale)
+    q_heads, k_heads = q_shape[1], k_shape[1]
+    q_many, k_many = q_shape[0] > 1, k_shape[0] > 1
+    at = q_offsets.data_ptr()
+    return _lib.fc_docs.of(kind, q_offsets.numel() - 1, q_heads, k_heads, int(causal), int(fill), scale, cap, q_shape[0], k_shape[0],
+                           q.data_ptr(), k.data_ptr(), v.data_ptr(), q_stride[0] if q_many else 0, q_stride[1] if q_heads > 1 else 0,
+                           k_stride[0] if k_many else 0, k_stride[1] if k_heads > 1 else 0, v_stride[0] if k_many else 0,
+                           v_stride[1] if k_heads > 1 else 0, at, at if k_offsets is None else k_offsets.data_ptr(),
+                           0 if prefix is None else prefix.data_ptr(), 0 if slopes is None else slopes.data_ptr())
 
 
 def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None,
@@ -633,20 +666,23 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
     key gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
 
     Rows behind the last document are left as they were in a given `out` (which may not overlap k or v), and 0 otherwise."""
-    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill=out is None)
+    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, out is None)
+    device, index = q.device, q.get_device()
     if out is None:
-        out = (torch.zeros if d.docs == 0 else torch.empty)(q.shape, dtype=q.dtype, device=q.device)
+        out = (torch.empty if d.docs else torch.zeros)(q.shape, dtype=q.dtype, device=device)
     else:
         _written(out, "out", q)
-        _on_device(q.device, out=out)
-    stats = torch.empty((*q.shape[:2], 2), dtype=torch.float32, device=q.device)
+        _on_device(index, out=out)
+    stats = torch.empty((q.shape[0], q.shape[1], 2), dtype=torch.float32, device=device)
     lib = _lib.load()
-    with torch.cuda.device(q.device):
-        if d.docs == 0 or not d.fill:  # (rows of no document keep these)
+    out_row, out_head = _strides(out)
+    with _On(index):
+        if not d.docs or not d.fill:  # (rows of no document keep these)
             stats[..., 0], stats[..., 1] = float("-inf"), 0.0
-        scratch = torch.empty(lib.fc_attention_docs_scratch_bytes(d), dtype=torch.uint8, device=q.device)
-        _lib.check(lib.fc_attention_docs(d, out.data_ptr(), *_strides(out), stats.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                                         _lib.current_stream()), "fc_attention_docs")
+        need = lib.fc_attention_docs_scratch_bytes(d)
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _lib.check(lib.fc_attention_docs(d, out.data_ptr(), out_row, out_head, stats.data_ptr(), _ptr(scratch), need,
+                                         _lib.stream_of(index)), "fc_attention_docs")
     return out, stats
 
 
@@ -673,18 +709,18 @@ def attention_docs_backward(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     for t, like, name in ((d_q, q, "d_q"), (d_k, k, "d_k"), (d_v, v, "d_v")):
         if t is not None:
             _written(t, name, like)
-    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill=fill)
-    make = torch.empty if fill and d.docs else torch.zeros
-    d_q, d_k, d_v = (make(like.shape, dtype=like.dtype, device=like.device) if t is None else t for t, like in zip(given, (q, k, v)))
-    _on_device(q.device, d_out=d_out, out=out, stats=stats, d_q=d_q, d_k=d_k, d_v=d_v)
+    d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill)
+    make, device, index = torch.empty if fill and d.docs else torch.zeros, q.device, q.get_device()
+    d_q, d_k, d_v = (make(like.shape, dtype=like.dtype, device=device) if t is None else t for t, like in zip(given, (q, k, v)))
+    _on_device(index, d_out=d_out, out=out, stats=stats, d_q=d_q, d_k=d_k, d_v=d_v)
     lib = _lib.load()
-    with torch.cuda.device(q.device):
-        d_slopes = torch.empty(q.shape[1], dtype=torch.float32, device=q.device) if slope_grad else None
+    with _On(index):
+        d_slopes = torch.empty(q.shape[1], dtype=torch.float32, device=device) if slope_grad else None
         if slope_grad and d.docs == 0:
             d_slopes.zero_()
-        scratch = torch.empty(lib.fc_attention_docs_backward_scratch_bytes(d), dtype=torch.uint8, device=q.device)
+        scratch = torch.empty(lib.fc_attention_docs_backward_scratch_bytes(d), dtype=torch.uint8, device=device)
         _lib.check(lib.fc_attention_docs_backward(d, out.data_ptr(), *_strides(out), stats.data_ptr(), d_out.data_ptr(), *_strides(d_out),
                                                   d_q.data_ptr(), *_strides(d_q), d_k.data_ptr(), *_strides(d_k), d_v.data_ptr(),
                                                   *_strides(d_v), _ptr(d_slopes), scratch.data_ptr(), scratch.numel(),
-                                                  _lib.current_stream()), "fc_attention_docs_backward")
+                                                  _lib.stream_of(index)), "fc_attention_docs_backward")
     return (d_q, d_k, d_v) + ((d_slopes,) if slope_grad else ())
