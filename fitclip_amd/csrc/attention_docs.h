@@ -83,17 +83,36 @@ __device__ __forceinline__ int wave_min_i(int v) {
 }
 __device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
 
+__device__ __forceinline__ int lanes_with(bool x) { return (int)__popcll(__ballot(x)); }  // (the builtin counts in unsigned)
+
 // how many of the sorted off[0 .. n) are <= x, found by the whole wave: 64 probes a step
 __device__ __forceinline__ int wave_count_le(const int32_t* off, int n, int x, int lane) {
   int lo = 0, hi = n;
   while (hi > lo) {
     const int step = (hi - lo + 63) >> 6, at = lo + lane * step + step - 1;
     const bool le = at < hi && off[at] <= x;
-    const int c = __popcll(__ballot(le));
+    const int c = lanes_with(le);
     hi = min(hi, lo + c * step + step - 1);
     lo += c * step;
   }
   return lo;
+}
+
+// 64 consecutive offsets off[first] .. (lane l: off[first + l], the last one repeated), among them the last one that is <= x.  Every step
+// here is a load that waits for the one before: two for up to 2048 documents, one for up to 63.
+__device__ __forceinline__ int offsets_around(const int32_t* off, int n, int x, int lane, int& first) {
+  first = 0;
+  if (n > 64) {
+    const int step = (n + 63) >> 6;
+    if (step <= 32) {
+      const int at = lane * step + step - 1;
+      first = max(lanes_with(at < n && off[min(at, n - 1)] <= x) * step - 1, 0);
+    } else {
+      first = max(wave_count_le(off, n, x, lane) - 1, 0);
+    }
+    first = min(max(first, 0), n - 1);
+  }
+  return off[min(first + lane, n - 1)];
 }
 
 struct Row {
@@ -106,22 +125,37 @@ struct Row {
 // wrong intervals but never one outside [0, k_rows).
 __device__ __forceinline__ Row find_row(const Args& a, int m0, int lane) {
   const int m = m0 + (lane & 31);
-  const int t0 = a.group.div(min(m0, a.rows - 1)), t1 = a.group.div(min(m0 + 31, a.rows - 1));
+  const int t0 = a.group.div(min(m0, a.rows - 1));
   const int token = a.group.div(min(m, a.rows - 1));
-  const int first = min(max(wave_count_le(a.q_off, a.docs + 1, t0, lane) - 1, 0), a.docs - 1);
-  int lo = first, hi = first;
-  if (a.docs > 1 && a.q_off[first + 1] <= t1) hi = min(max(wave_count_le(a.q_off, a.docs + 1, t1, lane) - 1, first), a.docs - 1);
-  for (int span = hi - lo; span > 0; span >>= 1) {  // (wave-uniform trip count; each lane narrows to its own document)
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.q_off[mid] <= token) lo = mid; else hi = mid - 1;
-    hi = max(hi, lo);
+  int first, i = 0;
+  const int w = offsets_around(a.q_off, a.docs + 1, t0, lane, first);
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)  // the last offset <= token
+    if (__shfl(w, i + step, 64) <= token) i += step;
+  int d = min(first + i, a.docs - 1);
+  int qs = __shfl(w, min(i, 63), 64), qe = __shfl(w, min(i + 1, 63), 64);
+  if (__any(i == 63)) {  // more documents than that in 32 rows (empty ones)
+    int hi = a.docs - 1;
+    for (int span = hi - first; span > 0; span >>= 1) {  // (wave-uniform trip count)
+      const int mid = (d + hi + 1) >> 1;
+      if (a.q_off[mid] <= token) d = mid; else hi = mid - 1;
+      hi = max(hi, d);
+    }
+    qs = a.q_off[d];
+    qe = a.q_off[d + 1];
   }
-  const int d = lo;
-  const int qs = min(max(a.q_off[d], 0), a.q_rows), qe = min(max(a.q_off[d + 1], qs), a.q_rows);
-  const int ks = min(max(a.k_off[d], 0), a.k_rows), ke = min(max(a.k_off[d + 1], ks), a.k_rows);
+  int ks = qs, ke = qe;
+  if (a.k_off != a.q_off) {
+    ks = a.k_off[d];
+    ke = a.k_off[d + 1];
+  }
+  const int pre = a.causal && a.prefix ? a.prefix[d] : 0;
+  qs = min(max(qs, 0), a.q_rows);
+  qe = min(max(qe, qs), a.q_rows);
+  ks = min(max(ks, 0), a.k_rows);
+  ke = min(max(ke, ks), a.k_rows);
   const int lk = ke - ks, p = token - qs + lk - (qe - qs);
-  int seen = lk;
-  if (a.causal) seen = min(lk, max(p + 1, a.prefix ? a.prefix[d] : 0));
+  const int seen = a.causal ? min(lk, max(p + 1, pre)) : lk;
   Row r;
   r.valid = m < a.rows && token >= qs && token < qe;
   r.lo = r.valid ? ks : 0;

@@ -92,8 +92,13 @@ __device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int
 // the rows of the documents that own keys k0 .. k0 + n - 1; causal: in the first of them from the first row that sees k0
 __device__ __forceinline__ void rows_of_keys(const Args& a, int k0, int n, int lane, int& r_lo, int& r_hi) {
   const int last = min(k0 + n, a.k_rows) - 1;
-  const int d0 = min(max(wave_count_le(a.k_off, a.docs + 1, k0, lane) - 1, 0), a.docs - 1);
-  const int d1 = min(max(wave_count_le(a.k_off, a.docs + 1, last, lane) - 1, d0), a.docs - 1);
+  int first;
+  const int w = offsets_around(a.k_off, a.docs + 1, k0, lane, first);
+  const int before = lanes_with(w <= last);
+  const int d0 = min(max(first + lanes_with(w <= k0) - 1, 0), a.docs - 1);
+  int d1 = first + before - 1;
+  if (before == 64 && first + 63 < a.docs) d1 = wave_count_le(a.k_off, a.docs + 1, last, lane) - 1;  // (many empty documents)
+  d1 = min(max(d1, d0), a.docs - 1);
   const int qs = min(max(a.q_off[d0], 0), a.q_rows), qe = min(max(a.q_off[d0 + 1], qs), a.q_rows);
   int skip = 0;
   if (a.causal) {

@@ -115,7 +115,8 @@ def _check_forward(q, k, v, q_len, k_len=None, **how):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("q_len", [[1], [2], [31], [32], [33], [64], [65], [127, 1], [130], [0, 5, 0, 0, 3, 0], [1] * 70,
-                                   [20, 0, 77, 4, 33, 1, 64], [197, 50]])
+                                   [20, 0, 77, 4, 33, 1, 64], [197, 50], [0] * 100 + [7] + [0] * 90 + [3, 30], [3] * 62, [2] * 63,
+                                   ([1, 0, 2] * 800)[:2300]])
 def test_attention_of_documents(dtype, causal, q_len):
     q, k, v = _operands(sum(q_len), sum(q_len), 2, 2, dtype, seed=len(q_len), layout="fused")
     _check_forward(q, k, v, q_len, causal=causal)
@@ -232,7 +233,8 @@ def _check_gradients(q, k, v, q_len, k_len=None, seed=50, ref=None, **how):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("q_len", [[1], [2], [31], [32], [33], [65], [127, 1], [0, 5, 0, 0, 3, 0], [1] * 70, [20, 0, 77, 4, 33, 1, 64]])
+@pytest.mark.parametrize("q_len", [[1], [2], [31], [32], [33], [65], [127, 1], [0, 5, 0, 0, 3, 0], [1] * 70, [20, 0, 77, 4, 33, 1, 64],
+                                   [0] * 100 + [7] + [0] * 90 + [3, 30], [3] * 62, [2] * 63, ([1, 0, 2] * 800)[:2300]])
 def test_gradients_of_documents(dtype, causal, q_len):
     q, k, v = _operands(sum(q_len), sum(q_len), 2, 2, dtype, seed=len(q_len), layout="fused")
     grads, _, _ = _check_gradients(q, k, v, q_len, causal=causal)
