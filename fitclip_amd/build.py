@@ -143,11 +143,12 @@ def audit_no_scratch(asm_path: Path, substrings) -> int:
 # hazard whose consumer sits inside an asm string (cdna_hip_programming.md section 5.7 item 2).  The one that can bite here: a VALU
 # write of an SGPR (v_readlane_b32 reloading a spilled scalar, v_readfirstlane_b32) needs 5 wait states before a VMEM instruction
 # reads that SGPR as descriptor or offset.  SALU writes are interlocked.  Checked on the generated ISA after every compile.
-ASM_DMA_AUDIT = {"gemm_split2.hip": ["gemm_split2_kernel"]}
+ASM_DMA_AUDIT = {"gemm_split2.hip": ["gemm_split2_kernel"], "attention_docs.hip": ["attention_docs_kernel"],
+                 "attention_docs_bwd.hip": ["docs_grad_rows_kernel", "docs_grad_keys_kernel"]}
 
 
 def audit_asm_dma_hazards(asm_path: Path, substrings) -> int:
-    """Raises if an LDS-DMA `buffer_load ... lds` of a kernel whose name contains one of `substrings` reads an SGPR whose latest
+    """Raises if an LDS-DMA `buffer_load ... lds` / `global_load_lds` of a kernel whose name contains one of `substrings` reads an SGPR whose latest
     writer, fewer than 5 wait states upstream (straight-line scan; s_nop N counts N + 1), is a VALU instruction.  Returns the number
     of DMA instructions checked."""
     import re
@@ -169,7 +170,7 @@ def audit_asm_dma_hazards(asm_path: Path, substrings) -> int:
         lines = [l.split(";")[0].strip() for l in body.splitlines()]
         lines = [l for l in lines if l and not l.endswith(":") and not l.startswith(".")]
         for n, c in enumerate(lines):
-            if not (c.startswith("buffer_load_dword") and c.endswith(" lds")):
+            if not (c.startswith("buffer_load_dword") and c.endswith(" lds") or c.startswith("global_load_lds_dword")):
                 continue
             checked += 1
             need, states, k = sregs(c), 0, n - 1

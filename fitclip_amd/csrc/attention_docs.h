@@ -205,8 +205,16 @@ template <> struct Tile<float> {
   static __device__ __forceinline__ int swizzle(int row) { return ((row >> 2) & 1) << 3 | ((row >> 3) & 1) << 2 | (row & 3); }
 };
 
-__device__ __forceinline__ void lds_dma(const char* src, char* dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// 16 (4) bytes per lane from base + off (base and dst wave-uniform) to LDS, 1 KiB (256 bytes) from dst on.  Spelled as asm: hipcc would wait
+// for all of them in front of the next LDS read, whatever it reads; every kernel here waits by hand where a tile is needed.  No register is
+// written, M0 is ours to set; a scalar that comes from a vector instruction needs five wait states in front of this (build.py looks).
+__device__ __forceinline__ void lds_dma(const char* base, unsigned off, char* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"((unsigned)(uintptr_t)dst), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma_4(const void* base, unsigned off, char* dst) {
+  const uint64_t b = (uint64_t)(uintptr_t)base;  // (said to be uniform once more: hipcc loses sight of it here)
+  const uint64_t u = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)b);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)dst)), "v"(off), "s"(u) : "memory", "m0");
 }
 
 // ROWS rows of 64 values, `stride` bytes apart from `base` on (wave-uniform; the rows behind the first n repeat row n - 1), into the LDS tile
@@ -239,16 +247,16 @@ struct Stager {
         const unsigned in = l / CH * stride;
 #pragma unroll
         for (int j = 0; j < NP / NW; ++j)
-          lds_dma(base + (unsigned)(j * NW * PIECE) * stride + (in + chunk(l, wave + j * NW)), dst + j * NW * 1024);
+          lds_dma(base + (unsigned)(j * NW * PIECE) * stride, in + chunk(l, wave + j * NW), dst + j * NW * 1024);
       } else {
 #pragma unroll
-        for (int j = 0; j < NP / NW; ++j) lds_dma(base + (unsigned)(j * NW * PIECE) * stride + off, dst + j * NW * 1024);
+        for (int j = 0; j < NP / NW; ++j) lds_dma(base + (unsigned)(j * NW * PIECE) * stride, off, dst + j * NW * 1024);
       }
     } else {
       asm volatile("" : "+v"(l));
 #pragma unroll
       for (int j = 0; j < NP / NW; ++j)
-        lds_dma(base + (min((wave + j * NW) * PIECE + l / CH, (unsigned)(n - 1)) * stride + chunk(l, wave + j * NW)), dst + j * NW * 1024);
+        lds_dma(base, min((wave + j * NW) * PIECE + l / CH, (unsigned)(n - 1)) * stride + chunk(l, wave + j * NW), dst + j * NW * 1024);
     }
   }
 };

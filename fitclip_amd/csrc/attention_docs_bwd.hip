@@ -408,11 +408,9 @@ docs_grad_keys_kernel(const Args a) {
 #pragma unroll
       for (int c = 0; c < NTAB; ++c)
         if ((SW == 1 || c % SW == sw) && (c != COL_INV || kInv))
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(column(a, c, qh) + first + lane),
-                                           (__attribute__((address_space(3))) void*)(dst + OFF_TAB + c * COLB), 4, 0, 0);
+          lds_dma_4(column(a, c, qh) + first, lane * 4, dst + OFF_TAB + c * COLB);
       if (lane < 4 * (TQ / 32) && (SW == 1 || sw == SW - 1))
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(block_keys(a, t * (TQ / 32)) + lane),
-                                         (__attribute__((address_space(3))) void*)(dst + OFF_KEYS), 4, 0, 0);
+        lds_dma_4(block_keys(a, t * (TQ / 32)), lane * 4, dst + OFF_KEYS);
     }
   };
   RowOff<T> roff;
