@@ -532,11 +532,27 @@ __device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool count
 
 #endif  // __HIPCC__
 
-// From how many workgroups of 128 rows (keys) on four waves share tiles instead of taking turns over them.  Sharing has a quarter of the
-// traffic, turns have work in smaller pieces; both measured on 12 heads of 1, 2, 3, 6, 12 x 3136 tokens (1.2 to 14 workgroups per compute
-// unit), forward, us: bf16 sharing 61 127 147 246 447, turns 62 113 155 297 576; fp32 (whose products take ten times as long) sharing
-// 354 802 1004 1617, turns 291 570 799 1585, and over 4 x 8192 tokens, 8 per compute unit, 4206 and 4555.
-inline long sharing_from(int kind) { return (kind == PREC_F32 ? 8L : 3L) * device_cus(); }
+// The three shapes of a workgroup (rows: of the forward and of d_q; read keys for rows and rows for keys where d_k and d_v are formed):
+//   SHARED  4 waves x 32 rows share every tile of 64 keys, double-buffered: a quarter of the traffic
+//   TURNS   4 waves over the same 32 rows, each takes every fourth tile of 32 keys into its own LDS; joined at the end.  No barrier in the
+//           loop, four times the waves and a quarter of the longest wave's way
+//   ALONE   a workgroup of one wave over 32 rows: documents of two or three tiles, where a fourth wave would find nothing to take and shared
+//           tiles are of use to one or two of the waves that wait for them
+// `way`: the keys that a row walks over, the mean over the documents (their lengths are on the device).  Measured, us (8 heads, bf16 forward;
+// fp32 forward; fp32 gradients): 20000 rows in documents of 40: shared 26.6, 83, 240, turns -, 88, 262, alone 22.5, 59, 177; of 160: 27.6, 119,
+// 358, turns -, 120, 357, alone 24.9, 88, 248; of 200: 35, 165, 502, turns -, 152, 453, alone 37, 144, 462.  Alone needs its waves to fill the
+// chip: 1200 rows of 77, fp32 gradients, turns 45, alone 64; 2400 rows 63 and 66, of 40 50 and 43.
+// Shared or turns: 12 heads of 1, 2, 3, 6, 12 x 3136 tokens (1.2 to 14 workgroups that share on a compute unit), forward: bf16 shared
+// 61 127 147 246 447, turns 62 113 155 297 576; fp32 (whose products take ten times as long) shared 354 802 1004 1617, turns 291 570 799 1585,
+// and over 4 x 8192 tokens, 8 per compute unit, 4206 and 4555.  Shorter ways in bf16, 8000 rows in documents of 200, 256, 400 (2 per compute
+// unit), gradients: shared 48 34 71, turns 64 57 79.
+enum Shape : int { SHARED, TURNS, ALONE };
+inline Shape shape_for(int kind, long rows, long heads, double way) {
+  const long cus = device_cus(), shared = (rows + 127) / 128 * heads;
+  if (way <= 160. && (rows + 31) / 32 * heads >= 2 * cus) return ALONE;
+  return shared >= (kind == PREC_F32 ? 8 * cus : way <= 512. ? 3 * cus / 2 : 3 * cus) ? SHARED : TURNS;
+}
+inline int tiles_of(Shape s, long rows) { return (int)(s == SHARED ? (rows + 127) / 128 : (rows + 31) / 32); }
 
 int check_docs(const fc_docs* d, const char* what);
 bool rows_aligned(const void* p, int64_t row, int64_t head, int kind);

@@ -4,9 +4,6 @@
 // accumulator IS the operand of O^T = V^T . P^T.  K and V stream through LDS in tiles between the lowest and the highest key that a row of
 // the workgroup sees; a wave skips tiles that none of its 32 rows sees and masks only tiles that one of them sees in part.
 //
-// Two shapes of a workgroup of four waves.  Many rows: 4 x 32 rows share every tile of 64 keys (a quarter of the traffic from L2).  Fewer:
-// the four waves hold the SAME 32 rows, each takes every fourth tile of 32 keys into its own LDS, and their (maximum, sum, O) are joined at
-// the end - four times the waves and a quarter of the longest wave's work, with no barrier in the loop.
 // Few rows over many keys (single tokens that are being written): the key range is cut into `splits` parts on top of that, each part leaves
 // its unnormalised O with (maximum, sum) in scratch, and a second kernel joins them in a fixed order.
 #include "attention_docs.h"
@@ -48,11 +45,11 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 }
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 3)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : KS > 1 && CAP && !BIAS ? 4 : 3)))
 attention_docs_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
-  constexpr int BUFS = KS > 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
-  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && STAGE >= 8192), "the output patches reuse the stages");
+  constexpr int BUFS = RW == 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
+  static_assert((KS == 1 && RW * 32 * ROWB <= BUFS * STAGE) || (RW == 1 && STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * RW];
   __shared__ float shares[KS > 1 ? KS : 1][2][32];
@@ -131,13 +128,13 @@ attention_docs_kernel(const Args a) {
   if (t < t_last) stage(t, 0);
   for (; t < t_last; t += KS, buf ^= BUFS - 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (KS == 1) {
+    if constexpr (RW > 1) {
       __syncthreads();  // tile t is there, and nobody reads tile t - 1 any more
       if (t + KS < t_last) stage(t + KS, buf ^ 1);
     }
     const int k0 = kbeg + t * TK;
     if (k0 >= whi || k0 + TK <= wlo) {  // (wave-uniform)
-      if (KS > 1 && t + KS < t_last) stage(t + KS, 0);
+      if (RW == 1 && t + KS < t_last) stage(t + KS, 0);
       continue;
     }
     const char* kt = stages + buf * STAGE;
@@ -148,7 +145,7 @@ attention_docs_kernel(const Args a) {
 #pragma unroll
     for (int u = 0; u < NT; ++u) read_rows(kt + u * 32 * ROWB, koff, kf[u]);
     ColFrag<T> vf[NT];
-    if constexpr (KS > 1) {
+    if constexpr (RW == 1) {
 #pragma unroll
       for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -161,7 +158,7 @@ attention_docs_kernel(const Args a) {
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
       s[u] = rows_dot(kf[u], qf, s[u]);
     }
-    if constexpr (KS == 1 && !CAP) {  // (on their way under the softmax; a cap has no registers for that)
+    if constexpr (RW > 1 && !CAP) {  // (on their way under the softmax; a cap has no registers for that)
 #pragma unroll
       for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
     }
@@ -187,7 +184,7 @@ attention_docs_kernel(const Args a) {
         for (int i = 0; i < 16; ++i) s[u][i] = pick(bits, i, s[u][i], -kInf);
       }
     }
-    if constexpr (KS == 1 && CAP) {
+    if constexpr (RW > 1 && CAP) {
 #pragma unroll
       for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
     }
@@ -347,16 +344,15 @@ __global__ void __launch_bounds__(256) attention_docs_join_kernel(const Args a) 
 }
 
 struct Plan {
-  bool shared;  // four waves x 32 rows share tiles of keys; otherwise four waves share 32 rows and each takes every fourth tile of keys
+  Shape shape;
   int tiles, splits;
 };
 
 Plan plan_forward(const fc_docs& d) {
   const long group = d.q_heads / d.kv_heads, rows = d.q_rows * group, cus = device_cus();
-  Plan p{true, (int)((rows + 127) / 128), 1};
-  if ((long)p.tiles * d.kv_heads >= sharing_from(d.kind)) return p;
-  p.shared = false;
-  p.tiles = (int)((rows + 31) / 32);
+  Plan p{shape_for(d.kind, rows, d.kv_heads, (double)d.k_rows / d.docs), 0, 1};
+  p.tiles = tiles_of(p.shape, rows);
+  if (p.shape != TURNS) return p;
   const long units = (long)p.tiles * d.kv_heads;
   // keys that a tile walks over, from the mean lengths: the documents that 32 kernel rows touch
   const double mean_rows = std::max(1.0, (double)rows / d.docs), mean_keys = (double)d.k_rows / d.docs;
@@ -371,7 +367,7 @@ size_t part_bytes(const fc_docs& d, const Plan& p) {
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
 int launch_forward(const Args& a, hipStream_t st) {
-  constexpr int lds = (KS > 1 ? KS : 2) * 2 * TK * Tile<T>::kRow;
+  constexpr int lds = (RW > 1 ? 2 : KS) * 2 * TK * Tile<T>::kRow;
   auto kern = attention_docs_kernel<T, RW, KS, TK, CAP, BIAS>;
   if (lds > 60 * 1024 && raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds) != hipSuccess)
     return fail(FC_ELAUNCH, "fc_attention_docs: cannot raise dynamic LDS");
@@ -388,14 +384,15 @@ int launch_forward(const Args& a, hipStream_t st) {
 }
 
 template <typename T, bool CAP, bool BIAS>
-int launch_waves(const Args& a, bool shared, hipStream_t st) {
-  return shared ? launch_forward<T, 4, 1, 64, CAP, BIAS>(a, st) : launch_forward<T, 1, 4, 32, CAP, BIAS>(a, st);
+int launch_waves(const Args& a, Shape shape, hipStream_t st) {
+  if (shape == ALONE) return launch_forward<T, 1, 1, 32, CAP, BIAS>(a, st);
+  return shape == SHARED ? launch_forward<T, 4, 1, 64, CAP, BIAS>(a, st) : launch_forward<T, 1, 4, 32, CAP, BIAS>(a, st);
 }
 
 template <typename T>
-int launch_type(const Args& a, bool cap, bool shared, hipStream_t st) {
-  if (a.slopes) return cap ? launch_waves<T, true, true>(a, shared, st) : launch_waves<T, false, true>(a, shared, st);
-  return cap ? launch_waves<T, true, false>(a, shared, st) : launch_waves<T, false, false>(a, shared, st);
+int launch_type(const Args& a, bool cap, Shape shape, hipStream_t st) {
+  if (a.slopes) return cap ? launch_waves<T, true, true>(a, shape, st) : launch_waves<T, false, true>(a, shape, st);
+  return cap ? launch_waves<T, true, false>(a, shape, st) : launch_waves<T, false, false>(a, shape, st);
 }
 
 }  // namespace
@@ -481,7 +478,7 @@ int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_
   a.part = (float*)scratch;
   a.tiles = p.tiles;
   a.splits = p.splits;
-  return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.shared, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.shared, st);
+  return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.shape, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.shape, st);
 }
 
 }  // extern "C"

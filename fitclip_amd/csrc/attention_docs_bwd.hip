@@ -12,8 +12,7 @@
 //   keys: 32 keys per wave (K and V in registers), tiles of the rows that see them, one query head of the group after the other - the
 //   gradients of shared heads need no further sum.  S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
-// Both have the forward's two shapes: four waves x 32 rows (keys) that share tiles, or four waves that take turns over the tiles of the
-// same 32 and add up at the end - where there are few of them, and each has a long way.
+// Both have the forward's three shapes (attention_docs.h, shape_for).
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -148,8 +147,8 @@ template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(2)))
 docs_grad_rows_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
-  constexpr int BUFS = KS > 1 ? 1 : 2;  // (as in the forward)
-  static_assert((KS == 1 && RW * 32 * ROWB <= 2 * STAGE) || (RW == 1 && STAGE >= 8192 && NT == 1), "the output patches reuse the stages");
+  constexpr int BUFS = RW == 1 ? 1 : 2;  // (as in the forward)
+  static_assert((KS == 1 && RW * 32 * ROWB <= BUFS * STAGE) || (RW == 1 && STAGE >= 8192 && NT == 1), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * RW];
   __shared__ float shares[KS > 1 ? KS : 1][3][32];
@@ -247,7 +246,7 @@ docs_grad_rows_kernel(const Args a) {
   if (t < ntile) stage(t, 0);
   for (; t < ntile; t += KS, buf ^= BUFS - 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (KS == 1) {
+    if constexpr (RW > 1) {
       __syncthreads();
       if (t + KS < ntile) stage(t + KS, buf ^ 1);
     }
@@ -258,7 +257,7 @@ docs_grad_rows_kernel(const Args a) {
     for (int u = 0; u < NT; ++u) {
       const int ku = k0 + 32 * u;
       if (ku >= whi || ku + 32 <= wlo) {  // (wave-uniform)
-        if (KS > 1 && t + KS < ntile) stage(t + KS, 0);
+        if (RW == 1 && t + KS < ntile) stage(t + KS, 0);
         continue;
       }
       const bool full = full_lo <= ku && ku + 32 <= full_hi;
@@ -273,7 +272,7 @@ docs_grad_rows_kernel(const Args a) {
       dp = rows_dot(vf, dof, dp);
       ColFrag<T> kc;  // (on their way under the next step)
       read_cols(kt + u * 32 * ROWB, coff, kc);
-      if constexpr (KS > 1) {
+      if constexpr (RW == 1) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (t + KS < ntile) stage(t + KS, 0);
       }
@@ -373,8 +372,8 @@ docs_grad_keys_kernel(const Args a) {
   constexpr int COLB = TQ * 4;                            // a column's share of a stage
   constexpr int OFF_KEYS = OFF_TAB + 6 * COLB;            // the blocks' four ints
   constexpr int STAGE = OFF_KEYS + 64;
-  constexpr int BUFS = KS > 1 && sizeof(T) == 4 ? 1 : 2;  // (fp32, a wave alone: one, or a second workgroup would not fit the CU)
-  static_assert((KS == 1 && KW * 32 * ROWB <= 2 * STAGE) || (KW == 1 && STAGE >= 8192 && TQ == 32), "the output patches reuse the stages");
+  constexpr int BUFS = KW == 1 && sizeof(T) == 4 ? 1 : 2;  // (fp32, a wave alone: one, or a second workgroup would not fit the CU)
+  static_assert((KS == 1 && KW * 32 * ROWB <= BUFS * STAGE) || (KW == 1 && STAGE >= 8192 && TQ == 32), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -443,7 +442,7 @@ docs_grad_keys_kernel(const Args a) {
   if (g < all) stage(head * a.share + g, t_first + t, 0);
   while (g < all) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if constexpr (KS == 1) __syncthreads();
+    if constexpr (KW > 1) __syncthreads();
     const int now = t_first + t;
     const float slope = BIAS ? a.slopes[head * a.share + g] * kLog2e : 0.f;
     t += KS;
@@ -620,21 +619,17 @@ int pad_rows(const fc_docs& d) { return (int)((d.q_rows + 127) / 128 * 128); }
 
 size_t table_bytes(const fc_docs& d) { return (size_t)pad_rows(d) * d.q_heads * COLS * 4 + (size_t)pad_rows(d) / 32 * 16; }
 
-// Workgroups of the keys kernel: four waves x 32 keys that share tiles of rows, or four waves that take turns over the rows of 32 keys; where
-// that leaves compute units without work, the rows of a key are cut into parts on top of it
 struct KeyPlan {
-  bool shared;
-  int tiles, splits;
+  Shape shape;
+  int tiles, splits;  // splits: parts of the rows of a key, where the keys alone leave compute units without work
 };
 KeyPlan plan_keys(const fc_docs& d) {
-  const long cus = device_cus();
-  KeyPlan p{true, (int)((d.k_rows + 127) / 128), 1};
-  if ((long)p.tiles * d.kv_heads >= sharing_from(d.kind)) return p;
-  p.shared = false;
-  p.tiles = (int)((d.k_rows + 31) / 32);
+  const double way = (double)d.q_rows / std::max(1, d.docs) * (d.q_heads / d.kv_heads);  // of a key through the rows, the mean
+  KeyPlan p{shape_for(d.kind, d.k_rows, d.kv_heads, way), 0, 1};
+  p.tiles = tiles_of(p.shape, d.k_rows);
+  if (p.shape != TURNS) return p;
   const long units = std::max(1L, (long)p.tiles * d.kv_heads);
-  const double rows = (double)d.q_rows / std::max(1, d.docs) * (d.q_heads / d.kv_heads);  // mean way of a key through the rows
-  p.splits = (int)std::max(1L, std::min({4 * cus / units, (long)(rows / 256.0), 64L}));
+  p.splits = (int)std::max(1L, std::min({4L * device_cus() / units, (long)(way / 256.0), 64L}));
   return p;
 }
 
@@ -659,22 +654,26 @@ int launch_grads(Args a, const KeyPlan& p, hipStream_t st) {
   constexpr int row = Tile<T>::kRow;
   const char *rows = "fc_attention_docs_backward (rows)", *keys = "fc_attention_docs_backward (keys)";
   const long heads = (long)a.kv_heads * a.share;
+  const Shape by = shape_for(sizeof(T) == 4 ? PREC_F32 : PREC_BF16, a.rows, heads, (double)a.k_rows / a.docs);
   int rc;
-  a.tiles = (a.rows + 127) / 128;
-  if (a.tiles * heads >= sharing_from(sizeof(T) == 4 ? PREC_F32 : PREC_BF16)) {
+  a.tiles = tiles_of(by, a.rows);
+  if (by == SHARED)
     rc = launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
-  } else {
-    a.tiles = (a.rows + 31) / 32;
+  else if (by == TURNS)
     rc = launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS>, a.tiles * heads, 4, 4 * 64 * row, a, rows, st);
-  }
+  else
+    rc = launch_docs(docs_grad_rows_kernel<T, 1, 1, 32, CAP, BIAS>, a.tiles * heads, 1, 64 * row, a, rows, st);
   if (rc != FC_OK) return rc;
   a.tiles = p.tiles;
   a.splits = p.splits;
   const long units = (long)p.tiles * p.splits * a.kv_heads;
-  if (p.shared)
+  constexpr int alone = (sizeof(T) == 4 ? 1 : 2) * (64 * row + 6 * 128 + 64);  // a wave's stages
+  if (p.shape == SHARED)
     rc = launch_docs(docs_grad_keys_kernel<T, 4, 1, 64, CAP, BIAS>, units, 4, 2 * (128 * row + 6 * 256 + 64), a, keys, st);
+  else if (p.shape == TURNS)
+    rc = launch_docs(docs_grad_keys_kernel<T, 1, 4, 32, CAP, BIAS>, units, 4, 4 * alone, a, keys, st);
   else
-    rc = launch_docs(docs_grad_keys_kernel<T, 1, 4, 32, CAP, BIAS>, units, 4, (sizeof(T) == 4 ? 4 : 8) * (64 * row + 6 * 128 + 64), a, keys, st);
+    rc = launch_docs(docs_grad_keys_kernel<T, 1, 1, 32, CAP, BIAS>, units, 1, alone, a, keys, st);
   if (rc == FC_OK && p.splits > 1)
     rc = launch_docs(docs_grad_join_kernel<T, CAP, BIAS>, ((long)a.k_rows + 3) / 4 * a.kv_heads, 4, 0, a, "fc_attention_docs_backward (join)", st);
   if (rc != FC_OK || !a.d_slopes) return rc;

@@ -152,22 +152,26 @@ def test_attention_of_few_rows_over_many_keys(dtype, q_len, k_len, causal):
     _check_forward(q, k, v, q_len, k_len, causal=causal)
 
 
-@pytest.mark.parametrize("dtype,heads", [(torch.float32, 352), (torch.bfloat16, 144)])
-def test_attention_four_wave_tiles(dtype, heads):
+# enough rows for waves that work alone (a mean below 160), and for 128 rows that share a tile of keys (6 or 8 tiles of 128 rows a head: more
+# than eight, bf16 three, workgroups per compute unit)
+MANY = [(torch.float32, 352, [300, 17, 129, 0, 64, 250]), (torch.bfloat16, 144, [300, 17, 129, 0, 64, 250]),
+        (torch.float32, 352, [600, 17, 129, 0, 250]), (torch.bfloat16, 144, [600, 17, 129, 0, 250])]
+
+
+@pytest.mark.parametrize("dtype,heads,q_len", MANY)
+def test_attention_four_wave_tiles(dtype, heads, q_len):
     """Enough rows that 128 of them share a tile of keys, in documents that end inside tiles."""
-    q_len = [300, 17, 129, 0, 64, 250]
-    rows = sum(q_len)
-    # 6 tiles of 128 rows a head: more than eight (bf16: three) workgroups per compute unit
+    rows, most = sum(q_len), max(q_len)
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     for causal in (False, True):
         out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=causal, cap=20.0)
         some = [0, 31, heads - 1]  # (the reference is slow: three heads of them)
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, cap=20.0)
-        ds = R.score_error(ref, 300, cap=20.0)
-        _within("out", out[:, some], ref["out"], R.out_bound(ref, v, dtype, 300, ds))
+        ds = R.score_error(ref, most, cap=20.0)
+        _within("out", out[:, some], ref["out"], R.out_bound(ref, v, dtype, most, ds))
         alone = [ops.attention_docs(q[:, h:h + 1], k[:, h:h + 1], v[:, h:h + 1], R.offsets(q_len), causal=causal, cap=20.0)[0] for h in some]
         for h, other in zip(some, alone):  # single waves form the same sums up to the order of the tiles
-            _within("one head", other, ref["out"][:, some.index(h):some.index(h) + 1], R.out_bound(ref, v, dtype, 300, ds)[:, :1])
+            _within("one head", other, ref["out"][:, some.index(h):some.index(h) + 1], R.out_bound(ref, v, dtype, most, ds)[:, :1])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -270,10 +274,9 @@ def test_gradients_of_other_numbers_of_keys(dtype, q_len, k_len, causal):
     _check_gradients(q, k, v, q_len, k_len, causal=causal)
 
 
-@pytest.mark.parametrize("dtype,heads", [(torch.float32, 352), (torch.bfloat16, 144)])
-def test_gradients_four_wave_tiles(dtype, heads):
-    q_len = [300, 17, 129, 0, 64, 250]
-    rows = sum(q_len)
+@pytest.mark.parametrize("dtype,heads,q_len", MANY)
+def test_gradients_four_wave_tiles(dtype, heads, q_len):
+    rows, most = sum(q_len), max(q_len)
     q, k, v = _operands(rows, rows, heads, heads, dtype, seed=4, layout="fused")
     d_out = _rand(rows, heads, 64, seed=5, dtype=dtype)
     for causal in (False, True):
@@ -281,9 +284,72 @@ def test_gradients_four_wave_tiles(dtype, heads):
         grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=causal)
         some = [0, heads - 1]
         ref = R.attention(q[:, some], k[:, some], v[:, some], q_len, causal=causal, d_out=d_out[:, some])
-        bounds = R.grad_bounds(ref, q[:, some], k[:, some], v[:, some], d_out[:, some], dtype, 300, R.score_error(ref, 300))
+        bounds = R.grad_bounds(ref, q[:, some], k[:, some], v[:, some], d_out[:, some], dtype, most, R.score_error(ref, most))
         for name, got in zip(("d_q", "d_k", "d_v"), grads):
             _within(name, got[:, some], ref[name], bounds[name])
+
+
+def _some_heads(q, k, v, d_out, q_len, k_len, kv_heads, **how):
+    """The reference of the given key heads' query heads alone (it is slow), with what to take of the operators' results."""
+    group = q.shape[1] // k.shape[1]
+    heads = [h * group + g for h in kv_heads for g in range(group)]
+    if how.get("slopes") is not None:
+        how["slopes"] = how["slopes"][heads]
+    keys, (q, k, v, d_out) = max(k_len or q_len), (q[:, heads], k[:, kv_heads], v[:, kv_heads], d_out[:, heads])
+    ref = R.attention(q, k, v, q_len, k_len, d_out=d_out, **how)
+    ds = R.score_error(ref, keys, how.get("slopes"), cap=how.get("cap", 0.0))
+    return ref, R.out_bound(ref, v, q.dtype, keys, ds), R.grad_bounds(ref, q, k, v, d_out, q.dtype, keys, ds, how.get("cap", 0.0), how.get("slopes")), heads
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,cross,how", [(24, 24, False, {}), (48, 24, False, dict(causal=True, cap=3.0)),
+                                                      (30, 30, True, dict(causal=True, slopes=True, prefix=True)),
+                                                      (27, 27, True, dict(cap=20.0, slopes=True))])
+def test_many_short_documents(dtype, heads, kv_heads, cross, how):
+    """More than two waves per compute unit, each alone with its rows or keys: documents of 0 to 70 tokens."""
+    g = torch.Generator().manual_seed(31)
+    q_len = torch.randint(0, 71, (22,), generator=g).tolist() + [70, 0, 1]
+    k_len = torch.randint(0, 71, (22,), generator=g).tolist() + [1, 70, 0] if cross else None
+    how = dict(how)
+    if how.get("prefix"):
+        how["prefix"] = torch.randint(-3, 60, (25,), generator=g, dtype=torch.int32).to(DEV)
+    if how.get("slopes"):
+        how["slopes"] = (0.3 * torch.rand(heads, generator=g)).to(DEV)
+    q, k, v = _operands(sum(q_len), sum(k_len or q_len), heads, kv_heads, dtype, seed=32, layout="apart" if cross else "fused")
+    d_out = _rand(*q.shape, seed=35, dtype=dtype)
+    q_off, k_off = R.offsets(q_len), R.offsets(k_len) if cross else None
+    out, stats = ops.attention_docs(q, k, v, q_off, k_off, **how)
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, q_off, k_off, slope_grad="slopes" in how, **how)
+    some = [0, kv_heads - 1]
+    ref, out_bound, bounds, of = _some_heads(q, k, v, d_out, q_len, k_len, some, **how)
+    _within("out", out[:, of], ref["out"], out_bound)
+    for name, got, which in zip(("d_q", "d_k", "d_v"), grads, (of, some, some)):
+        _within(name, got[:, which], ref[name], bounds[name])
+    if "slopes" in how:
+        _within("d_slopes", grads[3][of], ref["d_slopes"], bounds["d_slopes"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_short_documents_with_values_behind_masks(dtype):
+    """NaN and infinities of keys that a row does not see reach nobody, where a wave works alone."""
+    q_len = [29, 40, 3, 64] * 6
+    rows, heads = sum(q_len), 24
+    q, k, v = _operands(rows, rows, heads, heads, dtype, seed=33, layout="fused")
+    off, d_out = R.offsets(q_len), _rand(rows, heads, 64, seed=34, dtype=dtype)
+    some, start = [0, 23], 29 + 40  # (start: the third document, of three rows)
+    ref, out_bound, bounds, _ = _some_heads(q, k, v, d_out, q_len, None, some, causal=True)
+    k[start + 1], v[start + 1] = math.nan, math.inf  # seen by the document's last two rows alone
+    out, stats = ops.attention_docs(q, k, v, off, causal=True)
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, off, causal=True)
+    reached = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    reached[start + 1:start + 3] = True
+    assert not torch.isfinite(out[reached]).all() and torch.isfinite(stats[~reached]).all()
+    own = reached.clone()
+    own[start] = True  # keys that a reached row sees
+    for name, got, bound, kept in (("out", out, out_bound, ~reached), ("d_q", grads[0], bounds["d_q"], ~reached),
+                                   ("d_k", grads[1], bounds["d_k"], ~own), ("d_v", grads[2], bounds["d_v"], ~own)):
+        kept = kept.cpu()
+        _within(name, got[:, some].cpu()[kept], ref[name].cpu()[kept], bound.cpu().expand(rows, len(some), 64)[kept])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
