@@ -9,6 +9,7 @@
 #include "attention_docs.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace fc {
 namespace docs {
@@ -45,7 +46,7 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 }
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : KS > 1 && CAP && !BIAS ? 4 : 3)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : RW == 1 && !(CAP && BIAS) ? 4 : 3)))
 attention_docs_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
   constexpr int BUFS = RW == 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
@@ -166,7 +167,7 @@ attention_docs_kernel(const Args a) {
     // scores in log2 units; without a bias they are scaled in the exponent's fma
     if constexpr (CAP) {
 #pragma unroll
-      for (int u = 0; u < NT; ++u) bend(s[u], a.cap_in);
+      for (int u = 0; u < NT; ++u) bend(a, s[u]);
     }
     if constexpr (BIAS) {
       const float at = (float)(row.pos - k0 - 4 * hh);
@@ -439,7 +440,13 @@ Args make_args(const fc_docs& d) {
   a.rows = (int)(d.q_rows * (d.q_heads / d.kv_heads));
   a.causal = d.causal; a.fill = d.fill;
   a.c = (float)((double)(d.cap > 0.f ? d.cap : d.scale) * 1.4426950408889634);
-  a.cap_in = d.cap > 0.f ? (float)((double)d.scale / d.cap) : 0.f;
+  if (d.cap > 0.f) {
+    const double u = (double)d.scale / d.cap;
+    a.cap_in = (float)u;
+    a.near[0] = (float)u;
+    for (int k = 0; k < 3; ++k) a.near[k + 1] = (float)(kNear[k] * std::pow(u, 2 * k + 3));
+    a.near_end = u < 1e5 ? (float)(kTanhNear / u) : 0.f;  // (beyond, the coefficients leave fp32)
+  }
   a.scale = d.scale;
   a.splits = 1;
   return a;

@@ -278,7 +278,7 @@ docs_grad_rows_kernel(const Args a) {
       }
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
       const float at = BIAS ? (float)(row.pos - ku - 4 * hh) : 0.f;
-      if constexpr (CAP) bend(s, a.cap_in);
+      if constexpr (CAP) bend(a, s);
       f32x16 p;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -486,7 +486,7 @@ docs_grad_keys_kernel(const Args a) {
       ColFrag<T> cols;
       if constexpr (sizeof(T) == 2) read_cols(dt, coff, cols);  // (on their way under the next step; fp32: no registers for that)
       __builtin_amdgcn_sched_barrier(0);  // (what the next step needs is formed there, not kept through the products)
-      if constexpr (CAP) bend(s, a.cap_in);
+      if constexpr (CAP) bend(a, s);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         if constexpr (sizeof(T) == 4) asm volatile("" ::: "memory");  // (four rows of the table at a time)
