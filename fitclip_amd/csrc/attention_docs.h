@@ -77,10 +77,16 @@ __device__ __forceinline__ float swap_sum(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));  // (lanes l and l + 32 hold the same row)
-  return __builtin_amdgcn_readfirstlane(v);
+template <int N>
+__device__ __forceinline__ int rotated(int v) {  // within 16 lanes, with no way through LDS
+  return __builtin_amdgcn_update_dpp(v, v, 0x120 + N, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int wave_min_i(int v) {  // (lanes l and l + 32 hold the same row)
+  v = min(v, rotated<8>(v));
+  v = min(v, rotated<4>(v));
+  v = min(v, rotated<2>(v));
+  v = min(v, rotated<1>(v));
+  return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 __device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
 

@@ -46,7 +46,7 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 }
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : RW == 1 && !(CAP && BIAS) ? 4 : 3)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : RW == 1 && !(CAP && (BIAS || KS == 1)) ? 4 : 3)))
 attention_docs_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
   constexpr int BUFS = RW == 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
@@ -62,6 +62,13 @@ attention_docs_kernel(const Args a) {
   const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
   const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
+  RowFrag<T> qf;  // (sent for first: on its way under the search for the rows' documents)
+  float slope = 0.f;
+  {
+    const int m = min(m0 + r, a.rows - 1), token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+    qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
+    if constexpr (BIAS) slope = a.slopes[qh] * kLog2e;
+  }
   const Row row = find_row(a, m0, lane);
   const bool sees = row.lo < row.hi;
   // rows of no document neither widen the range nor ask for a mask; rows that see nothing always ask for one
@@ -89,14 +96,6 @@ attention_docs_kernel(const Args a) {
     const int part = (int)((unsigned)(ntile + a.splits - 1) / (unsigned)a.splits);
     t_first = min(ntile, split * part);
     t_last = min(ntile, t_first + part);
-  }
-
-  RowFrag<T> qf;
-  float slope = 0.f;
-  {
-    const int m = min(m0 + r, a.rows - 1), token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-    qf.load(a.q + token * a.q_row + qh * a.q_head, hh);
-    if constexpr (BIAS) slope = a.slopes[qh] * kLog2e;
   }
 
   const char* kbase = a.k + head * a.k_head;

@@ -157,7 +157,16 @@ docs_grad_rows_kernel(const Args a) {
   const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, tile = a.tiles - 1 - blockIdx.x / heads;
   const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
+  // (sent for first: on their way under the search for the rows' documents)
+  const int m = min(m0 + r, a.rows - 1);
+  RowFrag<T> qf, dof;
+  qf.load(a.q + m * a.q_row + qh * a.q_head, hh);
+  dof.load(a.d_out + m * a.do_row + qh * a.do_head, hh);
+  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * heads + qh) * 2);
+  RowFrag<T> of;
+  of.load(a.out + m * a.out_row + qh * a.out_head, hh);
   const Row row = find_row(a, m0, lane);
+  float D = swap_sum(dot(of, dof));
   const bool sees = row.lo < row.hi;
   const int wlo = wave_min_i(sees ? row.lo : INT_MAX), whi = wave_max_i(sees ? row.hi : -INT_MAX);
   const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);
@@ -179,17 +188,6 @@ docs_grad_rows_kernel(const Args a) {
   }
   const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
 
-  const int m = min(m0 + r, a.rows - 1);
-  RowFrag<T> qf, dof;
-  qf.load(a.q + m * a.q_row + qh * a.q_head, hh);
-  dof.load(a.d_out + m * a.do_row + qh * a.do_head, hh);
-  float D;
-  {
-    RowFrag<T> of;
-    of.load(a.out + m * a.out_row + qh * a.out_head, hh);
-    D = swap_sum(dot(of, dof));
-  }
-  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * heads + qh) * 2);
   // a row that sees nothing weighs nothing: its maximum is taken as +inf
   float top = sees ? st[0] : kInf, inv = sees ? 1.f / st[1] : 0.f;
   if constexpr (sizeof(T) == 2) {
@@ -253,12 +251,11 @@ docs_grad_rows_kernel(const Args a) {
     const int k0 = kbeg + t * TK;
     const char* kt = stages + buf * STAGE;
     const char* vt = kt + TK * ROWB;
-#pragma unroll 1
-    for (int u = 0; u < NT; ++u) {
+    const auto part = [&](int u) {
       const int ku = k0 + 32 * u;
       if (ku >= whi || ku + 32 <= wlo) {  // (wave-uniform)
         if (RW == 1 && t + KS < ntile) stage(t + KS, 0);
-        continue;
+        return;
       }
       const bool full = full_lo <= ku && ku + 32 <= full_hi;
       f32x16 s, dp;
@@ -304,6 +301,12 @@ docs_grad_rows_kernel(const Args a) {
       }
       __builtin_amdgcn_sched_barrier(0);
       cols_dot(kc, s, o);
+    };
+    if constexpr (NT == 1) {  // (no loop: hipcc would copy all of o at its end)
+      part(0);
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < NT; ++u) part(u);
     }
   }
   if constexpr (BIAS) {
@@ -381,15 +384,14 @@ docs_grad_keys_kernel(const Args a) {
   const int tile = rest % a.tiles, split = rest / a.tiles;  // (earlier keys first: causal, they cost most)
   const int k0 = tile * KW * 32, kw = k0 + (KS > 1 ? 0 : wave * 32);
 
-  int r_lo, r_hi;
-  rows_of_keys(a, k0, KW * 32, lane, r_lo, r_hi);
-  const int t_first = r_lo / TQ, steps = r_hi > r_lo ? (r_hi + TQ - 1) / TQ - t_first : 0;  // tiles of rows, for each query head of the group
-
   const int key = kw + r;
   const long kc = min(key, a.k_rows - 1);
   RowFrag<T> kf, vf;
   kf.load(a.k + kc * a.k_row + head * a.k_head, hh);
   vf.load(a.v + kc * a.v_row + head * a.v_head, hh);
+  int r_lo, r_hi;
+  rows_of_keys(a, k0, KW * 32, lane, r_lo, r_hi);
+  const int t_first = r_lo / TQ, steps = r_hi > r_lo ? (r_hi + TQ - 1) / TQ - t_first : 0;  // tiles of rows, for each query head of the group
 
   constexpr int SW = KS > 1 ? 1 : KW;  // waves that bring a tile together
   const int sw = KS > 1 ? 0 : wave;
