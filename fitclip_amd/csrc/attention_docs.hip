@@ -46,9 +46,12 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 }
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : RW == 1 && !(CAP && (BIAS || KS == 1)) ? 4 : 3)))
+__global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? (RW == 1 ? 3 : 2) : RW == 1 && !(CAP && (BIAS || KS == 1)) ? 4 : 3)))
 attention_docs_kernel(const Args a) {
-  constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
+  // a stage: K rows, then V rows.  fp32, a wave that reads its tile alone: K rows, and V in the same place once they have been read, so that
+  // LDS leaves room for a third wave on a SIMD
+  constexpr bool kApart = RW == 1 && sizeof(T) == 4;
+  constexpr int ROWB = Tile<T>::kRow, STAGE = (kApart ? 1 : 2) * TK * ROWB, NT = TK / 32;
   constexpr int BUFS = RW == 1 ? 1 : 2;  // (a wave that reads its tile alone has it in registers before the next one is sent for)
   static_assert((KS == 1 && RW * 32 * ROWB <= BUFS * STAGE) || (RW == 1 && STAGE >= 8192), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -106,11 +109,13 @@ attention_docs_kernel(const Args a) {
   kin.init((unsigned)a.k_row, sw, lane);
   vin.init((unsigned)a.v_row, sw, lane);
   char* const stages = smem + (KS > 1 ? wave * STAGE : 0);
+  auto stage_v = [&](int t, char* dst) {
+    vin.template rows<TK>(dst, vbase + (long)(kbeg + t * TK) * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, sw);
+  };
   auto stage = [&](int t, int buf) {
     char* dst = stages + buf * STAGE;
-    const long first = kbeg + t * TK;
-    kin.template rows<TK>(dst, kbase + first * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, sw);
-    vin.template rows<TK>(dst + TK * ROWB, vbase + first * a.v_row, (unsigned)a.v_row, kend - kbeg - t * TK, sw);
+    kin.template rows<TK>(dst, kbase + (long)(kbeg + t * TK) * a.k_row, (unsigned)a.k_row, kend - kbeg - t * TK, sw);
+    if constexpr (!kApart) stage_v(t, dst + TK * ROWB);
   };
 
   RowOff<T> koff;
@@ -138,14 +143,17 @@ attention_docs_kernel(const Args a) {
       continue;
     }
     const char* kt = stages + buf * STAGE;
-    const char* vt = kt + TK * ROWB;
+    const char* vt = kApart ? kt : kt + TK * ROWB;
     const bool full = full_lo <= k0 && k0 + TK <= full_hi;
     f32x16 s[NT];
     RowFrag<T> kf[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) read_rows(kt + u * 32 * ROWB, koff, kf[u]);
     ColFrag<T> vf[NT];
-    if constexpr (RW == 1) {
+    if constexpr (kApart) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      stage_v(t, stages);
+    } else if constexpr (RW == 1) {
 #pragma unroll
       for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -213,6 +221,14 @@ attention_docs_kernel(const Args a) {
         s[u][i] = __builtin_amdgcn_exp2f(BIAS ? s[u][i] - mm : __builtin_fmaf(s[u][i], a.c, -mm));
         l += s[u][i];
       }
+    if constexpr (kApart) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < NT; ++u) read_cols(vt + u * 32 * ROWB, voff, vf[u]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (t + KS < t_last) stage(t + KS, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int u = 0; u < NT; ++u) cols_dot(vf[u], s[u], o);
   }
@@ -367,7 +383,7 @@ size_t part_bytes(const fc_docs& d, const Plan& p) {
 
 template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
 int launch_forward(const Args& a, hipStream_t st) {
-  constexpr int lds = (RW > 1 ? 2 : KS) * 2 * TK * Tile<T>::kRow;
+  constexpr int lds = (RW > 1 ? 2 : KS) * (RW == 1 && sizeof(T) == 4 ? 1 : 2) * TK * Tile<T>::kRow;
   auto kern = attention_docs_kernel<T, RW, KS, TK, CAP, BIAS>;
   if (lds > 60 * 1024 && raise_dynamic_lds(reinterpret_cast<const void*>(kern), lds) != hipSuccess)
     return fail(FC_ELAUNCH, "fc_attention_docs: cannot raise dynamic LDS");
