@@ -423,8 +423,8 @@ int check_docs(const fc_docs* d, const char* what) {
     return fail(FC_EINVAL, "%s: %d query heads over %d key heads: a multiple is needed", what, d->q_heads, d->kv_heads);
   if (d->q_rows * d->q_heads >= (1LL << 31) - 256 || d->k_rows >= (1LL << 31) - 256)
     return fail(FC_EINVAL, "%s: %ld rows x %d heads or %ld keys reach 2^31", what, (long)d->q_rows, d->q_heads, (long)d->k_rows);
-  if (!(d->scale > 0.f) || !(d->scale < kInf)) return fail(FC_EINVAL, "%s: scale %g: a positive number is needed", what, d->scale);
-  if (!(d->cap >= 0.f) || !(d->cap < kInf)) return fail(FC_EINVAL, "%s: cap %g: 0 (none) or a positive number is needed", what, d->cap);
+  if (!(d->scale > 0.f) || !(d->scale <= 1e30f)) return fail(FC_EINVAL, "%s: scale %g: a positive number up to 1e30 is needed", what, d->scale);
+  if (!(d->cap >= 0.f) || !(d->cap <= 1e30f)) return fail(FC_EINVAL, "%s: cap %g: 0 (none) or a positive number up to 1e30 is needed", what, d->cap);
   if (d->prefix && !d->causal) return fail(FC_EINVAL, "%s: a prefix mask needs causal = 1", what);
   if (d->docs == 0 || (d->q_rows == 0 && d->k_rows == 0)) return FC_OK;
   if ((d->q_rows && !d->q) || !d->q_offsets || !d->k_offsets || (d->k_rows && (!d->k || !d->v))) return fail(FC_EINVAL, "%s: null operand", what);
@@ -432,6 +432,7 @@ int check_docs(const fc_docs* d, const char* what) {
   if ((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) ||
       ((d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head) * size & 15))
     return fail(FC_EINVAL, "%s: rows and heads must start on 16-byte boundaries", what);
+  if ((d->q_row | d->q_head | d->k_row | d->k_head | d->v_row | d->v_head) < 0) return fail(FC_EINVAL, "%s: negative strides", what);
   if (d->q_row * size >= 1 << 25 || d->k_row * size >= 1 << 25 || d->v_row * size >= 1 << 25)
     return fail(FC_EINVAL, "%s: rows of q, k or v lie 32 MiB or more apart", what);
   return FC_OK;
@@ -456,7 +457,7 @@ Args make_args(const fc_docs& d) {
   a.causal = d.causal; a.fill = d.fill;
   a.c = (float)((double)(d.cap > 0.f ? d.cap : d.scale) * 1.4426950408889634);
   if (d.cap > 0.f) {
-    const double u = (double)d.scale / d.cap;
+    const double u = std::min((double)d.scale / d.cap, 1e30);  // (beyond, every score but 0 is at the cap all the same)
     a.cap_in = (float)u;
     a.near[0] = (float)u;
     for (int k = 0; k < 3; ++k) a.near[k + 1] = (float)(kNear[k] * std::pow(u, 2 * k + 3));

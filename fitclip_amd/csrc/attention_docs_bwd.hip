@@ -708,7 +708,11 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
   const int rc = docs::check_docs(d, "fc_attention_docs_backward");
   if (rc != FC_OK) return rc;
   if (d_slopes && !d->slopes) return fail(FC_EINVAL, "fc_attention_docs_backward: a gradient of slopes that are not given");
-  if (d->docs == 0 || (d->q_rows == 0 && d->k_rows == 0)) return FC_OK;
+  if (d->docs == 0 || (d->q_rows == 0 && d->k_rows == 0)) {
+    docs::Args none{};  // (sums over no rows)
+    none.d_slopes = d_slopes;
+    return d_slopes ? docs::launch_docs(docs::docs_grad_slopes_kernel, d->q_heads, 16, 0, none, "fc_attention_docs_backward (slopes)", st) : FC_OK;
+  }
   if ((d->q_rows && (!out || !stats || !d_out || !d_q)) || (d->k_rows && (!d_k || !d_v)))
     return fail(FC_EINVAL, "fc_attention_docs_backward: null operand");
   if (!docs::rows_aligned(out, out_row, out_head, d->kind) || !docs::rows_aligned(d_out, do_row, do_head, d->kind) ||

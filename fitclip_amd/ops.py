@@ -549,6 +549,28 @@ def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [rows, heads, dim] views touch the same bytes.  Views of one fused projection lie side by side in its rows (or heads)."""
+    if not a.numel() or not b.numel():
+        return False
+    size = a.element_size()
+    span = lambda t, *axes: sum((t.shape[i] - 1) * t.stride(i) for i in axes) * size + t.shape[2] * size  # noqa: E731
+    at = b.data_ptr() - a.data_ptr()
+    if at >= span(a, 0, 1) or -at >= span(b, 0, 1):
+        return False
+    for inner, outer in ((1, 0), (0, 1)):  # the same step from row to row: disjoint where what lies between two steps is
+        step, one, two = a.stride(outer) * size, span(a, inner), span(b, inner)
+        if a.stride(outer) == b.stride(outer) and one <= step and two <= step and at % step >= one and at % step + two <= step:
+            return False
+    return True
+
+
+def _apart(t: torch.Tensor, name: str, **others: torch.Tensor) -> None:
+    for other, o in others.items():
+        if _meet(t, o):
+            raise ValueError(f"{name} overlaps {other}")
+
+
 def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
     for name, t in tensors.items():
         if t is None:
@@ -577,7 +599,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
     projection) turns by positions[row, axis(i)] * inv_freq[i].  positions int32 [rows, axes] (or [rows]); inv_freq float32
     [pairs], 2 pairs <= dim, the dimensions behind them are copied; `sections`: how many pairs turn with each axis; pairs are
     (i, i + pairs), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in 64 bits: exact at far positions.  `inverse` turns
-    back - the gradient.  `out` may be x (in place)."""
+    back - the gradient.  `out` may be x (in place), and must not overlap it otherwise."""
     _heads(x, "x", x.dtype, None)
     positions = positions[:, None] if positions.dim() == 1 else positions
     rows, heads, dim = x.shape
@@ -594,8 +616,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
         raise ValueError(f"{axes} sections that sum up to {pairs} pairs are needed, got {sections}")
     if out is not None:
         _written(out, "out", x)
-        if out.data_ptr() == x.data_ptr() and _strides(out) != _strides(x):
-            raise ValueError("in place needs the same strides")
+        if (out.data_ptr() != x.data_ptr() or _strides(out) != _strides(x)) and _meet(out, x):
+            raise ValueError("out overlaps x: in place needs the same place and strides")
     index = x.get_device()
     _on_device(index, x=x, positions=positions, inv_freq=inv_freq, out=out)
     if out is None:
@@ -625,9 +647,13 @@ def _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scal
     _vector(slopes, "slopes", torch.float32, q.shape[1])
     if prefix is not None and not causal:
         raise ValueError("a prefix mask needs causal=True")
-    if not 0 < scale < float("inf") or not 0 <= cap < float("inf"):
-        raise ValueError(f"scale must be positive and cap 0 (none) or positive, got {scale} and {cap}")
+    if not 0 < scale <= 1e30 or not 0 <= cap <= 1e30:
+        raise ValueError(f"scale must be positive and cap 0 (none) or positive, neither above 1e30, got {scale} and {cap}")
     _on_device(q.get_device(), q=q, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, prefix=prefix, slopes=slopes)
+
+
+def _fine(t: torch.Tensor, dtype: torch.dtype, n: int, index: int) -> bool:
+    return t.dtype is dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.get_device() == index
 
 
 def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill) -> "_lib.fc_docs":
@@ -638,9 +664,10 @@ def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fil
     if not (len(q_shape) == 3 == len(k_shape) and k_shape == v.shape and q_shape[2] == 64 == k_shape[2] and kind is not None
             and q.dtype is k.dtype is v.dtype and q_stride[2] == 1 == k_stride[2] == v_stride[2] and q_shape[0] and k_shape[0]
             and k_shape[1] and q_shape[1] and not q_shape[1] % k_shape[1] and index >= 0 and index == k.get_device() == v.get_device()
-            and index == q_offsets.get_device() and q_offsets.dtype is torch.int32 and q_offsets.dim() == 1 and q_offsets.numel()
-            and q_offsets.is_contiguous() and k_offsets is None and k_shape[0] == q_shape[0] and prefix is None and slopes is None
-            and scale > 0 and cap == 0 and scale < float("inf")):
+            and (docs := q_offsets.numel() - 1) >= 0 and _fine(q_offsets, torch.int32, docs + 1, index)
+            and (k_shape[0] == q_shape[0] if k_offsets is None else _fine(k_offsets, torch.int32, docs + 1, index))
+            and (prefix is None or causal and _fine(prefix, torch.int32, docs, index))
+            and (slopes is None or _fine(slopes, torch.float32, q_shape[1], index)) and 0 < scale <= 1e30 and 0 <= cap <= 1e30):
         _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale)
     q_heads, k_heads = q_shape[1], k_shape[1]
     q_many, k_many = q_shape[0] > 1, k_shape[0] > 1
@@ -666,12 +693,15 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
     key gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
 
     Rows behind the last document are left as they were in a given `out` (which may not overlap k or v), and 0 otherwise."""
+    if out is not None:
+        _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
+        _written(out, "out", q)
+        _apart(out, "out", k=k, v=v)
     d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, out is None)
     device, index = q.device, q.get_device()
     if out is None:
         out = (torch.empty if d.docs else torch.zeros)(q.shape, dtype=q.dtype, device=device)
     else:
-        _written(out, "out", q)
         _on_device(index, out=out)
     stats = torch.empty((q.shape[0], q.shape[1], 2), dtype=torch.float32, device=device)
     lib = _lib.load()
@@ -694,33 +724,45 @@ def attention_docs_backward(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     """Gradients of `attention_docs` (same operands and masks; `out` and `stats` are its results) from the gradient `d_out` of its
     output: (d_q, d_k, d_v), and d_slopes float32 [heads] if `slope_grad`.  Gradients of shared key heads are summed over their query
     heads; all sums have a fixed order.  Given d_q / d_k / d_v (strided rows and heads, e.g. the columns of a fused projection's
-    gradient) are written into, rows of no document left as they were; where none is given those rows get 0."""
-    given = [d_q, d_k, d_v]
-    fill = all(t is None for t in given)
-    _heads(q, "q", q.dtype)
-    for t, name in ((d_out, "d_out"), (out, "out")):
-        _heads(t, name, q.dtype)
-        if t.shape != q.shape:
-            raise ValueError(f"{name} must be {tuple(q.shape)}, got {tuple(t.shape)}")
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (*q.shape[:2], 2) or not stats.is_contiguous():
-        raise ValueError(f"stats must be contiguous float32 {(*q.shape[:2], 2)}, got {stats.dtype} {tuple(stats.shape)}")
+    gradient) are written into, rows of no document left as they were; where none is given those rows get 0.  They must not overlap
+    the operands or each other."""
+    fill = d_q is None and d_k is None and d_v is None
+    shape = q.shape
+    if not (len(shape) == 3 and d_out.shape == shape == out.shape and d_out.dtype is q.dtype is out.dtype and d_out.stride(2) == 1 == out.stride(2)
+            and stats.dtype is torch.float32 and stats.shape == (shape[0], shape[1], 2) and stats.is_contiguous()):
+        _heads(q, "q", q.dtype)
+        for t, name in ((d_out, "d_out"), (out, "out")):
+            _heads(t, name, q.dtype)
+            if t.shape != shape:
+                raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if stats.dtype != torch.float32 or tuple(stats.shape) != (*shape[:2], 2) or not stats.is_contiguous():
+            raise ValueError(f"stats must be contiguous float32 {(*shape[:2], 2)}, got {stats.dtype} {tuple(stats.shape)}")
     if slope_grad and slopes is None:
         raise ValueError("slope_grad needs slopes")
-    for t, like, name in ((d_q, q, "d_q"), (d_k, k, "d_k"), (d_v, v, "d_v")):
-        if t is not None:
-            _written(t, name, like)
+    if not fill:
+        _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
+        given = {n: t for n, t in (("d_q", d_q), ("d_k", d_k), ("d_v", d_v)) if t is not None}
+        for (name, t), like in zip((("d_q", d_q), ("d_k", d_k), ("d_v", d_v)), (q, k, v)):
+            if t is not None:
+                _written(t, name, like)
+                _apart(t, name, q=q, k=k, v=v, out=out, d_out=d_out, **{n: o for n, o in given.items() if n != name})
     d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fill)
-    make, device, index = torch.empty if fill and d.docs else torch.zeros, q.device, q.get_device()
-    d_q, d_k, d_v = (make(like.shape, dtype=like.dtype, device=device) if t is None else t for t, like in zip(given, (q, k, v)))
-    _on_device(index, d_out=d_out, out=out, stats=stats, d_q=d_q, d_k=d_k, d_v=d_v)
+    index = q.get_device()
+    if not (index == d_out.get_device() == out.get_device() == stats.get_device()):
+        _on_device(index, d_out=d_out, out=out, stats=stats)
+    make = torch.empty if fill and d.docs else torch.zeros  # (rows of no document keep 0)
+    d_q = make(shape, dtype=q.dtype, device=q.device) if d_q is None else d_q
+    d_k = make(k.shape, dtype=q.dtype, device=q.device) if d_k is None else d_k
+    d_v = make(k.shape, dtype=q.dtype, device=q.device) if d_v is None else d_v
+    if not fill:
+        _on_device(index, d_q=d_q, d_k=d_k, d_v=d_v)
     lib = _lib.load()
     with _On(index):
-        d_slopes = torch.empty(q.shape[1], dtype=torch.float32, device=device) if slope_grad else None
-        if slope_grad and d.docs == 0:
-            d_slopes.zero_()
-        scratch = torch.empty(lib.fc_attention_docs_backward_scratch_bytes(d), dtype=torch.uint8, device=device)
+        d_slopes = torch.empty(shape[1], dtype=torch.float32, device=q.device) if slope_grad else None
+        need = lib.fc_attention_docs_backward_scratch_bytes(d)
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
         _lib.check(lib.fc_attention_docs_backward(d, out.data_ptr(), *_strides(out), stats.data_ptr(), d_out.data_ptr(), *_strides(d_out),
                                                   d_q.data_ptr(), *_strides(d_q), d_k.data_ptr(), *_strides(d_k), d_v.data_ptr(),
-                                                  *_strides(d_v), _ptr(d_slopes), scratch.data_ptr(), scratch.numel(),
+                                                  *_strides(d_v), _ptr(d_slopes), scratch.data_ptr(), need,
                                                   _lib.stream_of(index)), "fc_attention_docs_backward")
     return (d_q, d_k, d_v) + ((d_slopes,) if slope_grad else ())

@@ -202,14 +202,16 @@ FC_API int fc_rotary(int32_t kind, const void* x, int64_t x_row, int64_t x_head,
  * k_offsets[d] .. k_offsets[d + 1] (dev int32 [docs + 1], not decreasing, inside the rows; the same array where every token is both).
  * Its query i stands at its key p = i + keys - queries.  score = scale q.k, then cap tanh(score / cap) if cap > 0, then
  * - slopes[head] |p - j| if slopes (dev f32 [q_heads]) is given.  A query sees all keys of its document or, if causal, those up to p and
- * the first prefix[d] ones (dev int32 [docs], may be null).  Query heads h g .. h g + g - 1, g = q_heads / kv_heads, share key head h. */
+ * the first prefix[d] ones (dev int32 [docs], may be null).  Query heads h g .. h g + g - 1, g = q_heads / kv_heads, share key head h.
+ * A head is 64 contiguous values; every row and head, of results too, starts on a 16-byte boundary; strides are in elements and not
+ * negative, rows of q, k, v and d_out less than 32 MiB apart. */
 typedef struct {
   int32_t struct_size; /* sizeof(fc_docs) as the caller declared it: checked first */
   int32_t kind;        /* fc_precision of q, k, v, out and the gradients */
   int32_t docs, q_heads, kv_heads;
   int32_t causal;
   int32_t fill;        /* 1: rows of no document are set to 0 (stats: -inf, 0) in the outputs; 0: they are left as they were */
-  float scale, cap;    /* scale > 0; cap 0: none */
+  float scale, cap;    /* scale > 0; cap 0: none; neither above 1e30 */
   int64_t q_rows, k_rows;
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
@@ -221,13 +223,13 @@ typedef struct {
  * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 where it sees nothing): what the gradients and a later
  * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
  * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
- * infinities included.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
+ * infinities included.  out must not overlap k or v.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
 FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
                       size_t scratch_bytes, fc_stream stream);
 /* Gradients of fc_attention_docs from the gradient d_out of its result: d_q, d_k, d_v of q, k, v (same element kind) and, if d_slopes
  * is given, of the slopes (dev f32 [q_heads]).  out and stats are the forward's.  Gradients of shared key heads are summed over their
- * query heads; every sum has a fixed order (no atomics).  scratch: fc_attention_docs_backward_scratch_bytes. */
+ * query heads; every sum has a fixed order (no atomics).  The gradients must not overlap operands or each other.  scratch: fc_attention_docs_backward_scratch_bytes. */
 FC_API size_t fc_attention_docs_backward_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_row, int64_t out_head, const float* stats,
                                const void* d_out, int64_t do_row, int64_t do_head, void* d_q, int64_t dq_row, int64_t dq_head,

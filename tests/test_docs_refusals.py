@@ -34,6 +34,8 @@ OFF = torch.tensor([0, 8], dtype=torch.int32)
     (dict(cap=float("nan")), ValueError, "cap"),
     (dict(scale=0.0), ValueError, "scale"),
     (dict(scale=float("inf")), ValueError, "scale"),
+    (dict(scale=2e30), ValueError, "1e30"),
+    (dict(cap=2e30), ValueError, "1e30"),
     (dict(), _lib.FitclipHipError, "no CPU fallback"),
 ])
 def test_attention_refuses(change, error, match):
@@ -51,6 +53,37 @@ def test_written_tensors_may_not_overlap_themselves():
             ops._written(bad, "out", x)
     for fine in (torch.zeros(8, 12, 64)[:, 4:8], torch.zeros(4, 8, 64).transpose(0, 1), torch.zeros(8, 4, 80)[..., :64]):
         ops._written(fine, "out", x)
+
+
+def test_results_may_not_overlap_operands():
+    qkv = torch.zeros(8, 3 * 128)
+    q, k, v = (x.view(8, 2, 64) for x in qkv.split(128, 1))
+    first = torch.zeros(3, 4, 9, 64)
+    a, b, c = (x.transpose(0, 1) for x in first)            # heads first, one block behind the other
+    mixed = torch.zeros(4, 3, 9, 64)
+    d, e, f = (mixed[:, i].transpose(0, 1) for i in range(3))  # ... in turns
+    for one, two in ((q, k), (q, v), (v, k), (a, b), (c, a), (d, e), (f, d), (q, a), (q[:0], q), (q[:4], q[4:]), (q[:, :1], q[:, 1:])):
+        assert not ops._meet(one, two) and not ops._meet(two, one)
+    shifted = qkv[:, 64:192].view(8, 2, 64)
+    for one, two in ((q, q), (q, shifted), (shifted, k), (q[:5], q[4:]), (a, first[0, 1:].transpose(0, 1)), (d, mixed[:, 0, 1:].transpose(0, 1)),
+                     (q, qkv.view(-1)[1300:1300 + 128 * 8].view(8, 2, 64))):
+        assert ops._meet(one, two) and ops._meet(two, one)
+    off = OFF
+    with pytest.raises(ValueError, match="out overlaps k"):
+        ops.attention_docs(q, k, v, off, out=k)
+    with pytest.raises(ValueError, match="out overlaps v"):
+        ops.attention_docs(q, k, v, off, out=v)
+    out, stats = torch.zeros(8, 2, 64), torch.zeros(8, 2, 2)
+    for given, match in ((dict(d_q=q), "d_q overlaps q"), (dict(d_k=v), "d_k overlaps v"), (dict(d_v=out), "d_v overlaps out"),
+                         (dict(d_k=torch.zeros(8, 2, 64), d_q=shifted), "d_q overlaps")):
+        with pytest.raises(ValueError, match=match):
+            ops.attention_docs_backward(torch.zeros(8, 2, 64), q, k, v, out, stats, off, **given)
+    one = torch.zeros(8, 2, 64)
+    with pytest.raises(ValueError, match="d_k overlaps d_v"):
+        ops.attention_docs_backward(torch.zeros(8, 2, 64), q, k, v, out, stats, off, d_k=one, d_v=one)
+    positions, inv_freq = torch.zeros(8, dtype=torch.int32), torch.zeros(32)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.rotary(q, positions, inv_freq, out=shifted)
 
 
 @pytest.mark.parametrize("change,error,match", [
@@ -82,6 +115,8 @@ def _c_docs(**change):
     (dict(kind=2), b"element kind"), (dict(docs=-1), b"negative"), (dict(kv_heads=0), b"multiple"), (dict(q_heads=5), b"multiple"),
     (dict(q_rows=1 << 30), b"2\\^31"), (dict(k_rows=1 << 31), b"2\\^31"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"),
     (dict(cap=-1.0), b"cap"), (dict(prefix=4096), b"causal"), (dict(q=None), b"null"), (dict(q_offsets=None), b"null"), (dict(v=None), b"null"),
+    (dict(scale=2e30), b"1e30"), (dict(cap=2e30), b"1e30"), (dict(q_row=-256), b"negative"), (dict(v_head=-64), b"negative"),
+    (dict(q_row=1 << 23), b"32 MiB"), (dict(k_row=1 << 23), b"32 MiB"), (dict(v_row=1 << 23), b"32 MiB"),
     (dict(k=4104), b"16-byte"), (dict(q_row=258), b"16-byte"), (dict(v_head=2), b"16-byte"),
 ])
 def test_the_c_entry_refuses(change, match):

@@ -559,3 +559,92 @@ def test_attention_offsets_beyond_32_bits():
     tail = cache[-700:].clone()
     ref = R.attention(q, tail, tail, [1, 1], [400, 300])
     _within("far", out, ref["out"], R.out_bound(ref, tail, torch.bfloat16, 400, R.score_error(ref, 400)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_extreme_caps_scales_and_slopes(dtype):
+    q_len = [40, 3, 33]
+    q, k, v = _operands(76, 76, 2, 2, dtype, seed=60)
+    # a cap so small that its reciprocal leaves fp32: every score is 0 up to 1e-35, the weights are equal
+    flat = R.attention(torch.zeros_like(q), k, v, q_len, causal=True)
+    even = R.out_bound(flat, v, dtype, 40, 2.0 ** -24)
+    for how in (dict(cap=1e-36), dict(scale=1e-36), dict(cap=1e30, scale=1e-36)):
+        out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=True, **how)
+        _within(str(how), out, flat["out"], even)
+        grads = ops.attention_docs_backward(torch.ones_like(out), q, k, v, out, stats, R.offsets(q_len), causal=True, **how)
+        assert all(torch.isfinite(g).all() for g in grads)
+    # a slope so steep that every query sees its own place alone (weights below 2^-1000 beside 1)
+    out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), slopes=torch.tensor([1e4, 3e30], device=DEV))
+    assert torch.equal(out, v) and (stats[..., 1] == 1).all()
+    # slopes of the other sign: the first key is the farthest, and alone (distances within a document differ by one)
+    out, _ = ops.attention_docs(q, k, v, R.offsets(q_len), causal=True, slopes=torch.full((2,), -1e5, device=DEV))
+    firsts = torch.tensor([0] * 40 + [40] * 3 + [43] * 33, device=DEV)
+    assert torch.equal(out, v[firsts])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_queries_or_no_rows_at_all(dtype):
+    k = _rand(70, 2, 64, seed=61, dtype=dtype)
+    q = torch.empty(0, 4, 64, dtype=dtype, device=DEV)
+    slopes = torch.ones(4, device=DEV)
+    for keys, docs in ((k, 3), (k[:0], 3), (k[:0], 0)):
+        q_off = torch.zeros(docs + 1, dtype=torch.int32, device=DEV)
+        k_off = R.offsets([30, 0, 40]) if len(keys) else q_off
+        out, stats = ops.attention_docs(q, keys, keys, q_off, k_off, slopes=slopes)
+        assert out.shape == (0, 4, 64) and stats.shape == (0, 4, 2)
+        d_q, d_k, d_v, d_slopes = ops.attention_docs_backward(out, q, keys, keys, out, stats, q_off, k_off, slopes=slopes, slope_grad=True)
+        assert d_q.shape == q.shape and (d_k == 0).all() and (d_v == 0).all() and (d_slopes == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_into_its_own_queries(dtype):
+    """out may be q: each row is read by the workgroup that writes it, before it does (splits over the keys among them)."""
+    for q_len, k_len in (([40, 77, 3], None), ([1, 2], [900, 1100])):
+        q, k, v = _operands(sum(q_len), sum(k_len or q_len), 6, 2, dtype, seed=62)
+        offs = (R.offsets(q_len), None if k_len is None else R.offsets(k_len))
+        want, stats = ops.attention_docs(q, k, v, *offs, causal=True)
+        got, own = ops.attention_docs(q, k, v, *offs, causal=True, out=q)
+        assert got is q and torch.equal(got, want) and torch.equal(own, stats)
+
+
+def test_calls_on_two_streams_at_once():
+    """Scratch is each call's own: splits and row tables of calls that overlap in time."""
+    q_len, k_len = [1] * 6, [700, 2000, 1, 900, 1500, 40]
+    sets = []
+    for seed in (70, 71):
+        q, k, v = _operands(6, sum(k_len), 6, 2, torch.bfloat16, seed=seed)
+        sets.append((q, k, v, _rand(6, 6, 64, seed=seed + 5, dtype=torch.bfloat16)))
+    offs = (R.offsets(q_len), R.offsets(k_len))
+
+    def both(q, k, v, d_out):
+        out, stats = ops.attention_docs(q, k, v, *offs, causal=True)
+        return (out, stats) + ops.attention_docs_backward(d_out, q, k, v, out, stats, *offs, causal=True)
+    want = [both(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(both(*s))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+def test_results_in_the_norm(dtype, cap):
+    """Errors of single values may reach their bounds; all of them together may not: in the 2-norm they add up like noise.  A result's
+    roundings (bf16: its own, its weights', d_out and out as the gradient reads them: 4 of at most 2^-8, a third of that in the mean square, and
+    twice as much where differences dP - D take something away) stay below 6 x 2^-8 of the norm; fp32 sums of up to 400 terms below 400 x 2^-24."""
+    q_len = [160, 40, 200]
+    q, k, v = _operands(400, 400, 4, 2, dtype, seed=80, layout="fused")
+    d_out = _rand(400, 4, 64, seed=81, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=True, cap=cap)
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=True, cap=cap)
+    ref = R.attention(q, k, v, q_len, causal=True, cap=cap, d_out=d_out)
+    for name, got in (("out", out), ("d_q", grads[0]), ("d_k", grads[1]), ("d_v", grads[2])):
+        want = ref[name].to(DEV).double()
+        far = float((got.double() - want).norm() / want.norm())
+        assert far <= (6 * R.HALF[dtype] if dtype == torch.bfloat16 else 400 * 2.0 ** -24), (name, far)
