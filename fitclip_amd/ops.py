@@ -2,6 +2,8 @@
 checks shapes / dtypes / device, allocates the output with torch, and makes ONE C-ABI call on the current stream."""
 from __future__ import annotations
 
+import ctypes
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -600,9 +602,37 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
     [pairs], 2 pairs <= dim, the dimensions behind them are copied; `sections`: how many pairs turn with each axis; pairs are
     (i, i + pairs), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in 64 bits: exact at far positions.  `inverse` turns
     back - the gradient.  `out` may be x (in place), and must not overlap it otherwise."""
-    _heads(x, "x", x.dtype, None)
     positions = positions[:, None] if positions.dim() == 1 else positions
-    rows, heads, dim = x.shape
+    shape, kind, index, pairs = x.shape, _KIND.get(x.dtype), x.get_device(), inv_freq.numel()
+    axes = positions.shape[-1] if positions.dim() else 0
+    sections = tuple(sections or ()) if sections is not None or axes != 1 else (pairs,)
+    # the operands as they should be, looked over at once; anything else is named by _check_rotary
+    if not (len(shape) == 3 and kind is not None and shape[2] > 1 and x.stride(2) == 1 and 1 <= axes <= 3 and positions.dtype is torch.int32
+            and positions.shape == (shape[0], axes) and positions.is_contiguous() and _fine(inv_freq, torch.float32, pairs, index) and index >= 0
+            and positions.get_device() == index and len(sections) == axes and sum(sections) == pairs and out is None):
+        _check_rotary(x, positions, inv_freq, sections, out)
+    rows, heads, dim = shape
+    x_row, x_head = _strides(x)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out_row, out_head = heads * dim, dim
+    else:
+        out_row, out_head = _strides(out)
+    with _On(index):
+        _lib.check(_lib.load().fc_rotary(kind, x.data_ptr(), x_row, x_head, positions.data_ptr(), axes, inv_freq.data_ptr(), _sections(sections),
+                                         pairs, int(interleaved), int(inverse), out.data_ptr(), out_row, out_head, rows, heads, dim,
+                                         _lib.stream_of(index)), "fc_rotary")
+    return out
+
+
+@functools.lru_cache(maxsize=64)
+def _sections(sections: "tuple[int, ...]") -> ctypes.Array:
+    return (_lib._i32 * len(sections))(*sections)
+
+
+def _check_rotary(x, positions, inv_freq, sections, out) -> None:
+    _heads(x, "x", x.dtype, None)
+    rows = x.shape[0]
     if positions.dtype != torch.int32:
         raise TypeError(f"positions must be {torch.int32}, got {positions.dtype}")
     if positions.dim() != 2 or positions.shape[0] != rows or not 1 <= positions.shape[1] <= 3:
@@ -611,23 +641,13 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
         raise ValueError("positions must be contiguous")
     _vector(inv_freq, "inv_freq", torch.float32)
     axes, pairs = positions.shape[1], inv_freq.numel()
-    sections = [pairs] if sections is None and axes == 1 else list(sections or ())
     if len(sections) != axes or sum(sections) != pairs:
-        raise ValueError(f"{axes} sections that sum up to {pairs} pairs are needed, got {sections}")
+        raise ValueError(f"{axes} sections that sum up to {pairs} pairs are needed, got {list(sections)}")
     if out is not None:
         _written(out, "out", x)
         if (out.data_ptr() != x.data_ptr() or _strides(out) != _strides(x)) and _meet(out, x):
             raise ValueError("out overlaps x: in place needs the same place and strides")
-    index = x.get_device()
-    _on_device(index, x=x, positions=positions, inv_freq=inv_freq, out=out)
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=x.dtype, device=x.device)
-    (x_row, x_head), (out_row, out_head) = _strides(x), _strides(out)
-    with _On(index):
-        _lib.check(_lib.load().fc_rotary(_KIND[x.dtype], x.data_ptr(), x_row, x_head, positions.data_ptr(), axes, inv_freq.data_ptr(),
-                                         (_lib._i32 * axes)(*sections), pairs, int(interleaved), int(inverse), out.data_ptr(),
-                                         out_row, out_head, rows, heads, dim, _lib.stream_of(index)), "fc_rotary")
-    return out
+    _on_device(x.get_device(), x=x, positions=positions, inv_freq=inv_freq, out=out)
 
 
 def _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale) -> None:
