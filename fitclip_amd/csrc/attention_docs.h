@@ -15,7 +15,10 @@
 //     reading a tile free of bank conflicts: rows as an operand (16 bytes per lane, 16 rows at a time) and columns as an operand
 //     (ds_read_b64_tr_b16 for bf16, 4-byte reads for fp32).  bf16: 8 chunks, swizzle = row bits 1, 2, 3 reversed (two rows share a
 //     256-byte bank line; bit 1 must move a 64-byte half for the transposing read).  fp32: 16 chunks, row bit 2 moves a 128-byte half.
-//   * tiles arrive by LDS-DMA, double-buffered: the swizzle is applied to each lane's source address.
+//   * tiles arrive by LDS-DMA: the swizzle is applied to each lane's source address.  Waves that share tiles have two of each, a wave that reads
+//     its tiles alone has one (it sends for the next as soon as this one is in registers).
+//   * NaN and infinities behind a mask: a weight of 0 times NaN is NaN, and looking at every value would cost more than the mask.  So the fast way
+//     lets them through, looks at the RESULTS, and does a row (key) whose result is not finite again, key by key over what it sees.
 #pragma once
 #include "common.h"
 
@@ -557,14 +560,18 @@ __device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool count
 //           loop, four times the waves and a quarter of the longest wave's way
 //   ALONE   a workgroup of one wave over 32 rows: documents of two or three tiles, where a fourth wave would find nothing to take and shared
 //           tiles are of use to one or two of the waves that wait for them
-// `way`: the keys that a row walks over, the mean over the documents (their lengths are on the device).  Measured, us (8 heads, bf16 forward;
-// fp32 forward; fp32 gradients): 20000 rows in documents of 40: shared 26.6, 83, 240, turns -, 88, 262, alone 22.5, 59, 177; of 160: 27.6, 119,
-// 358, turns -, 120, 357, alone 24.9, 88, 248; of 200: 35, 165, 502, turns -, 152, 453, alone 37, 144, 462.  Alone needs its waves to fill the
-// chip: 1200 rows of 77, fp32 gradients, turns 45, alone 64; 2400 rows 63 and 66, of 40 50 and 43.
-// Shared or turns: 12 heads of 1, 2, 3, 6, 12 x 3136 tokens (1.2 to 14 workgroups that share on a compute unit), forward: bf16 shared
-// 61 127 147 246 447, turns 62 113 155 297 576; fp32 (whose products take ten times as long) shared 354 802 1004 1617, turns 291 570 799 1585,
-// and over 4 x 8192 tokens, 8 per compute unit, 4206 and 4555.  Shorter ways in bf16, 8000 rows in documents of 200, 256, 400 (2 per compute
-// unit), gradients: shared 48 34 71, turns 64 57 79.
+// `way`: the keys that a row walks over, the mean over the documents (their lengths are on the device).  All measured with each shape, us:
+//   8 heads, 20000 rows              shared   turns   alone      12 heads, tokens       shared   turns
+//   of 40   bf16 forward               25.1    35.1    22.0      1 x 3136 bf16 forward    65.1    54.7   (1.2 sharing workgroups
+//           fp32 forward, gradients  86 239  81 275  58 186      2 x 3136                108.7    99.3    per compute unit)
+//   of 160  bf16 forward               26.3    38.2    23.6      3 x 3136                133.3   139.2
+//           fp32 forward, gradients 120 355 104 382  83 248      6 x 3136                234.7   271.1
+//   of 200  bf16 forward               33.7    40.4    33.2      12 x 3136               423.7   533.7   (14)
+//           fp32 forward, gradients 163 490 132 459 134 452      1 x 3136 fp32 forward   397     268
+// Alone needs enough waves: 8 heads, fp32 gradients, 1200 rows   3 x 3136                930     746
+// of 77: turns 47, alone 65; 2400 rows of 77 63, 67, of 40 50,   6 x 3136               1590    1477     (7)
+// 45.  bf16 with shorter ways, 8000 rows of 200, 256, 400 (2     4 x 8192, 8 heads      4141    4290     (8)
+// per compute unit), gradients: shared 48 35 72, turns 65 57 79
 enum Shape : int { SHARED, TURNS, ALONE };
 inline Shape shape_for(int kind, long rows, long heads, double way) {
   const long cus = device_cus(), shared = (rows + 127) / 128 * heads;
