@@ -551,6 +551,11 @@ def _written(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape and type (empty_like takes half of empty's time)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two [rows, heads, dim] views touch the same bytes.  Views of one fused projection lie side by side in its rows (or heads)."""
     if not a.numel() or not b.numel():
@@ -614,7 +619,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sec
     rows, heads, dim = shape
     x_row, x_head = _strides(x)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = _dense_like(x)
         out_row, out_head = heads * dim, dim
     else:
         out_row, out_head = _strides(out)
@@ -718,19 +723,23 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
         _written(out, "out", q)
         _apart(out, "out", k=k, v=v)
     d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, out is None)
-    device, index = q.device, q.get_device()
-    if out is None:
-        out = (torch.empty if d.docs else torch.zeros)(q.shape, dtype=q.dtype, device=device)
+    index, (rows, heads, _), docs = q.get_device(), q.shape, d.docs
+    fresh = out is None
+    if fresh:
+        out = _dense_like(q)
+        out_row, out_head = heads * 64, 64
+        if not docs:
+            out.zero_()
     else:
         _on_device(index, out=out)
-    stats = torch.empty((q.shape[0], q.shape[1], 2), dtype=torch.float32, device=device)
+        out_row, out_head = _strides(out)
+    stats = q.new_empty((rows, heads, 2), dtype=torch.float32)
     lib = _lib.load()
-    out_row, out_head = _strides(out)
     with _On(index):
-        if not d.docs or not d.fill:  # (rows of no document keep these)
+        if not docs or not fresh:  # (rows of no document keep these)
             stats[..., 0], stats[..., 1] = float("-inf"), 0.0
         need = lib.fc_attention_docs_scratch_bytes(d)
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        scratch = q.new_empty(need, dtype=torch.uint8) if need else None
         _lib.check(lib.fc_attention_docs(d, out.data_ptr(), out_row, out_head, stats.data_ptr(), _ptr(scratch), need,
                                          _lib.stream_of(index)), "fc_attention_docs")
     return out, stats
@@ -770,17 +779,17 @@ def attention_docs_backward(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     index = q.get_device()
     if not (index == d_out.get_device() == out.get_device() == stats.get_device()):
         _on_device(index, d_out=d_out, out=out, stats=stats)
-    make = torch.empty if fill and d.docs else torch.zeros  # (rows of no document keep 0)
-    d_q = make(shape, dtype=q.dtype, device=q.device) if d_q is None else d_q
-    d_k = make(k.shape, dtype=q.dtype, device=q.device) if d_k is None else d_k
-    d_v = make(k.shape, dtype=q.dtype, device=q.device) if d_v is None else d_v
+    make = _dense_like if fill and d.docs else lambda t: t.new_zeros(t.shape)  # (rows of no document keep 0)
+    d_q = make(q) if d_q is None else d_q
+    d_k = make(k) if d_k is None else d_k
+    d_v = make(v) if d_v is None else d_v
     if not fill:
         _on_device(index, d_q=d_q, d_k=d_k, d_v=d_v)
     lib = _lib.load()
     with _On(index):
-        d_slopes = torch.empty(shape[1], dtype=torch.float32, device=q.device) if slope_grad else None
+        d_slopes = q.new_empty(shape[1], dtype=torch.float32) if slope_grad else None
         need = lib.fc_attention_docs_backward_scratch_bytes(d)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(need, dtype=torch.uint8)
         _lib.check(lib.fc_attention_docs_backward(d, out.data_ptr(), *_strides(out), stats.data_ptr(), d_out.data_ptr(), *_strides(d_out),
                                                   d_q.data_ptr(), *_strides(d_q), d_k.data_ptr(), *_strides(d_k), d_v.data_ptr(),
                                                   *_strides(d_v), _ptr(d_slopes), scratch.data_ptr(), need,
