@@ -74,7 +74,9 @@ attention_docs_kernel(const Args a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // key head fastest (one XCD then works on few heads: K and V stay in its L2), later rows first (causal: they cost most)
   const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int tile = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+  const int rank = (int)((unsigned)rest / (unsigned)a.splits), split = rest - rank * a.splits;
+  const int tile = RW * KS > 1 && a.by_way ? tile_by_way(a.q_off, a.k_off, a.docs, a.q_rows, (int)a.group.d, 32 * RW, a.tiles, rank, true, lane)
+                                          : a.tiles - 1 - rank;
   const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
   RowFrag<T> qf;  // (sent for first: on its way under the search for the rows' documents)
@@ -513,6 +515,7 @@ int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_
   a.part = (float*)scratch;
   a.tiles = p.tiles;
   a.splits = p.splits;
+  a.by_way = ordered(p.shape, d->docs, p.splits == 1 ? (long)p.tiles * d->kv_heads : 0);
   return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.shape, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.shape, st);
 }
 

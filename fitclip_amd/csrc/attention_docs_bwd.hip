@@ -162,7 +162,8 @@ docs_grad_rows_kernel(const Args a) {
   __shared__ float shares[KS > 1 ? KS : 1][3][32];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, tile = a.tiles - 1 - blockIdx.x / heads;
+  const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, rank = blockIdx.x / heads;
+  const int tile = RW * KS > 1 && a.by_way ? tile_by_way(a.q_off, a.k_off, a.docs, a.q_rows, 1, 32 * RW, a.tiles, rank, true, lane) : a.tiles - 1 - rank;
   const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
 
   // (sent for first: on their way under the search for the rows' documents)
@@ -389,7 +390,8 @@ docs_grad_keys_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int tile = rest % a.tiles, split = rest / a.tiles;  // (earlier keys first: causal, they cost most)
+  const int rank = (int)((unsigned)rest / (unsigned)a.splits), split = rest - rank * a.splits;  // (earlier keys first: causal, they cost most)
+  const int tile = KW * KS > 1 && a.by_way ? tile_by_way(a.k_off, a.q_off, a.docs, a.k_rows, 1, 32 * KW, a.tiles, rank, false, lane) : rank;
   const int k0 = tile * KW * 32, kw = k0 + (KS > 1 ? 0 : wave * 32);
 
   const int key = kw + r;
@@ -667,6 +669,7 @@ int launch_grads(Args a, const KeyPlan& p, hipStream_t st) {
   const Shape by = shape_for(sizeof(T) == 4 ? PREC_F32 : PREC_BF16, a.rows, heads, (double)a.k_rows / a.docs);
   int rc;
   a.tiles = tiles_of(by, a.rows);
+  a.by_way = ordered(by, a.docs, a.tiles * heads);
   if (by == SHARED)
     rc = launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
   else if (by == TURNS)
@@ -677,6 +680,7 @@ int launch_grads(Args a, const KeyPlan& p, hipStream_t st) {
   a.tiles = p.tiles;
   a.splits = p.splits;
   const long units = (long)p.tiles * p.splits * a.kv_heads;
+  a.by_way = ordered(p.shape, a.docs, units);
   constexpr int alone = (sizeof(T) == 4 ? 1 : 2) * (64 * row + 6 * 128 + 64);  // a wave's stages
   if (p.shape == SHARED)
     rc = launch_docs(docs_grad_keys_kernel<T, 4, 1, 64, CAP, BIAS>, units, 4, 2 * (128 * row + 6 * 256 + 64), a, keys, st);

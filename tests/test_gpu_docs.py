@@ -648,3 +648,32 @@ def test_results_in_the_norm(dtype, cap):
         want = ref[name].to(DEV).double()
         far = float((got.double() - want).norm() / want.norm())
         assert far <= (6 * R.HALF[dtype] if dtype == torch.bfloat16 else 400 * 2.0 ** -24), (name, far)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,how", [(22, 22, {}), (44, 22, dict(causal=True, slopes=True)), (26, 26, dict(causal=True, prefix=True, cap=8.0))])
+def test_uneven_documents_in_the_order_of_their_ways(dtype, heads, kv_heads, how):
+    """More than two workgroups per compute unit take their tiles longest way first, those that reach into the next document before all: every
+    tile exactly once, rows in front of the first and behind the last document among them."""
+    g = torch.Generator().manual_seed(90)
+    q_len = [37, 400, 0, 5, 500, 129, 1]
+    n, lead, rows = sum(q_len), 5, sum(q_len) + 5 + 60
+    how = dict(how)
+    if how.get("prefix"):
+        how["prefix"] = torch.randint(-3, 300, (7,), generator=g, dtype=torch.int32).to(DEV)
+    if how.get("slopes"):
+        how["slopes"] = (0.1 * torch.rand(heads, generator=g)).to(DEV)
+    q, k, v = _operands(rows, rows, heads, kv_heads, dtype, seed=91)
+    d_out, off = _rand(rows, heads, 64, seed=92, dtype=dtype), R.offsets(q_len) + lead
+    out, stats = ops.attention_docs(q, k, v, off, **how)
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, off, slope_grad="slopes" in how, **how)
+    own = slice(lead, lead + n)
+    some = [0, kv_heads - 1]
+    ref, out_bound, bounds, of = _some_heads(q[own], k[own], v[own], d_out[own], q_len, None, some, **how)
+    _within("out", out[own][:, of], ref["out"], out_bound)
+    for name, got, which in zip(("d_q", "d_k", "d_v"), grads, (of, some, some)):
+        _within(name, got[own][:, which], ref[name], bounds[name])
+        assert (got[:lead] == 0).all() and (got[lead + n:] == 0).all()
+    assert (out[:lead] == 0).all() and (out[lead + n:] == 0).all() and (stats[lead + n:, :, 1] == 0).all() and (stats[:lead, :, 1] == 0).all()
+    if "slopes" in how:
+        _within("d_slopes", grads[3][of], ref["d_slopes"], bounds["d_slopes"])
