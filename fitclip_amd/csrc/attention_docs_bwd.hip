@@ -12,15 +12,20 @@
 //   keys: 32 keys per wave (K and V in registers), tiles of the rows that see them, one query head of the group after the other - the
 //   gradients of shared heads need no further sum.  S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
+// bf16: `out` comes rounded, and D = dO.out with it; P and dS are rounded in front of their products (once each: 2^-9 of a term, where the result's
+// own rounding is as much).  D's error matters to rows of few keys, where no sum over keys evens it out: a row whose keys all lie in one tile has its
+// D formed again from the tile, as sum P dP.  (dS in two parts, an operand for what its rounding left, made d_q's error 1.0 to 1.4 times its
+// own rounding's instead of 1.4 to 1.5, for a third more time in rows: not kept.)
 // Both have the forward's three shapes (attention_docs.h, shape_for).  The scores and dP are formed twice, 7 products where 5 would do: one
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
 //
 // What bounds them, and what they reach (10 x 64 operations per pair and head that see each other, for both kernels):
-//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1966 us
-//     = 699 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 121 us, keys 200 us; 6 clips of 784 to
-//     1568 tokens, 12 heads, a cap: 107 and 169, 143 of them without bringing any tiles.
+//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads @@4 us
+//     = @@5 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 121 us, keys 200 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
+//     107 and 169, 143 of the latter without bringing any tiles.
 //   fp32: the matrix instructions; 4 x 8192 tokens 14.2 ms = 97 TFLOP/s, 136 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
-//     rows 47 us, keys 63 us - there 32 x 32 tiles hold three times the pairs that the masks leave.
+//     rows 47 us, keys 63 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
+//     2: rows 105, keys 135.
 #include "attention_docs.h"
 
 #include <algorithm>
@@ -156,10 +161,11 @@ __global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_
 docs_grad_rows_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
   constexpr int BUFS = RW == 1 ? 1 : 2;  // (as in the forward)
+  constexpr bool kExact = sizeof(T) == 2;  // D of short rows to more than bf16 holds (see the top)
   static_assert((KS == 1 && RW * 32 * ROWB <= BUFS * STAGE) || (RW == 1 && STAGE >= 8192 && NT == 1), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * RW];
-  __shared__ float shares[KS > 1 ? KS : 1][3][32];
+  __shared__ float shares[KS > 1 ? KS : 1][4][32];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, rank = blockIdx.x / heads;
@@ -208,7 +214,7 @@ docs_grad_rows_kernel(const Args a) {
   if (KS == 1 || wave == 0) {
     if (hh == 0) {  // (m0 + r < rows_pad)
       column(a, COL_MAX, qh)[m0 + r] = top;
-      column(a, COL_D, qh)[m0 + r] = D;
+      if constexpr (!kExact) column(a, COL_D, qh)[m0 + r] = D;
       column(a, COL_LO, qh)[m0 + r] = __int_as_float(row.lo);
       column(a, COL_HI, qh)[m0 + r] = __int_as_float(row.hi);
       if constexpr (sizeof(T) == 4) column(a, COL_INV, qh)[m0 + r] = inv;
@@ -248,7 +254,8 @@ docs_grad_rows_kernel(const Args a) {
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-  float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|
+  float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|; tile by tile, so that long sums lose little
+  float off = 0.f;                      // what D, from a rounded out, was off by
   int t = KS > 1 ? wave : 0, buf = 0;
   if (t < ntile) stage(t, 0);
   for (; t < ntile; t += KS, buf ^= BUFS - 1) {
@@ -297,17 +304,32 @@ docs_grad_rows_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) p[i] = pick(bits, i, p[i], 0.f);
       }
+      if constexpr (kExact) {
+        const bool whole = sees && row.lo >= ku && row.hi <= ku + 32;
+        if (__any(whole)) {
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x = __builtin_fmaf(p[i], dp[i], x);
+          x = swap_sum(x);
+          if (whole && x * 0.f == 0.f) {  // (NaN: from a key behind a mask)
+            off = x - D;
+            D = x;
+          }
+        }
+      }
+      float tpd = 0.f, tpf = 0.f, tpdf = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if constexpr (BIAS) {
           const float far = fabsf(at - (float)(8 * (i >> 2) + (i & 3))), y = p[i] * dp[i];
-          pd += y;
-          pf = __builtin_fmaf(p[i], far, pf);
-          pdf = __builtin_fmaf(y, far, pdf);
+          tpd += y;
+          tpf = __builtin_fmaf(p[i], far, tpf);
+          tpdf = __builtin_fmaf(y, far, tpdf);
         }
         const float ds = p[i] * (dp[i] - D);
         s[i] = CAP ? ds * __builtin_fmaf(-s[i], s[i], 1.f) : ds;
       }
+      if constexpr (BIAS) pd += tpd, pf += tpf, pdf += tpdf;
       __builtin_amdgcn_sched_barrier(0);
       cols_dot(kc, s, o);
     };
@@ -328,6 +350,7 @@ docs_grad_rows_kernel(const Args a) {
   if constexpr (KS == 1) {
     const float probe = swap_sum(not_finite(o));
     const bool again = row.valid && probe != probe;
+    if (kExact && hh == 0) column(a, COL_D, qh)[m0 + r] = D;
     if (BIAS && hh == 0 && !again) column(a, COL_DSLOPE, qh)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
     __syncthreads();  // (the patches reuse the stages)
     // (a row that sees one key: its weight is 1 whatever the score)
@@ -335,12 +358,13 @@ docs_grad_rows_kernel(const Args a) {
                   [&](int w) { return a.dq + (long)(m0 + w) * a.dq_row + qh * a.dq_head; });
     bad = (unsigned)__ballot(again);
   } else {
-    if constexpr (BIAS) {
-      if (hh == 0) {
+    if (hh == 0) {
+      if constexpr (BIAS) {
         shares[wave][0][r] = pd;
         shares[wave][1][r] = pf;
         shares[wave][2][r] = pdf;
       }
+      if constexpr (kExact) shares[wave][3][r] = off;
     }
     f32x4 y[2];
     sum_waves<KS>(smem, STAGE, o, 1.f, wave, lane, y);  // (with a barrier inside)
@@ -349,6 +373,12 @@ docs_grad_rows_kernel(const Args a) {
     const bool valid = __shfl((int)row.valid, rr, 64), many = __shfl(row.hi - row.lo, rr, 64) > 1;
     bad = bad_of_eight(y, valid);
     const bool again = bad >> (lane >> 3) & 1;
+    if constexpr (kExact) {
+      float exact = __shfl(D - off, rr, 64);
+#pragma unroll
+      for (int w = 0; w < KS; ++w) exact += shares[w][3][rr];
+      if ((lane & 7) == 0) column(a, COL_D, qh)[mr] = exact;  // (mr < rows_pad)
+    }
     if (mr < a.rows && !again) {
       if (valid || a.fill) store_eight<T>(a.dq + (long)mr * a.dq_row + qh * a.dq_head, y, many ? a.scale : 0.f, lane);
       if constexpr (BIAS) {

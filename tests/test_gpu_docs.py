@@ -677,3 +677,31 @@ def test_uneven_documents_in_the_order_of_their_ways(dtype, heads, kv_heads, how
     assert (out[:lead] == 0).all() and (out[lead + n:] == 0).all() and (stats[lead + n:, :, 1] == 0).all() and (stats[:lead, :, 1] == 0).all()
     if "slopes" in how:
         _within("d_slopes", grads[3][of], ref["d_slopes"], bounds["d_slopes"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_thousands_of_documents_and_runs_of_empty_ones(dtype):
+    """The search for a row's (key's) document in more than 2048 of them, with more empty ones in a row than a wave looks at in one step."""
+    q_len = [3] * 300 + [0] * 200 + [2, 0, 0, 1] * 400 + [0] * 70 + [5] * 100 + [0] * 65
+    rows = sum(q_len)
+    q, k, v = _operands(rows, rows, 9, 9, dtype, seed=95, layout="fused")
+    d_out, off = _rand(rows, 9, 64, seed=96, dtype=dtype), R.offsets(q_len)
+    out, stats = ops.attention_docs(q, k, v, off, causal=True)
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, off, causal=True)
+    ref, out_bound, bounds, _ = _some_heads(q, k, v, d_out, q_len, None, [4], causal=True)
+    _within("out", out[:, [4]], ref["out"], out_bound)
+    for name, got in zip(("d_q", "d_k", "d_v"), grads):
+        _within(name, got[:, [4]], ref[name], bounds[name])
+    one, one_stats = ops.attention_docs(q[:, 4:5], k[:, 4:5], v[:, 4:5], off, causal=True)  # (few workgroups: another shape)
+    _within("one head", one, ref["out"], out_bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,heads", [(70, 3), (3000, 8)])
+def test_queries_without_any_keys(dtype, rows, heads):
+    q, none = _rand(rows, heads, 64, seed=97, dtype=dtype), torch.empty(0, heads, 64, dtype=dtype, device=DEV)
+    q_off, k_off = R.offsets([rows // 2, 0, rows - rows // 2]), torch.zeros(4, dtype=torch.int32, device=DEV)
+    out, stats = ops.attention_docs(q, none, none, q_off, k_off, causal=True)
+    assert (out == 0).all() and (stats[..., 0] == -math.inf).all() and (stats[..., 1] == 0).all()
+    d_q, d_k, d_v = ops.attention_docs_backward(torch.ones_like(q), q, none, none, out, stats, q_off, k_off, causal=True)
+    assert (d_q == 0).all() and d_k.shape == d_v.shape == none.shape
