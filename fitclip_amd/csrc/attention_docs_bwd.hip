@@ -3,8 +3,8 @@
 //   P = 2^(score - maximum) / sum (score in units of ln 2; both from the forward's stats)
 //   D_i = sum_d dO_id O_id,   dP = dO V^T,   dS = P (dP - D)      (0 exactly where a row sees one key)
 //   dV = P^T dO,   dQ = scale dS' K,   dK = scale dS'^T Q         dS' = dS (1 - tanh^2) behind a cap
-//   d slope_h = - sum dS |p_i - j| = - (sum_j P dP |p - j| - (sum_j P dP) (sum_j P |p - j|)) per row: every factor in fp32 (the D of a
-//   bf16 output is rounded)
+//   d slope_h = - sum_j P (dP - sum P dP) f = (sum dS) (sum P f) - sum dS f per row, f = |p_i - j| less any constant: every factor in fp32, and
+//   whatever D is (that of a bf16 output is rounded)
 //
 // Two kernels, no atomics: every sum has one owner and a fixed order.  A kernel row is a row of ONE query head here: 32 rows of a head lie at
 // one stride, and all sources are a uniform base plus a lane offset.
@@ -254,7 +254,13 @@ docs_grad_rows_kernel(const Args a) {
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[n][i] = 0.f;
-  float pd = 0.f, pf = 0.f, pdf = 0.f;  // per lane: sums of P dP, P |p - j|, P dP |p - j|; tile by tile, so that long sums lose little
+  // per lane: sums of dS, P f and dS f, f = |p - j| - mid; tile by tile, so that long sums lose little.  As dS adds up to 0 and P to 1, any `mid`
+  // gives the same gradient: near the mean distance (half of it all, or 1 / slope) the terms that cancel are small
+  float pd = 0.f, pf = 0.f, pdf = 0.f, mid = 0.f;
+  if constexpr (BIAS) {
+    const float most = (float)max(row.pos - row.lo, row.hi - 1 - row.pos), s = a.slopes[qh];
+    mid = s * most > 2.f ? 1.f / s : 0.5f * most;
+  }
   float off = 0.f;                      // what D, from a rounded out, was off by
   int t = KS > 1 ? wave : 0, buf = 0;
   if (t < ntile) stage(t, 0);
@@ -320,13 +326,13 @@ docs_grad_rows_kernel(const Args a) {
       float tpd = 0.f, tpf = 0.f, tpdf = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if constexpr (BIAS) {
-          const float far = fabsf(at - (float)(8 * (i >> 2) + (i & 3))), y = p[i] * dp[i];
-          tpd += y;
-          tpf = __builtin_fmaf(p[i], far, tpf);
-          tpdf = __builtin_fmaf(y, far, tpdf);
-        }
         const float ds = p[i] * (dp[i] - D);
+        if constexpr (BIAS) {
+          const float far = fabsf(at - (float)(8 * (i >> 2) + (i & 3))) - mid;
+          tpd += ds;
+          tpf = __builtin_fmaf(p[i], far, tpf);
+          tpdf = __builtin_fmaf(ds, far, tpdf);
+        }
         s[i] = CAP ? ds * __builtin_fmaf(-s[i], s[i], 1.f) : ds;
       }
       if constexpr (BIAS) pd += tpd, pf += tpf, pdf += tpdf;
