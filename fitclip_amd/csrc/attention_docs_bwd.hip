@@ -13,8 +13,9 @@
 //   gradients of shared heads need no further sum.  S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
 // bf16: `out` comes rounded, and D = dO.out with it; P and dS are rounded in front of their products (once each: 2^-9 of a term, where the result's
-// own rounding is as much).  D's error matters to rows of few keys, where no sum over keys evens it out: a row whose keys all lie in one tile has its
-// D formed again from the tile, as sum P dP.  (dS in two parts, an operand for what its rounding left, made d_q's error 1.0 to 1.4 times its
+// own rounding is as much).  D's error matters where few keys have all the weight and no sum over keys evens it out: a kernel in front forms D, and a
+// workgroup of it with such a row (a sum of weights below 8 times the largest: the first rows of a causal document, steep slopes) walks over its
+// keys for D = sum P dP, two products of the three in rows; the others are done at once.  (dS in two parts, an operand for what its rounding left, made d_q's error 1.0 to 1.4 times its
 // own rounding's instead of 1.4 to 1.5, for a third more time in rows: not kept.)
 // Both have the forward's three shapes (attention_docs.h, shape_for).  The scores and dP are formed twice, 7 products where 5 would do: one
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
@@ -29,6 +30,7 @@
 #include "attention_docs.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fc {
 namespace docs {
@@ -156,16 +158,17 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
 }
 
 // ------------------------------------------------------------------------------------------------------------------ rows
-template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS>
+// FOR_D: what the other one finds as D in the row table (bf16)
+template <typename T, int RW, int KS, int TK, bool CAP, bool BIAS, bool FOR_D = false>
 __global__ void __launch_bounds__(RW * KS * 64) __attribute__((amdgpu_waves_per_eu(2)))
 docs_grad_rows_kernel(const Args a) {
   constexpr int ROWB = Tile<T>::kRow, STAGE = 2 * TK * ROWB, NT = TK / 32;  // a stage: K rows, then V rows
   constexpr int BUFS = RW == 1 ? 1 : 2;  // (as in the forward)
-  constexpr bool kExact = sizeof(T) == 2;  // D of short rows to more than bf16 holds (see the top)
+  constexpr bool kFound = sizeof(T) == 2 && !FOR_D;
   static_assert((KS == 1 && RW * 32 * ROWB <= BUFS * STAGE) || (RW == 1 && STAGE >= 8192 && NT == 1), "the output patches reuse the stages");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int range[2 * RW];
-  __shared__ float shares[KS > 1 ? KS : 1][4][32];
+  __shared__ int range[3 * RW];
+  __shared__ float shares[KS > 1 ? KS : 1][3][32];
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = a.kv_heads * a.share, qh = blockIdx.x % heads, head = qh / a.share, rank = blockIdx.x / heads;
@@ -178,25 +181,30 @@ docs_grad_rows_kernel(const Args a) {
   qf.load(a.q + m * a.q_row + qh * a.q_head, hh);
   dof.load(a.d_out + m * a.do_row + qh * a.do_head, hh);
   const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * heads + qh) * 2);
+  float D;
   RowFrag<T> of;
-  of.load(a.out + m * a.out_row + qh * a.out_head, hh);
+  if constexpr (kFound) D = column(a, COL_D, qh)[m0 + r];
+  else of.load(a.out + m * a.out_row + qh * a.out_head, hh);
   const Row row = find_row(a, m0, lane);
-  float D = swap_sum(dot(of, dof));
+  if constexpr (!kFound) D = swap_sum(dot(of, dof));
   const bool sees = row.lo < row.hi;
   const int wlo = wave_min_i(sees ? row.lo : INT_MAX), whi = wave_max_i(sees ? row.hi : -INT_MAX);
   const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);
   const int full_hi = wave_min_i(row.valid ? (sees ? row.hi : -INT_MAX) : INT_MAX);
+  bool peaked = __any(sees && st[1] < 8.f);  // (st[1]: how many keys of the largest weight the row's weights would make)
   int kbeg = wlo, kend = whi;
   if constexpr (RW > 1) {
     if (lane == 0) {
       range[wave] = wlo;
       range[RW + wave] = whi;
+      range[2 * RW + wave] = peaked;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
       kbeg = min(kbeg, range[w]);
       kend = max(kend, range[RW + w]);
+      peaked |= range[2 * RW + w] != 0;
     }
     kbeg = __builtin_amdgcn_readfirstlane(kbeg);
     kend = __builtin_amdgcn_readfirstlane(kend);
@@ -210,11 +218,17 @@ docs_grad_rows_kernel(const Args a) {
     inv = 1.f;
   }
   if (!sees) D = 0.f;
+  if constexpr (FOR_D) {
+    if (!peaked) {  // (uniform over the workgroup)
+      if ((KS == 1 || wave == 0) && hh == 0) column(a, COL_D, qh)[m0 + r] = D;
+      return;
+    }
+  }
   const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
-  if (KS == 1 || wave == 0) {
+  if (!FOR_D && (KS == 1 || wave == 0)) {
     if (hh == 0) {  // (m0 + r < rows_pad)
       column(a, COL_MAX, qh)[m0 + r] = top;
-      if constexpr (!kExact) column(a, COL_D, qh)[m0 + r] = D;
+      if constexpr (!kFound) column(a, COL_D, qh)[m0 + r] = D;
       column(a, COL_LO, qh)[m0 + r] = __int_as_float(row.lo);
       column(a, COL_HI, qh)[m0 + r] = __int_as_float(row.hi);
       if constexpr (sizeof(T) == 4) column(a, COL_INV, qh)[m0 + r] = inv;
@@ -261,7 +275,7 @@ docs_grad_rows_kernel(const Args a) {
     const float most = (float)max(row.pos - row.lo, row.hi - 1 - row.pos), s = a.slopes[qh];
     mid = s * most > 2.f ? 1.f / s : 0.5f * most;
   }
-  float off = 0.f;                      // what D, from a rounded out, was off by
+  float exact = 0.f;  // per lane: sum of P dP
   int t = KS > 1 ? wave : 0, buf = 0;
   if (t < ntile) stage(t, 0);
   for (; t < ntile; t += KS, buf ^= BUFS - 1) {
@@ -290,7 +304,7 @@ docs_grad_rows_kernel(const Args a) {
       s = rows_dot(kf, qf, s);
       dp = rows_dot(vf, dof, dp);
       ColFrag<T> kc;  // (on their way under the next step)
-      read_cols(kt + u * 32 * ROWB, coff, kc);
+      if constexpr (!FOR_D) read_cols(kt + u * 32 * ROWB, coff, kc);
       if constexpr (RW == 1) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (t + KS < ntile) stage(t + KS, 0);
@@ -310,18 +324,10 @@ docs_grad_rows_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) p[i] = pick(bits, i, p[i], 0.f);
       }
-      if constexpr (kExact) {
-        const bool whole = sees && row.lo >= ku && row.hi <= ku + 32;
-        if (__any(whole)) {
-          float x = 0.f;
+      if constexpr (FOR_D) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x = __builtin_fmaf(p[i], dp[i], x);
-          x = swap_sum(x);
-          if (whole && x * 0.f == 0.f) {  // (NaN: from a key behind a mask)
-            off = x - D;
-            D = x;
-          }
-        }
+        for (int i = 0; i < 16; ++i) exact = __builtin_fmaf(p[i], dp[i], exact);
+        return;
       }
       float tpd = 0.f, tpf = 0.f, tpdf = 0.f;
 #pragma unroll
@@ -346,6 +352,19 @@ docs_grad_rows_kernel(const Args a) {
       for (int u = 0; u < NT; ++u) part(u);
     }
   }
+  if constexpr (FOR_D) {
+    exact = swap_sum(exact);
+    if constexpr (KS > 1) {
+      if (hh == 0) shares[wave][0][r] = exact;
+      __syncthreads();
+      exact = 0.f;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) exact += shares[w][0][r];
+    }
+    if (sees && exact * 0.f == 0.f) D = exact;  // (NaN: from a key behind a mask)
+    if ((KS == 1 || wave == 0) && hh == 0) column(a, COL_D, qh)[m0 + r] = D;
+    return;
+  }
   if constexpr (BIAS) {
     pd = swap_sum(pd);
     pf = swap_sum(pf);
@@ -356,7 +375,6 @@ docs_grad_rows_kernel(const Args a) {
   if constexpr (KS == 1) {
     const float probe = swap_sum(not_finite(o));
     const bool again = row.valid && probe != probe;
-    if (kExact && hh == 0) column(a, COL_D, qh)[m0 + r] = D;
     if (BIAS && hh == 0 && !again) column(a, COL_DSLOPE, qh)[m0 + r] = row.hi - row.lo > 1 ? pd * pf - pdf : 0.f;
     __syncthreads();  // (the patches reuse the stages)
     // (a row that sees one key: its weight is 1 whatever the score)
@@ -364,13 +382,12 @@ docs_grad_rows_kernel(const Args a) {
                   [&](int w) { return a.dq + (long)(m0 + w) * a.dq_row + qh * a.dq_head; });
     bad = (unsigned)__ballot(again);
   } else {
-    if (hh == 0) {
-      if constexpr (BIAS) {
+    if constexpr (BIAS) {
+      if (hh == 0) {
         shares[wave][0][r] = pd;
         shares[wave][1][r] = pf;
         shares[wave][2][r] = pdf;
       }
-      if constexpr (kExact) shares[wave][3][r] = off;
     }
     f32x4 y[2];
     sum_waves<KS>(smem, STAGE, o, 1.f, wave, lane, y);  // (with a barrier inside)
@@ -379,12 +396,6 @@ docs_grad_rows_kernel(const Args a) {
     const bool valid = __shfl((int)row.valid, rr, 64), many = __shfl(row.hi - row.lo, rr, 64) > 1;
     bad = bad_of_eight(y, valid);
     const bool again = bad >> (lane >> 3) & 1;
-    if constexpr (kExact) {
-      float exact = __shfl(D - off, rr, 64);
-#pragma unroll
-      for (int w = 0; w < KS; ++w) exact += shares[w][3][rr];
-      if ((lane & 7) == 0) column(a, COL_D, qh)[mr] = exact;  // (mr < rows_pad)
-    }
     if (mr < a.rows && !again) {
       if (valid || a.fill) store_eight<T>(a.dq + (long)mr * a.dq_row + qh * a.dq_head, y, many ? a.scale : 0.f, lane);
       if constexpr (BIAS) {
@@ -703,15 +714,17 @@ int launch_grads(Args a, const KeyPlan& p, hipStream_t st) {
   const char *rows = "fc_attention_docs_backward (rows)", *keys = "fc_attention_docs_backward (keys)";
   const long heads = (long)a.kv_heads * a.share;
   const Shape by = shape_for(sizeof(T) == 4 ? PREC_F32 : PREC_BF16, a.rows, heads, (double)a.k_rows / a.docs);
-  int rc;
   a.tiles = tiles_of(by, a.rows);
   a.by_way = ordered(by, a.docs, a.tiles * heads);
-  if (by == SHARED)
-    rc = launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
-  else if (by == TURNS)
-    rc = launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS>, a.tiles * heads, 4, 4 * 64 * row, a, rows, st);
-  else
-    rc = launch_docs(docs_grad_rows_kernel<T, 1, 1, 32, CAP, BIAS>, a.tiles * heads, 1, 64 * row, a, rows, st);
+  const auto launch_rows = [&](auto for_d) {
+    constexpr bool F = decltype(for_d)::value;
+    if (by == SHARED) return launch_docs(docs_grad_rows_kernel<T, 4, 1, 64, CAP, BIAS, F>, a.tiles * heads, 4, 2 * 128 * row, a, rows, st);
+    if (by == TURNS) return launch_docs(docs_grad_rows_kernel<T, 1, 4, 32, CAP, BIAS, F>, a.tiles * heads, 4, 4 * 64 * row, a, rows, st);
+    return launch_docs(docs_grad_rows_kernel<T, 1, 1, 32, CAP, BIAS, F>, a.tiles * heads, 1, 64 * row, a, rows, st);
+  };
+  int rc = FC_OK;
+  if constexpr (sizeof(T) == 2) rc = launch_rows(std::true_type{});
+  if (rc == FC_OK) rc = launch_rows(std::false_type{});
   if (rc != FC_OK) return rc;
   a.tiles = p.tiles;
   a.splits = p.splits;
