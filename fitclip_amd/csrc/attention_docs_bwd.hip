@@ -12,18 +12,18 @@
 //   keys: 32 keys per wave (K and V in registers), tiles of the rows that see them, one query head of the group after the other - the
 //   gradients of shared heads need no further sum.  S = Q . K^T has the rows of Q on the accumulator rows, and P and dS are the operands of
 //   dV^T = dO^T . P and dK^T = Q^T . dS as they come.
-// bf16: `out` comes rounded, and D = dO.out with it; P and dS are rounded in front of their products (once each: 2^-9 of a term, where the result's
-// own rounding is as much).  D's error matters where few keys have all the weight and no sum over keys evens it out: a kernel in front forms D, and a
-// workgroup of it with such a row (a sum of weights below 8 times the largest: the first rows of a causal document, steep slopes) walks over its
-// keys for D = sum P dP, two products of the three in rows; the others are done at once.  (dS in two parts, an operand for what its rounding left, made d_q's error 1.0 to 1.4 times its
-// own rounding's instead of 1.4 to 1.5, for a third more time in rows: not kept.)
+// bf16: `out` comes rounded, and D = dO.out with it; P and dS are rounded in front of their products (once each: at most 2^-8 of a term, where the
+// result's own rounding is as much).  D's error matters where few keys have all the weight and no sum over keys evens it out: a kernel in front
+// forms D, and a workgroup of it with such a row (a sum of weights below 8 times the largest: the first rows of a causal document, steep
+// slopes) walks over its keys for D = sum P dP, two products of the three in rows; the others are done at once.  (dS in two parts, an operand
+// for what its rounding left, would take d_q from 1.4 times its own rounding's error to 1.0, for a third more time in rows: not kept.)
 // Both have the forward's three shapes (attention_docs.h, shape_for).  The scores and dP are formed twice, 7 products where 5 would do: one
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
 //
 // What bounds them, and what they reach (10 x 64 operations per pair and head that see each other, for both kernels):
-//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads @@4 us
-//     = @@5 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 121 us, keys 200 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
-//     107 and 169, 143 of the latter without bringing any tiles.
+//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1966
+//     us = 699 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 16 + 114 us, keys 198 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
+//     29 + 101 and 166, 84 % of the latter without bringing any tiles.
 //   fp32: the matrix instructions; 4 x 8192 tokens 14.2 ms = 97 TFLOP/s, 136 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
 //     rows 47 us, keys 63 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
 //     2: rows 105, keys 135.
