@@ -12,7 +12,7 @@
 //
 // What bounds it, and what it reaches (4 x 64 operations per pair and head that see each other):
 //   bf16, long ways: vector and matrix instructions, whose times add up for a wave (32 x 32 scores are 8 matrix instructions of 32 cycles and 90
-//     vector ones of 4, 16 of them exponentials of 16): 4 x 8192 tokens, 8 heads 610 us = 901 TFLOP/s; a large product reaches 1144.  With
+//     vector ones of 4, 16 of them exponentials of 16): 4 x 8192 tokens, 8 heads 599 us = 918 TFLOP/s; a large product reaches 1144.  With
 //     3 x 3136 tokens, 12 heads, 888 workgroups for room for 768: 120 us = 755 TFLOP/s.
 //   fp32: the matrix instructions (16 times as long as bf16's for a product); 4 x 8192 tokens 4157 us = 132 TFLOP/s of 153, one document of 3136
 //     tokens (98 x 12 workgroups of 32 rows) 268 us = 113.

@@ -21,8 +21,8 @@
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
 //
 // What bounds them, and what they reach (10 x 64 operations per pair and head that see each other, for both kernels):
-//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1966
-//     us = 699 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 16 + 114 us, keys 198 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
+//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1928
+//     us = 713 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 16 + 114 us, keys 198 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
 //     29 + 101 and 166, 84 % of the latter without bringing any tiles.
 //   fp32: the matrix instructions; 4 x 8192 tokens 14.2 ms = 97 TFLOP/s, 136 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
 //     rows 47 us, keys 63 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
