@@ -578,6 +578,11 @@ def _apart(t: torch.Tensor, name: str, **others: torch.Tensor) -> None:
             raise ValueError(f"{name} overlaps {other}")
 
 
+def _in_place_or_apart(out: torch.Tensor, t: torch.Tensor, name: str) -> None:
+    if (out.data_ptr() != t.data_ptr() or _strides(out) != _strides(t)) and _meet(out, t):
+        raise ValueError(f"out overlaps {name}: in place needs the same place and strides")
+
+
 def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
     for name, t in tensors.items():
         if t is None:
@@ -650,8 +655,7 @@ def _check_rotary(x, positions, inv_freq, sections, out) -> None:
         raise ValueError(f"{axes} sections that sum up to {pairs} pairs are needed, got {list(sections)}")
     if out is not None:
         _written(out, "out", x)
-        if (out.data_ptr() != x.data_ptr() or _strides(out) != _strides(x)) and _meet(out, x):
-            raise ValueError("out overlaps x: in place needs the same place and strides")
+        _in_place_or_apart(out, x, "x")
     _on_device(x.get_device(), x=x, positions=positions, inv_freq=inv_freq, out=out)
 
 
@@ -717,11 +721,13 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
     cap tanh(score / cap) if `cap` > 0, minus slopes[head] * distance if `slopes` (float32 [heads]) is given.  A row that sees no
     key gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
 
-    Rows behind the last document are left as they were in a given `out` (which may not overlap k or v), and 0 otherwise."""
+    Rows behind the last document are left as they were in a given `out`, and 0 otherwise.  `out` may be q (in place: the same place and
+    strides), and must not overlap it otherwise, nor k or v."""
     if out is not None:
         _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
         _written(out, "out", q)
         _apart(out, "out", k=k, v=v)
+        _in_place_or_apart(out, q, "q")
     d = _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, out is None)
     index, (rows, heads, _), docs = q.get_device(), q.shape, d.docs
     fresh = out is None

@@ -223,7 +223,7 @@ typedef struct {
  * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 where it sees nothing): what the gradients and a later
  * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
  * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
- * infinities included.  out must not overlap k or v.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
+ * infinities included.  out may be q (with q's strides) and must not overlap it otherwise, nor k or v.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
 FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
                       size_t scratch_bytes, fc_stream stream);
