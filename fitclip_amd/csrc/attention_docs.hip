@@ -4,6 +4,8 @@
 // accumulator IS the operand of O^T = V^T . P^T.  K and V stream through LDS in tiles between the lowest and the highest key that a row of
 // the workgroup sees; a wave skips tiles that none of its 32 rows sees and masks only tiles that one of them sees in part.
 //
+// A row whose scores are all -inf (keys of -inf, products beyond fp32) has a sum of 0, as one that sees nothing: its result is 0.
+//
 // The sums refer to a maximum that follows the true one in steps of 2^8: rescaling O at every tile would cost a quarter more vector
 // instructions, and fp32 has the headroom.
 //
@@ -29,7 +31,7 @@ namespace {
 
 // One kernel row again, key by key (64 lanes = 64 keys for the scores, 64 dimensions for the sums), over keys [lo, hi).
 template <typename T, bool CAP, bool BIAS>
-__device__ void row_again(const Args& a, int head, int m, int lo, int hi, int pos, int split, bool sees, int lane) {
+__device__ void row_again(const Args& a, int head, int m, int lo, int hi, int pos, int split, int lane) {
   const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
   const float q = value_at<T>(a.q + token * a.q_row + qh * a.q_head, lane), slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
   const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
@@ -53,7 +55,7 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
     if (lane == 0) *reinterpret_cast<f32x2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64 + at * 2) = f32x2{top, l};
     return;
   }
-  put_at<T>(a.out + token * a.out_row + qh * a.out_head, lane, sees ? o / l : 0.f);
+  put_at<T>(a.out + token * a.out_row + qh * a.out_head, lane, l == 0.f ? 0.f : o / l);
   if (lane == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{top, l};
 }
 
@@ -269,7 +271,7 @@ attention_docs_kernel(const Args a) {
         if (hh == 0) part_ml[at] = float2{mtop, row.valid ? l : -1.f};  // (sum -1: a row of no document)
       }
     } else {
-      const float inv = sees ? down / l : 0.f;
+      const float inv = sees && l != 0.f ? down / l : 0.f;
       const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
       if (hh == 0 && write) {
         int m = m0 + r;
@@ -314,7 +316,7 @@ attention_docs_kernel(const Args a) {
       }
     } else if (write) {
       const int tk = a.group.div(mr), h = head * (int)a.group.d + (mr - tk * (int)a.group.d);
-      store_eight<T>(a.out + tk * a.out_row + h * a.out_head, y, see ? 1.f / sum : 0.f, lane);
+      store_eight<T>(a.out + tk * a.out_row + h * a.out_head, y, see && sum != 0.f ? 1.f / sum : 0.f, lane);
       if ((lane & 7) == 0)
         *reinterpret_cast<f32x2*>(a.stats + ((long)tk * a.kv_heads * (int)a.group.d + h) * 2) = f32x2{valid ? top : -kInf, valid ? sum : 0.f};
     }
@@ -323,7 +325,7 @@ attention_docs_kernel(const Args a) {
     const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
     const int lo = __builtin_amdgcn_readlane(row.lo, w), hi = __builtin_amdgcn_readlane(row.hi, w), pos = __builtin_amdgcn_readlane(row.pos, w);
-    row_again<T, CAP, BIAS>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lo < hi, lane);
+    row_again<T, CAP, BIAS>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lane);
   }
 }
 
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(256) attention_docs_join_kernel(const Args a) 
     l += sums[s][64];
   }
   const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-  const bool zero = !valid || l == 0.f;  // (sum 0: the row sees nothing)
+  const bool zero = !valid || l == 0.f;
   put_at<T>(a.out + token * a.out_row + qh * a.out_head, tid, zero ? 0.f : x / l);
   if (tid == 0) *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{valid ? top : -kInf, valid ? l : 0.f};
 }

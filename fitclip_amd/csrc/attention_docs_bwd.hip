@@ -185,8 +185,9 @@ docs_grad_rows_kernel(const Args a) {
   RowFrag<T> of;
   if constexpr (kFound) D = column(a, COL_D, qh)[m0 + r];
   else of.load(a.out + m * a.out_row + qh * a.out_head, hh);
-  const Row row = find_row(a, m0, lane);
+  Row row = find_row(a, m0, lane);
   if constexpr (!kFound) D = swap_sum(dot(of, dof));
+  if (st[1] == 0.f) row.hi = row.lo;  // (every score -inf: the row weighs nothing, as if it saw nothing)
   const bool sees = row.lo < row.hi;
   const int wlo = wave_min_i(sees ? row.lo : INT_MAX), whi = wave_max_i(sees ? row.hi : -INT_MAX);
   const int full_lo = wave_max_i(row.valid ? (sees ? row.lo : INT_MAX) : -INT_MAX);

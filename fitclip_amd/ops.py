@@ -719,7 +719,7 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets:
     not decreasing; k_offsets defaults to q_offsets).  Its last query stands at its last key.  `causal`: a query sees the keys up to
     its own place, and the first prefix[d] ones (`prefix` int32 [docs]).  Scores are scale q.k (scale 1 / 8 by default), bent to
     cap tanh(score / cap) if `cap` > 0, minus slopes[head] * distance if `slopes` (float32 [heads]) is given.  A row that sees no
-    key gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
+    key, or scores -inf with all of them, gets 0.  stats: the row's largest score in units of ln 2 and the sum of 2^(score - largest).
 
     Rows behind the last document are left as they were in a given `out`, and 0 otherwise.  `out` may be q (in place: the same place and
     strides), and must not overlap it otherwise, nor k or v."""

@@ -219,8 +219,8 @@ typedef struct {
   const float* slopes;
 } fc_docs;
 #define FC_DOCS_INIT {(int32_t)sizeof(fc_docs)}
-/* out = softmax(scores) v per row and head (0 where a row sees nothing); stats dev f32 [q_rows, q_heads, 2] <- the row's largest
- * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 where it sees nothing): what the gradients and a later
+/* out = softmax(scores) v per row and head (0 where a row sees nothing, or scores of -inf alone); stats dev f32 [q_rows, q_heads, 2] <- the row's largest
+ * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 in rows of 0): what the gradients and a later
  * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
  * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
  * infinities included.  out may be q (with q's strides) and must not overlap it otherwise, nor k or v.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
