@@ -41,6 +41,12 @@ struct FastDiv {
   __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, mul) >> (shift - 1)); }
 };
 
+// A weight is 2^(fma(raw score, c, -maximum)): the product keeps all its bits, the maximum is rounded to 24, and where it is large the largest weight
+// is no longer 1.  The forward's sum makes up for that (both gradients divide by it) as long as neither leaves fp32, which it can from 2^30 on; in
+// bf16 the gradients add the sum's logarithm to the maximum, which is off by half a bf16 step from 2^17 on.  Rows with a maximum as far away as
+// this are done again key by key, from rounded scores whose largest less the maximum is 0.
+template <typename T> constexpr float kFar = sizeof(T) == 4 ? 16777216.f : 131072.f;
+
 struct Args {
   const char *q, *k, *v;                                // strides in bytes
   long q_row, q_head, k_row, k_head, v_row, v_head;
@@ -453,11 +459,12 @@ __device__ __forceinline__ void cols_dot(const ColFrag<float>& f, const f32x16& 
     for (int n = 0; n < 2; ++n) out[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(f.v[i][n], p[i], out[n], 0, 0, 0);
 }
 
-// score of a raw product in log2 units
+// score of a raw product in log2 units, rounded (hipcc would multiply again in the fma that takes the maximum off)
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ float score(const Args& a, float raw, float slope, float far) {
   float x = CAP ? a.c * tanh_f32(raw * a.cap_in) : raw * a.c;
   if constexpr (BIAS) x = __builtin_fmaf(-slope, far, x);
+  asm("" : "+v"(x));
   return x;
 }
 
@@ -571,14 +578,14 @@ __device__ __forceinline__ void store_eight(char* dst, const f32x4 (&y)[2], floa
     *reinterpret_cast<bf16x8*>(dst + 16 * (lane & 7)) = w;
   }
 }
-// which of the wave's eight rows hold a value that is not finite (bit k: row 8 w + k)
-__device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool counts) {
+// which of the wave's eight rows hold a value that is not finite, or are bad already (bit k: row 8 w + k)
+__device__ __forceinline__ unsigned bad_of_eight(const f32x4 (&y)[2], bool counts, bool bad = false) {
   float x = 0.f;
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int e = 0; e < 4; ++e) x = __builtin_fmaf(y[c][e], 0.f, x);
-  const unsigned long long b = __ballot(counts && x != x);
+  const unsigned long long b = __ballot(counts && (bad || x != x));
   unsigned rows = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) rows |= (unsigned)((b >> (8 * k) & 0xff) != 0) << k;

@@ -248,6 +248,7 @@ attention_docs_kernel(const Args a) {
 #pragma unroll
     for (int u = 0; u < NT; ++u) cols_dot(vf[u], s[u], o);
   }
+  const auto far_away = [](float x) { return x != -kInf && fabsf(x) >= kFar<T>; };
   l = swap_sum(l);
   float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
   l *= down;
@@ -257,7 +258,7 @@ attention_docs_kernel(const Args a) {
 
   if constexpr (KS == 1) {
     const float probe = swap_sum(not_finite(o));
-    const bool again = row.valid && probe != probe;
+    const bool again = row.valid && (probe != probe || far_away(mtop));
     if (a.splits > 1) {
       const long at = ((long)split * a.kv_heads + head) * a.rows + m0 + r;
       if (m0 + r < a.rows && !again) {
@@ -306,7 +307,7 @@ attention_docs_kernel(const Args a) {
     const bool valid = __shfl((int)row.valid, rr, 64), see = __shfl((int)sees, rr, 64);
     top = __shfl(top, rr, 64);
     sum = __shfl(sum, rr, 64);
-    bad = bad_of_eight(y, valid);
+    bad = bad_of_eight(y, valid, far_away(top));
     const bool again = bad >> (lane >> 3) & 1, write = mr < a.rows && !again && (valid || a.fill || a.splits > 1);
     if (a.splits > 1) {
       const long at = ((long)split * a.kv_heads + head) * a.rows + mr;

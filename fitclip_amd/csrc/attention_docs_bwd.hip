@@ -72,34 +72,43 @@ __device__ __forceinline__ float bent_by(const Args& a, float raw, float ds) {
   return ds;
 }
 
-// d_q of one row again, key by key (see attention_docs.h)
+// d_q of one row again, key by key (see attention_docs.h), with D from the same weights: where one key has all the weight, dP - D is exactly 0
 template <typename T, bool CAP, bool BIAS>
-__device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int pos, float top, float inv, float D, int lane) {
+__device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int pos, int lane) {
   const int head = qh / a.share;
+  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * a.kv_heads * a.share + qh) * 2);
+  const float top = st[0], inv = 1.f / st[1];
   const float q = value_at<T>(a.q + m * a.q_row + qh * a.q_head, lane), go = value_at<T>(a.d_out + m * a.do_row + qh * a.do_head, lane);
   const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
   const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
-  float o = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f;
+  float o = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f, raw, far, p, g;
+  const auto weigh = [&](int j) {
+    const int key = min(j + lane, hi - 1);
+    raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
+    p = j + lane < hi ? __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - top) * inv : 0.f;
+    g = row_dot<T>(vb + key * a.v_row, go);
+  };
 #pragma unroll 1
   for (int j = lo; j < hi; j += 64) {
-    const int key = min(j + lane, hi - 1);
-    const float raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
-    float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - top) * inv;
-    const float g = row_dot<T>(vb + key * a.v_row, go);
-    if (j + lane >= hi) p = 0.f;
+    weigh(j);
     pd = __builtin_fmaf(p, g, pd);
     pf = __builtin_fmaf(p, far, pf);
     pdf = __builtin_fmaf(p * g, far, pdf);
+  }
+  const float D = wave_sum(pd);
+  if (lane == 0) column(a, COL_D, qh)[m] = D;
+#pragma unroll 1
+  for (int j = lo; j < hi; j += 64) {
+    weigh(j);
     const float ds = bent_by<CAP>(a, raw, p * (g - D));
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
   }
   put_at<T>(a.dq + m * a.dq_row + qh * a.dq_head, lane, hi - lo > 1 ? o * a.scale : 0.f);
   if constexpr (BIAS) {
-    pd = wave_sum(pd);
     pf = wave_sum(pf);
     pdf = wave_sum(pdf);
-    if (lane == 0) column(a, COL_DSLOPE, qh)[m] = hi - lo > 1 ? pd * pf - pdf : 0.f;
+    if (lane == 0) column(a, COL_DSLOPE, qh)[m] = hi - lo > 1 ? D * pf - pdf : 0.f;
   }
 }
 
@@ -142,8 +151,8 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
       if (!seen) continue;
       const float raw = row_dot<T>(qb + m * a.q_row, k), g = row_dot<T>(db + m * a.do_row, v);
       const float far = BIAS ? fabsf((float)(__float_as_int(column(a, COL_POS, qh)[m]) - key)) : 0.f;
-      float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - column(a, COL_MAX, qh)[m]);
-      if constexpr (sizeof(T) == 4) p *= column(a, COL_INV, qh)[m];
+      const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * a.kv_heads * a.share + qh) * 2);
+      const float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - st[0]) * (1.f / st[1]);
       const float ds = hi - lo == 1 ? 0.f : bent_by<CAP>(a, raw, p * (g - column(a, COL_D, qh)[m]));
 #pragma unroll 1
       for (int w = 0; w < 64; ++w) {
@@ -218,6 +227,7 @@ docs_grad_rows_kernel(const Args a) {
     if (sees) top += __builtin_amdgcn_logf(st[1]);
     inv = 1.f;
   }
+  if (sees && fabsf(st[0]) >= kFar<T>) top = __builtin_nanf("");  // (done again, by this kernel and for the keys that the row sees)
   if (!sees) D = 0.f;
   if constexpr (FOR_D) {
     if (!peaked) {  // (uniform over the workgroup)
@@ -417,7 +427,7 @@ docs_grad_rows_kernel(const Args a) {
     const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
     row_grad_again<T, CAP, BIAS>(a, qh, m0 + w, __builtin_amdgcn_readlane(row.lo, w), __builtin_amdgcn_readlane(row.hi, w),
-                                 __builtin_amdgcn_readlane(row.pos, w), lane_value(top, w), lane_value(inv, w), lane_value(D, w), lane);
+                                 __builtin_amdgcn_readlane(row.pos, w), lane);
   }
 }
 

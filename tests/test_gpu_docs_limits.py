@@ -53,3 +53,76 @@ def test_rows_whose_scores_are_all_minus_infinity(dtype, shape, how):
     for got, want, start, roundings in ((out, clean[0], m, 3), (grads[0], clean[2], m, 8), (grads[1], clean[3], n, 8), (grads[2], clean[4], n, 8)):
         got, want = got[start:].double(), want[start:].double()
         assert float((got - want).abs().max()) <= (roundings * R.HALF[dtype] + 5440 * 2.0 ** -24) * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale,size,slopes", [(1e30, 1.0, False), (1e12, 1.0, False), (0.125, 1e5, False), (1e30, 1.0, True)])
+def test_scores_so_large_that_one_key_has_all_the_weight(dtype, shape, scale, size, slopes):
+    """Scores of up to 1e31, the largest of a row (beyond 2^24 in units of ln 2) 100 and more above the others, whatever the rounding of the products:
+    the result is that key's value and its gradient the sum of the rows' that chose it, and q and k get no gradient at all."""
+    q_len, k_len, heads = SHAPES[shape]
+    rows, keys = sum(q_len), sum(k_len or q_len)
+    q, k, v = (size * _rand(rows, heads, 64, seed=11)).to(dtype), (size * _rand(keys, heads, 64, seed=12)).to(dtype), _rand(keys, heads, 64, seed=13, dtype=dtype)
+    d_out = _rand(rows, heads, 64, seed=14, dtype=dtype)
+    off = (R.offsets(q_len), None if k_len is None else R.offsets(k_len))
+    how = dict(scale=scale, causal=True) | (dict(slopes=torch.full((heads,), 0.5, device=DEV)) if slopes else {})
+    out, stats = ops.attention_docs(q, k, v, *off, **how)
+    d_q, d_k, d_v = ops.attention_docs_backward(d_out, q, k, v, out, stats, *off, **how)[:3]
+    want_v, sizes = torch.zeros(keys, heads, 64, dtype=torch.float64), torch.zeros(keys, heads, 64, dtype=torch.float64)
+    a = b = 0
+    plain = torch.zeros(rows, heads, dtype=torch.bool)  # rows whose choice no rounding can change
+    chosen = torch.zeros(rows, heads, dtype=torch.long)
+    for n, m in zip(q_len, k_len or q_len):
+        x, y = q[a:a + n].cpu().double().transpose(0, 1), k[b:b + m].cpu().double().transpose(0, 1)
+        hidden = torch.arange(m)[None] > torch.arange(n)[:, None] + (m - n)
+        score = (x @ y.transpose(1, 2).contiguous() * scale).masked_fill(hidden, -math.inf)
+        sure = 4 * 68 * 2.0 ** -24 * scale * (x.abs() @ y.abs().transpose(1, 2).contiguous()).amax(-1) + 100 + 0.5 * m
+        top = score.topk(2, -1)
+        plain[a:a + n] = ((top.values[..., 0] - top.values[..., -1] > sure) & (top.values[..., 0].abs() > 1.2e7)).t()
+        chosen[a:a + n] = top.indices[..., 0].t() + b
+        a, b = a + n, b + m
+    assert plain.float().mean() > 0.9  # (a check of the inputs)
+    at = chosen[..., None].expand(-1, -1, 64)
+    picked = v.cpu().gather(0, at)
+    assert torch.equal(out.cpu()[plain], picked[plain])
+    assert not d_q.cpu()[plain].any()
+    d_out64 = d_out.cpu().double()
+    want_v.scatter_add_(0, at, d_out64)
+    sizes.scatter_add_(0, at, d_out64.abs())
+    sure_keys = torch.ones(keys, heads, dtype=torch.bool)  # keys of documents and heads in which every row's choice is plain
+    a = b = 0
+    for n, m in zip(q_len, k_len or q_len):
+        sure_keys[b:b + m] = plain[a:a + n].all(0)
+        a, b = a + n, b + m
+    assert sure_keys.any()
+    assert not d_k.cpu()[sure_keys].any()
+    bound = R.HALF[dtype] * want_v.abs() + rows * 2.0 ** -24 * sizes  # a sum of up to `rows` terms in fp32, rounded once
+    assert ((d_v.cpu().double() - want_v).abs() <= bound)[sure_keys].all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_weights_of_large_scores_add_up_to_one(dtype, shape):
+    """Scores of 2^16 to 2^26 (on both sides of what a maximum rounded to 24 bits can do), several keys of comparable weight: whatever each weight is, a row's add up
+    to 1, so a document's d_v adds up to its d_out."""
+    q_len, k_len, heads = SHAPES[shape]
+    rows, keys = sum(q_len), sum(k_len or q_len)
+    off = (R.offsets(q_len), None if k_len is None else R.offsets(k_len))
+    for large in (2.0 ** 8, 2.0 ** 9, 2.0 ** 10, 2.0 ** 13):  # scores of large^2 x 8 / 8
+        q, k = _rand(rows, heads, 64, seed=21, dtype=dtype), _rand(keys, heads, 64, seed=22, dtype=dtype)
+        q[..., :8], k[..., :8] = large, large
+        v, d_out = _rand(keys, heads, 64, seed=23, dtype=dtype), _rand(rows, heads, 64, seed=24, dtype=dtype)
+        out, stats = ops.attention_docs(q, k, v, *off)
+        d_q, d_k, d_v = ops.attention_docs_backward(d_out, q, k, v, out, stats, *off)
+        assert all(torch.isfinite(t).all() for t in (out, d_q, d_k, d_v))
+        a = b = 0
+        for n, m in zip(q_len, k_len or q_len):
+            got, want = d_v[b:b + m].double().sum(0), d_out[a:a + n].double().sum(0)
+            # d_v's rounding; bf16: the weights' in front of the product, half a step of the maximum's size in log2 units in the exponent
+            # (2^-7 ln 2 at 2^17, at most); sums of n and m terms in fp32, exponents of up to 64 in
+            # units of 2^-24 on both sides
+            terms = d_out[a:a + n].double().abs().sum(0)
+            bound = R.HALF[dtype] * (d_v[b:b + m].double().abs().sum(0) + terms) + ((2.0 ** -7 if dtype == torch.bfloat16 else 0) + (n + m + 256) * 2.0 ** -24) * terms
+            assert ((got - want).abs() <= bound).all(), (large, float(((got - want).abs() / bound).max()))
+            a, b = a + n, b + m
