@@ -624,6 +624,7 @@ inline int ordered(Shape s, int docs, long workgroups) { return s != ALONE && do
 
 int check_docs(const fc_docs* d, const char* what);
 bool rows_aligned(const void* p, int64_t row, int64_t head, int kind);
+bool capped(const fc_docs& d);
 Args make_args(const fc_docs& d);
 
 }  // namespace docs

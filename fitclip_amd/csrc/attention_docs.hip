@@ -459,6 +459,9 @@ bool rows_aligned(const void* p, int64_t row, int64_t head, int kind) {
   return !(((uintptr_t)p & 15) || ((row | head) * (kind == PREC_F32 ? 4 : 2) & 15));
 }
 
+// (a cap so far above the scale that fp32 has too few bits of the quotient left is none: only products beyond 1e34 would come near it)
+bool capped(const fc_docs& d) { return d.cap > 0.f && (double)d.scale / d.cap >= 0x1p-127; }
+
 Args make_args(const fc_docs& d) {
   const int size = d.kind == PREC_F32 ? 4 : 2;
   Args a{};
@@ -472,13 +475,13 @@ Args make_args(const fc_docs& d) {
   a.group = FastDiv((unsigned)(d.q_heads / d.kv_heads));
   a.rows = (int)(d.q_rows * (d.q_heads / d.kv_heads));
   a.causal = d.causal; a.fill = d.fill;
-  a.c = (float)((double)(d.cap > 0.f ? d.cap : d.scale) * 1.4426950408889634);
-  if (d.cap > 0.f) {
+  a.c = (float)((double)(capped(d) ? d.cap : d.scale) * 1.4426950408889634);
+  if (capped(d)) {
     const double u = std::min((double)d.scale / d.cap, 1e30);  // (beyond, every score but 0 is at the cap all the same)
     a.cap_in = (float)u;
     a.near[0] = (float)u;
     for (int k = 0; k < 3; ++k) a.near[k + 1] = (float)(kNear[k] * std::pow(u, 2 * k + 3));
-    a.near_end = u < 1e5 ? (float)(kTanhNear / u) : 0.f;  // (beyond, the coefficients leave fp32)
+    a.near_end = u > 1e-5 && u < 1e5 ? (float)(kTanhNear / u) : 0.f;  // (else the coefficients, or the squares of the products, leave fp32)
   }
   a.scale = d.scale;
   a.splits = 1;
@@ -521,7 +524,7 @@ int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_
   a.tiles = p.tiles;
   a.splits = p.splits;
   a.by_way = ordered(p.shape, d->docs, p.splits == 1 ? (long)p.tiles * d->kv_heads : 0);
-  return d->kind == PREC_F32 ? docs::launch_type<float>(a, d->cap > 0.f, p.shape, st) : docs::launch_type<bf16>(a, d->cap > 0.f, p.shape, st);
+  return d->kind == PREC_F32 ? docs::launch_type<float>(a, docs::capped(*d), p.shape, st) : docs::launch_type<bf16>(a, docs::capped(*d), p.shape, st);
 }
 
 }  // extern "C"

@@ -815,7 +815,7 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
   const docs::KeyPlan p = docs::plan_keys(*d);
   a.part = reinterpret_cast<float*>((char*)scratch + docs::table_bytes(*d));
   a.rows_pad = docs::pad_rows(*d);
-  return d->kind == PREC_F32 ? docs::launch_grads_type<float>(a, p, d->cap > 0.f, st) : docs::launch_grads_type<bf16>(a, p, d->cap > 0.f, st);
+  return d->kind == PREC_F32 ? docs::launch_grads_type<float>(a, p, docs::capped(*d), st) : docs::launch_grads_type<bf16>(a, p, docs::capped(*d), st);
 }
 
 }  // extern "C"

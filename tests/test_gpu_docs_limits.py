@@ -126,3 +126,44 @@ def test_weights_of_large_scores_add_up_to_one(dtype, shape):
             bound = R.HALF[dtype] * (d_v[b:b + m].double().abs().sum(0) + terms) + ((2.0 ** -7 if dtype == torch.bfloat16 else 0) + (n + m + 256) * 2.0 ** -24) * terms
             assert ((got - want).abs() <= bound).all(), (large, float(((got - want).abs() / bound).max()))
             a, b = a + n, b + m
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale,cap", [(1.0, 1e6), (1.0, 1e8), (1.0, 1e10), (1.0, 1e14), (1.0, 1e20), (1e-20, 30.0), (1e-25, 1.0), (1e-30, 1e8)])
+def test_caps_far_above_the_scale(dtype, scale, cap):
+    """Scores of a quarter of the cap, where it bends them by 2 %, for quotients scale / cap down to 1e-38: powers of the quotient leave fp32."""
+    rows, heads = 33, 2
+    size = (0.25 * cap / scale / 64) ** 0.5  # all products positive: `big` of the error bound is the score itself
+    q, k = ((size * (0.9 + 0.1 * torch.rand(rows, heads, 64, generator=torch.Generator().manual_seed(s)))).to(dtype).to(DEV) for s in (31, 32))
+    v, d_out = _rand(rows, heads, 64, seed=33, dtype=dtype), _rand(rows, heads, 64, seed=34, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, R.offsets([rows]), cap=cap, scale=scale)
+    ref = R.attention(q, k, v, [rows], cap=cap, scale=scale)
+    ds = R.score_error(ref, rows, cap=cap, scale=scale)
+    want = ref["stats"][..., 0]
+    assert ((stats[..., 0].double().cpu() - want).abs() <= R.LOG2E * ds + 2.0 ** -23 * want.abs()).all()
+    assert torch.isfinite(out).all()
+    grads = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets([rows]), cap=cap, scale=scale)
+    assert all(torch.isfinite(g).all() for g in grads)
+    # whatever each weight is, a row's add up to 1
+    bound = R.HALF[dtype] * (grads[2].double().abs().sum(0) + d_out.double().abs().sum(0)) + ((2.0 ** -7 if dtype == torch.bfloat16 else 0) + 400 * 2.0 ** -24) * d_out.double().abs().sum(0)
+    assert ((grads[2].double().sum(0) - d_out.double().sum(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale,cap", [(1e-30, 1e30), (1e-36, 30.0), (1e-20, 1e20), (1e-10, 1e29)])
+def test_small_scores_under_far_caps(dtype, scale, cap):
+    """Scores of up to 4 or so from a small scale and large products, below the cap by up to 29 powers of ten."""
+    q_len = [40, 3]
+    size = (1 / scale) ** 0.5 / 4
+    q, k = (size * _rand(43, 2, 64, seed=35)).to(dtype), (size * _rand(43, 2, 64, seed=36)).to(dtype)
+    v, d_out = _rand(43, 2, 64, seed=37, dtype=dtype), _rand(43, 2, 64, seed=38, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, R.offsets(q_len), causal=True, cap=cap, scale=scale)
+    ref = R.attention(q, k, v, q_len, causal=True, cap=cap, scale=scale)
+    ds = R.score_error(ref, 40, scale=scale, cap=cap)
+    assert ((out.double().cpu() - ref["out"]).abs() <= R.out_bound(ref, v, dtype, 40, ds)).all()
+    assert float(ref["stats"][..., 1].max()) > 2 and float((stats[..., 0].double().cpu() - ref["stats"][..., 0]).abs().max()) <= R.LOG2E * ds + 2.0 ** -20
+    # (30 is no far cap: it bends a score of 4 by 0.6 %, so the weights are those of the definition with its cap, not those without one)
+    ref = R.attention(q, k, v, q_len, causal=True, cap=cap, scale=scale, d_out=d_out)
+    d_v = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=True, cap=cap, scale=scale)[2]
+    bound = R.grad_bounds(ref, q, k, v, d_out, dtype, 40, ds, cap, scale=scale)["d_v"]
+    assert ((d_v.double().cpu() - ref["d_v"]).abs() <= bound).all()
