@@ -659,6 +659,9 @@ def _check_rotary(x, positions, inv_freq, sections, out) -> None:
     _on_device(x.get_device(), x=x, positions=positions, inv_freq=inv_freq, out=out)
 
 
+_SMALL = 2.0 ** -149  # the smallest number of fp32: a cap below it would come out as none
+
+
 def _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale) -> None:
     _heads(q, "q", q.dtype), _heads(k, "k", q.dtype), _heads(v, "v", q.dtype)
     if k.shape != v.shape:
@@ -676,8 +679,8 @@ def _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scal
     _vector(slopes, "slopes", torch.float32, q.shape[1])
     if prefix is not None and not causal:
         raise ValueError("a prefix mask needs causal=True")
-    if not 0 < scale <= 1e30 or not 0 <= cap <= 1e30:
-        raise ValueError(f"scale must be positive and cap 0 (none) or positive, neither above 1e30, got {scale} and {cap}")
+    if not _SMALL <= scale <= 1e30 or not (cap == 0 or _SMALL <= cap <= 1e30):
+        raise ValueError(f"scale must be positive and cap 0 (none) or positive, neither above 1e30 or rounded to 0 in float32, got {scale} and {cap}")
     _on_device(q.get_device(), q=q, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, prefix=prefix, slopes=slopes)
 
 
@@ -696,7 +699,8 @@ def _docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale, fil
             and (docs := q_offsets.numel() - 1) >= 0 and _fine(q_offsets, torch.int32, docs + 1, index)
             and (k_shape[0] == q_shape[0] if k_offsets is None else _fine(k_offsets, torch.int32, docs + 1, index))
             and (prefix is None or causal and _fine(prefix, torch.int32, docs, index))
-            and (slopes is None or _fine(slopes, torch.float32, q_shape[1], index)) and 0 < scale <= 1e30 and 0 <= cap <= 1e30):
+            and (slopes is None or _fine(slopes, torch.float32, q_shape[1], index)) and _SMALL <= scale <= 1e30
+            and (cap == 0 or _SMALL <= cap <= 1e30)):
         _check_docs(q, k, v, q_offsets, k_offsets, causal, prefix, slopes, cap, scale)
     q_heads, k_heads = q_shape[1], k_shape[1]
     q_many, k_many = q_shape[0] > 1, k_shape[0] > 1

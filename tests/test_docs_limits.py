@@ -39,3 +39,13 @@ def test_the_c_entry_takes_q_as_out_with_its_strides_alone():
     for change in (dict(out_row=512), dict(out_head=128)):
         a = dict(out=4096, out_row=256, out_head=64) | change
         assert lib.fc_attention_docs(_c_docs(), *a.values(), 4096, None, 0, None) == -1 and b"in place" in lib.fc_last_error()
+
+
+@pytest.mark.parametrize("how", [dict(cap=1e-50), dict(cap=2.0 ** -150), dict(scale=1e-46), dict(cap=float("nan")), dict(cap=float("inf"))])
+def test_caps_and_scales_that_float32_cannot_hold(how):
+    """A cap that is rounded to 0 would be none at all."""
+    q = torch.zeros(8, 2, 64)
+    with pytest.raises(ValueError, match="scale must be positive"):
+        ops.attention_docs(q, q, q, OFF, **how)
+    with pytest.raises(_lib.FitclipHipError, match="no CPU fallback"):
+        ops.attention_docs(q, q, q, OFF, cap=2.0 ** -149, scale=2.0 ** -149)
