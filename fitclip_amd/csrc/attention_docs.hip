@@ -508,6 +508,7 @@ int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_
   if (!out || !stats) return fail(FC_EINVAL, "fc_attention_docs: null output");
   if (!docs::rows_aligned(out, out_row, out_head, d->kind) || ((uintptr_t)stats & 7))
     return fail(FC_EINVAL, "fc_attention_docs: outputs must start on 16-byte boundaries");
+  if ((out_row | out_head) < 0) return fail(FC_EINVAL, "fc_attention_docs: negative strides");
   if (out == d->q && ((d->q_rows > 1 && out_row != d->q_row) || (d->q_heads > 1 && out_head != d->q_head)))
     return fail(FC_EINVAL, "fc_attention_docs: in place needs q's strides");
   const docs::Plan p = docs::plan_forward(*d);

@@ -791,6 +791,8 @@ int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_ro
       !docs::rows_aligned(d_q, dq_row, dq_head, d->kind) || !docs::rows_aligned(d_k, dk_row, dk_head, d->kind) ||
       !docs::rows_aligned(d_v, dv_row, dv_head, d->kind) || ((uintptr_t)stats & 7))
     return fail(FC_EINVAL, "fc_attention_docs_backward: rows and heads must start on 16-byte boundaries");
+  if ((out_row | out_head | do_row | do_head | dq_row | dq_head | dk_row | dk_head | dv_row | dv_head) < 0)
+    return fail(FC_EINVAL, "fc_attention_docs_backward: negative strides");
   if (do_row * (d->kind == PREC_F32 ? 4 : 2) >= 1 << 25)
     return fail(FC_EINVAL, "fc_attention_docs_backward: rows of d_out lie 32 MiB or more apart");
   const size_t need = docs::grad_bytes(*d);

@@ -49,3 +49,19 @@ def test_caps_and_scales_that_float32_cannot_hold(how):
         ops.attention_docs(q, q, q, OFF, **how)
     with pytest.raises(_lib.FitclipHipError, match="no CPU fallback"):
         ops.attention_docs(q, q, q, OFF, cap=2.0 ** -149, scale=2.0 ** -149)
+
+
+def test_the_c_entries_refuse_negative_strides_of_results_and_d_out():
+    """d_out's row stride goes into 32-bit offsets: a negative one would read far outside."""
+    lib = _lib.load()
+    d = _c_docs()
+    for change in (dict(row=-256), dict(head=-64)):
+        a = dict(out=8192, row=256, head=64) | change
+        assert lib.fc_attention_docs(d, *a.values(), 4096, None, 0, None) == -1 and b"negative" in lib.fc_last_error()
+    for at in range(5):  # out, d_out, d_q, d_k, d_v
+        for which in (0, 1):
+            strides = [[256, 64], [256, 64], [256, 64], [128, 64], [128, 64]]
+            strides[at][which] *= -1
+            o, g, q, k, v = strides
+            assert lib.fc_attention_docs_backward(d, 4096, *o, 4096, 4096, *g, 4096, *q, 4096, *k, 4096, *v, None, 4096, 1 << 30, None) == -1
+            assert b"negative" in lib.fc_last_error(), lib.fc_last_error()
