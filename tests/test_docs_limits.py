@@ -65,3 +65,10 @@ def test_the_c_entries_refuse_negative_strides_of_results_and_d_out():
             o, g, q, k, v = strides
             assert lib.fc_attention_docs_backward(d, 4096, *o, 4096, 4096, *g, 4096, *q, 4096, *k, 4096, *v, None, 4096, 1 << 30, None) == -1
             assert b"negative" in lib.fc_last_error(), lib.fc_last_error()
+
+
+def test_rotary_refuses_rows_beyond_a_launch():
+    import ctypes
+    lib = _lib.load()
+    assert lib.fc_rotary(1, 8192, 16, 16, 4096, 1, 4096, (ctypes.c_int32 * 1)(8), 8, 0, 0, 4096, 16, 16, 1 << 35, 1, 16, None) == -1
+    assert b"rows" in lib.fc_last_error()

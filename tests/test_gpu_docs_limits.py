@@ -167,3 +167,19 @@ def test_small_scores_under_far_caps(dtype, scale, cap):
     d_v = ops.attention_docs_backward(d_out, q, k, v, out, stats, R.offsets(q_len), causal=True, cap=cap, scale=scale)[2]
     bound = R.grad_bounds(ref, q, k, v, d_out, dtype, 40, ds, cap, scale=scale)["d_v"]
     assert ((d_v.double().cpu() - ref["d_v"]).abs() <= bound).all()
+
+
+def test_rotary_of_more_rows_than_a_launch_has_workgroups_of_sixteen():
+    rows, last = (1 << 28) + 5, 37
+    x = torch.zeros(rows, 1, 16, dtype=torch.bfloat16, device=DEV)
+    x[-last:] = _rand(last, 1, 16, seed=41, dtype=torch.bfloat16)
+    x[:last] = _rand(last, 1, 16, seed=42, dtype=torch.bfloat16)
+    ends = torch.cat([x[:last], x[-last:]]).clone()
+    positions = torch.arange(rows, dtype=torch.int32, device=DEV)
+    inv_freq = _rand(8, seed=43).abs()
+    assert ops.rotary(x, positions, inv_freq, out=x) is x
+    want = R.rotary(ends, torch.cat([positions[:last], positions[-last:]]), inv_freq, (8,))
+    got = torch.cat([x[:last], x[-last:]]).double().cpu()
+    # two products and their sum in fp32 with cos and sin good to 2^-22 (2 ulp, and an angle of 2^28 turns from a 64-bit product), rounded once
+    assert ((got - want).abs() <= R.HALF[torch.bfloat16] * want.abs() + 8 * 2.0 ** -22 * ends.double().abs().max().cpu()).all()
+    assert not x[last:-last].any()
