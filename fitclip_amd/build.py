@@ -149,8 +149,9 @@ ASM_DMA_AUDIT = {"gemm_split2.hip": ["gemm_split2_kernel"], "attention_docs.hip"
 
 def audit_asm_dma_hazards(asm_path: Path, substrings) -> int:
     """Raises if an LDS-DMA `buffer_load ... lds` / `global_load_lds` of a kernel whose name contains one of `substrings` reads an SGPR whose latest
-    writer, fewer than 5 wait states upstream (straight-line scan; s_nop N counts N + 1), is a VALU instruction.  Returns the number
-    of DMA instructions checked."""
+    writer, fewer than 5 wait states upstream on any way to it (s_nop N counts N + 1, everything else 1), is a VALU instruction.  A kernel's
+    body goes up to its `.Lfunc_end` label: blocks are laid out behind its first `s_endpgm` too, and are reached by branches.  Returns the
+    number of DMA instructions checked."""
     import re
     text = asm_path.read_text()
     checked = 0
@@ -160,33 +161,64 @@ def audit_asm_dma_hazards(asm_path: Path, substrings) -> int:
         for a, b in re.findall(r"\bs\[(\d+):(\d+)\]", tok):
             out.update(range(int(a), int(b) + 1))
         out.update(int(a) for a in re.findall(r"\bs(\d+)\b", tok))
+        if re.search(r"\bvcc\b", tok):
+            out.update(("vcc_lo", "vcc_hi"))
+        out.update(re.findall(r"\bvcc_(?:lo|hi)\b", tok))
         return out
+
+    def written(code):
+        op, _, rest = code.partition(" ")
+        if re.match(r"s_cmp|s_bitcmp", op):  # (these only read)
+            return set()
+        operands = rest.split(",")
+        two = op.startswith("v_") and ("_co_" in op or "div_scale" in op or "mad_u64" in op or "mad_i64" in op)  # (carry or flag behind the result)
+        return set().union(*(sregs(o) for o in operands[:2 if two else 1]))
 
     for m in re.finditer(r"^(\S+):\s*;\s*@", text, flags=re.M):
         if not any(sub in m.group(1) for sub in substrings):
             continue
-        body = text[m.end():]
-        body = body[:body.find("s_endpgm")]
-        lines = [l.split(";")[0].strip() for l in body.splitlines()]
-        lines = [l for l in lines if l and not l.endswith(":") and not l.startswith(".")]
-        for n, c in enumerate(lines):
+        end = re.search(r"^\.Lfunc_end\d+:", text[m.end():], flags=re.M)
+        if not end:
+            raise RuntimeError(f"{asm_path.name}: {m.group(1)}: no end of the function (audit out of date?)")
+        code, labels, waiting = [], {}, []   # instructions; label -> index of the instruction behind it
+        for line in text[m.end():m.end() + end.start()].splitlines():
+            line = line.split(";")[0].strip()
+            if line.endswith(":"):
+                waiting.append(line[:-1])
+            elif line and not line.startswith("."):
+                labels.update((name, len(code)) for name in waiting)
+                waiting = []
+                code.append(line)
+        before = [[n - 1] if n and not re.match(r"s_branch|s_endpgm|s_setpc|s_trap", code[n - 1]) else [] for n in range(len(code))]
+        for n, c in enumerate(code):
+            if re.match(r"s_setpc|s_swappc|s_cbranch_i|s_cbranch_g", c):
+                raise RuntimeError(f"{asm_path.name}: {m.group(1)}: `{c}`: where it goes is not known (audit out of date?)")
+            target = re.match(r"s_c?branch\S*\s+(\S+)", c)
+            if target and target.group(1) in labels:
+                before[labels[target.group(1)]].append(n)
+            elif target and target.group(1) not in waiting:
+                raise RuntimeError(f"{asm_path.name}: {m.group(1)}: `{c}`: no such label (audit out of date?)")
+        for n, c in enumerate(code):
             if not (c.startswith("buffer_load_dword") and c.endswith(" lds") or c.startswith("global_load_lds_dword")):
                 continue
             checked += 1
-            need, states, k = sregs(c), 0, n - 1
-            while k >= 0 and states < 5 and need:
-                p = lines[k]
-                k -= 1
-                dst = re.match(r"(\S+)\s+(s\[\d+:\d+\]|s\d+)\b", p)
-                if dst:
-                    written = sregs(dst.group(2)) & need
-                    if written:
-                        if p.startswith("v_"):
-                            raise RuntimeError(f"{asm_path.name}: {m.group(1)}: `{p}` writes an SGPR {states} wait state(s) before `{c}` "
-                                               f"reads it inside an asm statement (a VALU-written SGPR needs 5 before a VMEM read)")
-                        need -= written   # an SALU write: interlocked, and it hides older writers
-                nop = re.match(r"s_nop\s+(\d+)", p)
+            ways = [(k, 0, frozenset(sregs(c))) for k in before[n]]
+            seen = set()
+            while ways:
+                way = ways.pop()
+                if way in seen:
+                    continue
+                seen.add(way)
+                k, states, need = way
+                hit = written(code[k]) & need
+                if hit and code[k].startswith("v_"):
+                    raise RuntimeError(f"{asm_path.name}: {m.group(1)}: `{code[k]}` writes an SGPR {states} wait state(s) before `{c}` "
+                                       f"reads it inside an asm statement (a VALU-written SGPR needs 5 before a VMEM read)")
+                need -= hit                  # an SALU write: interlocked, and it hides older writers
+                nop = re.match(r"s_nop\s+(\d+)", code[k])
                 states += int(nop.group(1)) + 1 if nop else 1
+                if states < 5 and need:
+                    ways.extend((b, states, need) for b in before[k])
     if checked == 0:
         raise RuntimeError(f"{asm_path.name}: no LDS-DMA instruction found in {substrings} (audit out of date?)")
     return checked
