@@ -31,7 +31,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
 
-// n / d for 0 <= n < 2^31 by one multiplication: mul = ceil(2^(32 + shift) / d) with 2^shift >= d
+// n / d for 0 <= n < 2^31 by one multiplication: mul = ceil(2^(31 + shift) / d) with 2^shift >= d (below 2^32)
 struct FastDiv {
   unsigned d, mul, shift;
   FastDiv(unsigned div = 1) : d(div), mul(0), shift(0) {

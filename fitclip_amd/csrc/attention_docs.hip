@@ -30,7 +30,7 @@ namespace docs {
 namespace {
 
 // One kernel row again, key by key (64 lanes = 64 keys for the scores, 64 dimensions for the sums), over keys [lo, hi).
-template <typename T, bool CAP, bool BIAS>
+template <typename T, bool CAP, bool BIAS, bool PARTS>
 __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int pos, int split, int lane) {
   const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
   const float q = value_at<T>(a.q + token * a.q_row + qh * a.q_head, lane), slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
@@ -49,7 +49,7 @@ __device__ void row_again(const Args& a, int head, int m, int lo, int hi, int po
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(p, w), value_at<T>(vb + (long)(j + w) * a.v_row, lane), o);
   }
-  if (a.splits > 1) {
+  if (PARTS && a.splits > 1) {
     const long at = ((long)split * a.kv_heads + head) * a.rows + m;
     a.part[at * 64 + lane] = o;
     if (lane == 0) *reinterpret_cast<f32x2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64 + at * 2) = f32x2{top, l};
@@ -76,7 +76,7 @@ attention_docs_kernel(const Args a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // key head fastest (one XCD then works on few heads: K and V stay in its L2), later rows first (causal: they cost most)
   const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int rank = (int)((unsigned)rest / (unsigned)a.splits), split = rest - rank * a.splits;
+  const int rank = KS > 1 ? (int)((unsigned)rest / (unsigned)a.splits) : rest, split = KS > 1 ? rest - rank * a.splits : 0;
   const int tile = RW * KS > 1 && a.by_way ? tile_by_way(a.q_off, a.k_off, a.docs, a.q_rows, (int)a.group.d, 32 * RW, a.tiles, rank, true, lane)
                                           : a.tiles - 1 - rank;
   const int m0 = (tile * RW + (KS > 1 ? 0 : wave)) * 32;
@@ -111,7 +111,7 @@ attention_docs_kernel(const Args a) {
   }
   const int ntile = kend > kbeg ? (kend - kbeg + TK - 1) / TK : 0;
   int t_first = 0, t_last = ntile;
-  if (a.splits > 1) {
+  if (KS > 1 && a.splits > 1) {  // (waves that take turns alone: plan_forward)
     const int part = (int)((unsigned)(ntile + a.splits - 1) / (unsigned)a.splits);
     t_first = min(ntile, split * part);
     t_last = min(ntile, t_first + part);
@@ -252,40 +252,25 @@ attention_docs_kernel(const Args a) {
   l = swap_sum(l);
   float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
   l *= down;
-  float2* const part_ml = reinterpret_cast<float2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64);
   unsigned bad;  // rows to be done again: bit k = row bad0 + k
   int bad0 = 0;
 
   if constexpr (KS == 1) {
     const float probe = swap_sum(not_finite(o));
     const bool again = row.valid && (probe != probe || far_away(mtop));
-    if (a.splits > 1) {
-      const long at = ((long)split * a.kv_heads + head) * a.rows + m0 + r;
-      if (m0 + r < a.rows && !again) {
-        float* po = a.part + at * 64;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<f32x4*>(po + 32 * n + 8 * b + 4 * hh) =
-                f32x4{o[n][4 * b] * down, o[n][4 * b + 1] * down, o[n][4 * b + 2] * down, o[n][4 * b + 3] * down};
-        if (hh == 0) part_ml[at] = float2{mtop, row.valid ? l : -1.f};  // (sum -1: a row of no document)
-      }
-    } else {
-      const float inv = sees && l != 0.f ? down / l : 0.f;
-      const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
-      if (hh == 0 && write) {
-        int m = m0 + r;
-        asm volatile("" : "+v"(m));  // (token and head are formed here again, not kept through the loop)
-        const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
-        *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
-      }
-      __syncthreads();  // (the patches reuse the stages)
-      store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
-        const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
-        return a.out + tk * a.out_row + h * a.out_head;
-      });
+    const float inv = sees && l != 0.f ? down / l : 0.f;
+    const bool write = row.valid ? !again : a.fill && m0 + r < a.rows;
+    if (hh == 0 && write) {
+      int m = m0 + r;
+      asm volatile("" : "+v"(m));  // (token and head are formed here again, not kept through the loop)
+      const int token = a.group.div(m), qh = head * (int)a.group.d + (m - token * (int)a.group.d);
+      *reinterpret_cast<f32x2*>(a.stats + ((long)token * a.kv_heads * (int)a.group.d + qh) * 2) = f32x2{row.valid ? mtop : -kInf, row.valid ? l : 0.f};
     }
+    __syncthreads();  // (the patches reuse the stages)
+    store_rows<T>(smem + wave * 32 * ROWB, o, inv, lane, __ballot(write), [&](int w) {
+      const int mw = m0 + w, tk = a.group.div(mw), h = head * (int)a.group.d + (mw - tk * (int)a.group.d);
+      return a.out + tk * a.out_row + h * a.out_head;
+    });
     bad = (unsigned)__ballot(again);
   } else {
     if (hh == 0) {
@@ -310,6 +295,7 @@ attention_docs_kernel(const Args a) {
     bad = bad_of_eight(y, valid, far_away(top));
     const bool again = bad >> (lane >> 3) & 1, write = mr < a.rows && !again && (valid || a.fill || a.splits > 1);
     if (a.splits > 1) {
+      float2* const part_ml = reinterpret_cast<float2*>(a.part + (long)a.splits * a.kv_heads * a.rows * 64);
       const long at = ((long)split * a.kv_heads + head) * a.rows + mr;
       if (write) {
         store_eight<float>(reinterpret_cast<char*>(a.part + at * 64), y, 1.f, lane);
@@ -326,7 +312,7 @@ attention_docs_kernel(const Args a) {
     const int w = bad0 + __builtin_ctz(bad);
     bad &= bad - 1;
     const int lo = __builtin_amdgcn_readlane(row.lo, w), hi = __builtin_amdgcn_readlane(row.hi, w), pos = __builtin_amdgcn_readlane(row.pos, w);
-    row_again<T, CAP, BIAS>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lane);
+    row_again<T, CAP, BIAS, (KS > 1)>(a, head, m0 + w, max(lo, kbeg + t_first * TK), min(hi, kbeg + t_last * TK), pos, split, lane);
   }
 }
 

@@ -448,7 +448,7 @@ docs_grad_keys_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const int rank = (int)((unsigned)rest / (unsigned)a.splits), split = rest - rank * a.splits;  // (earlier keys first: causal, they cost most)
+  const int rank = KS > 1 ? (int)((unsigned)rest / (unsigned)a.splits) : rest, split = KS > 1 ? rest - rank * a.splits : 0;  // (earlier keys first: causal, they cost most)
   const int tile = KW * KS > 1 && a.by_way ? tile_by_way(a.k_off, a.q_off, a.docs, a.k_rows, 1, 32 * KW, a.tiles, rank, false, lane) : rank;
   const int k0 = tile * KW * 32, kw = k0 + (KS > 1 ? 0 : wave * 32);
 
@@ -494,7 +494,7 @@ docs_grad_keys_kernel(const Args a) {
     for (int i = 0; i < 16; ++i) dk[n][i] = dv[n][i] = 0.f;
   int g = 0, t = KS > 1 ? wave : 0, buf = 0;  // query head of the group, tile of rows
   int left = steps * a.share;                 // tiles of this part of the rows, from here on
-  if (a.splits > 1) {
+  if (KS > 1 && a.splits > 1) {  // (waves that take turns alone: plan_keys)
     const int part = (int)((unsigned)(left + a.splits - 1) / (unsigned)a.splits);
     t += split * part;
     left = min(part, left - split * part);
@@ -608,7 +608,6 @@ docs_grad_keys_kernel(const Args a) {
   const bool owned = key >= a.k_off[0] && key < a.k_off[a.docs];
   unsigned bad = 0;  // keys to be done again: bit k = key kw + bad0 + k
   int bad0 = 0;
-  float* const part = a.part + ((long)split * a.kv_heads + head) * a.k_rows * 128;  // d_k and d_v of a part of the rows, 64 values each
   if constexpr (KS == 1) {
     __syncthreads();  // (the patches reuse the stages)
     const float probe = swap_sum(not_finite(dk) + not_finite(dv));
@@ -627,6 +626,7 @@ docs_grad_keys_kernel(const Args a) {
     __syncthreads();
     sum_waves<KS>(smem, BUFS * STAGE, dv, 1.f, wave, lane, z);
     if (a.splits > 1) {
+      float* const part = a.part + ((long)split * a.kv_heads + head) * a.k_rows * 128;  // d_k and d_v of a part of the rows, 64 values each
       if (in) {
         store_eight<float>(reinterpret_cast<char*>(part + (long)(kw + rr) * 128), y, 1.f, lane);
         store_eight<float>(reinterpret_cast<char*>(part + (long)(kw + rr) * 128 + 64), z, 1.f, lane);

@@ -96,7 +96,6 @@ template <typename T>
 int launch_rotary_t(const RotaryArgs& a, int interleaved, hipStream_t st) {
   int r = 16;
   while (r > 1 && a.rows < 1024L * r) r >>= 1;  // small calls: one row per workgroup reaches more compute units
-  while (r > 1 && a.pairs * r > 4096) r >>= 1;
   while (a.rows / r >= 1L << 24 && a.pairs * r * 16 <= 32 * 1024) r <<= 1;  // (a launch has fewer than 2^32 threads)
   const long blocks = (a.rows + r - 1) / r;
   if (blocks >= 1L << 24) return fail(FC_EINVAL, "fc_rotary: %ld rows", a.rows);
