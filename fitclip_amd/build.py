@@ -41,13 +41,24 @@ NO_SCRATCH_AUDIT = {
 }
 
 
-def source_fingerprint() -> str:
-    """Hash of every kernel / ABI source the library is built from.  Profiling artefacts (profiles/traffic_*.json) are
-    stamped with it, and bench.py refuses a PMC pass that was made with other sources than the ones in the tree."""
+# The kernels that PMC passes are made of (bench.py: `roofline.traffic`)
+MEASURED_SOURCES = ["gemm.hip", "gemm_split2.hip", "gemm_split3.hip"]
+
+
+def source_fingerprint(csrc: Path = CSRC) -> str:
+    """Hash of the sources that the measured kernels are built from: MEASURED_SOURCES and the headers beside them that they include.  Profiling
+    artefacts (profiles/traffic_*.json) are stamped with it, and bench.py refuses a PMC pass that was made with other sources than the ones
+    in the tree; other kernels do not touch it."""
     import hashlib
+    import re
+    found, ahead = set(), [csrc / s for s in MEASURED_SOURCES]
+    while ahead:
+        path = ahead.pop()
+        if path.parent == csrc and path not in found:
+            found.add(path)
+            ahead += [(csrc / name).resolve() for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.M)]
     h = hashlib.sha256()
-    for path in sorted([*(CSRC / s for s in SOURCES), *CSRC.glob("*.h"), *CSRC.glob("*.inc"),
-                        *(REPO / "include").glob("*.h")]):
+    for path in sorted(found):
         h.update(path.name.encode())
         h.update(path.read_bytes())
     return h.hexdigest()[:16]

@@ -10,11 +10,12 @@
 # Raw output goes to gpurun_out/prof_*; summaries to profiles/ AND gpurun_out/profiles_<tag>/ (the latter travels back).
 # The program stays directly after `--` (no env / bash -c hop: the profiler has already initialised the GPU).
 set -e
-tag=${1:-r04}
+tag=${1-r04}        # ('': the files of the tree as it is, traffic_<precision>.json and bench_<precision>_*)
+pre=${tag:+${tag}_}
 prec=${2:-fp32}
 repo=$(pwd)
 out=$repo/gpurun_out
-keep=$out/profiles_${tag}
+keep=$out/profiles_${tag:-now}
 mkdir -p "$out" "$keep"
 cd /tmp && export TMPDIR=/tmp
 # The profiled runs keep the two towers on ONE stream (FITCLIP_OVERLAP_TEXT=0): with the default two-stream forward the
@@ -85,17 +86,17 @@ echo "write pass done"
 rocprofv3 --pmc SQ_WAVE_CYCLES SQ_VALU_MFMA_BUSY_CYCLES SQ_ACTIVE_INST_ANY SQ_WAIT_INST_ANY SQ_LDS_BANK_CONFLICT GRBM_GUI_ACTIVE --kernel-trace --output-format csv -d "$out/prof_sq_$prec" -o bench -- python3 "$repo/bench.py" --steps $([ "$prec" = c3 ] && echo 1 || echo 2) --warmup 1 --no-plant $common $pmc_extra > /dev/null 2> "$out/prof_sq_$prec.err" || echo "SQ pass failed (counters may need separate passes)"
 echo "sq pass done"
 cd "$repo"
-find "$out/prof_trace_$prec" -name "*kernel_stats.csv" -exec cp {} "$keep/${tag}_bench_${prec}_kernel_stats.csv" \;
+find "$out/prof_trace_$prec" -name "*kernel_stats.csv" -exec cp {} "$keep/${pre}bench_${prec}_kernel_stats.csv" \;
 trace=$(find "$out/prof_trace_$prec" -name "*kernel_trace.csv" | head -1)
 if [ "$prec" != fp32x6 ] && [ "$prec" != fp32x3 ]; then  # (the split legs share their trace with the fp32 leg: only the kernel table is kept)
-  python3 tools/trace_summary.py "$trace" $chunk $([ "$prec" = c3 ] && echo fp32 || echo $prec) > "$keep/${tag}_bench_${prec}_trace_summary.txt"
+  python3 tools/trace_summary.py "$trace" $chunk $([ "$prec" = c3 ] && echo fp32 || echo $prec) > "$keep/${pre}bench_${prec}_trace_summary.txt"
 fi
-cp "$out/prof_trace_$prec.json" "$keep/${tag}_bench_${prec}_under_rocprof.json"
+cp "$out/prof_trace_$prec.json" "$keep/${pre}bench_${prec}_under_rocprof.json"
 f=$(find "$out/prof_fetch_$prec" -name "*counter_collection.csv" | head -1)
 w=$(find "$out/prof_write_$prec" -name "*counter_collection.csv" | head -1)
 q=$(find "$out/prof_sq_$prec" -name "*counter_collection.csv" | head -1)
 python3 tools/pmc_traffic.py --fetch "$f" --write "$w" ${q:+--sq "$q"} --spec "$spec_fc" --spec "$spec_proj" \
-  --precision $([ "$prec" = c3 ] && echo fp32 || echo $prec) --out "$keep/traffic_${tag}_$([ "$prec" = c3 ] && echo fp32_c3 || echo $prec).json"
+  --precision $([ "$prec" = c3 ] && echo fp32 || echo $prec) --out "$keep/traffic_${pre}$([ "$prec" = c3 ] && echo fp32_c3 || echo $prec).json"
 cp "$keep"/* profiles/
 # the raw traces are large: keep only the summaries for the trip back
 rm -rf "$out/prof_trace_$prec" "$out/prof_fetch_$prec" "$out/prof_write_$prec" "$out/prof_sq_$prec"
