@@ -38,7 +38,7 @@ The same JSON line carries
     timed one ("instrumented_repeat_ms_per_step");
     achieved = algorithmic FLOPs per launch / that duration; peak = dense MFMA peak of the dtype (MI355X_MICROARCH.md);
     traffic = HBM bytes per launch from the PMC passes of tools/profile_round.sh, accepted only if the pass was made
-    with the SAME kernel sources (fingerprint of fitclip_amd/csrc + include), else null.
+    with the SAME GEMM sources (build.source_fingerprint), else null.
   * after the timed region, untimed: one fully instrumented step ("time_split", "roofline_all_gemms", and the check of
     which kernel dominates) and K passes of the visual tower alone ("roofline_vit_forward").
   * "retrieval": the towers are random, so `visual.proj`, `visual.ln_post.bias` and `text_projection` are PLANTED before
