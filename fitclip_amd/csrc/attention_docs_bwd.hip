@@ -15,18 +15,21 @@
 // bf16: `out` comes rounded, and D = dO.out with it; P and dS are rounded in front of their products (once each: at most 2^-8 of a term, where the
 // result's own rounding is as much).  D's error matters where few keys have all the weight and no sum over keys evens it out: a kernel in front
 // forms D, and a workgroup of it with such a row (a sum of weights below 8 times the largest: the first rows of a causal document, steep
-// slopes) walks over its keys for D = sum P dP, two products of the three in rows; the others are done at once.  (dS in two parts, an operand
+// slopes) walks over its keys for D = sum P dP, two products of the three in rows; the others are done at once, and a D of theirs is off by what
+// the rounding of `out` makes of dO.out: 2^-8 of |dO||out| at most, which is large beside dP - D where the values of a row's keys are nearly alike.  (dS in two parts, an operand
 // for what its rounding left, would take d_q from 1.4 times its own rounding's error to 1.0, for a third more time in rows: not kept.)
 // Both have the forward's three shapes (attention_docs.h, shape_for).  The scores and dP are formed twice, 7 products where 5 would do: one
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
 //
 // What bounds them, and what they reach (10 x 64 operations per pair and head that see each other, for both kernels):
-//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1928
-//     us = 713 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 16 + 114 us, keys 198 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
-//     29 + 101 and 166, 84 % of the latter without bringing any tiles.
-//   fp32: the matrix instructions; 4 x 8192 tokens 14.2 ms = 97 TFLOP/s, 136 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
-//     rows 47 us, keys 63 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
-//     2: rows 105, keys 135.
+//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1980
+//     us = 694 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 17 + 118 us, keys 203 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
+//     31 + 103 and 170, 84 % of the latter without bringing any tiles.  The kernel in front that forms D (17 and 31 us) is not paid for by the rows
+//     that walk (matrix instructions in less than 1 % of its cycles): all four waves of a workgroup load Q, dO and out, search the documents and
+//     form the same 32 numbers.
+//   fp32: the matrix instructions; 4 x 8192 tokens 14.3 ms = 96 TFLOP/s, 135 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
+//     rows 47 us, keys 62 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
+//     2: rows 107, keys 132.
 #include "attention_docs.h"
 
 #include <algorithm>

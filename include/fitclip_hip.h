@@ -204,7 +204,7 @@ FC_API int fc_rotary(int32_t kind, const void* x, int64_t x_row, int64_t x_head,
  * - slopes[head] |p - j| if slopes (dev f32 [q_heads]) is given.  A query sees all keys of its document or, if causal, those up to p and
  * the first prefix[d] ones (dev int32 [docs], may be null).  Query heads h g .. h g + g - 1, g = q_heads / kv_heads, share key head h.
  * A head is 64 contiguous values; every row and head, of results too, starts on a 16-byte boundary; strides are in elements and not
- * negative, rows of q, k, v and d_out less than 32 MiB apart. */
+ * negative, rows of q, k, v and d_out less than 32 MiB apart.  A cap above 2^127 times the scale is none. */
 typedef struct {
   int32_t struct_size; /* sizeof(fc_docs) as the caller declared it: checked first */
   int32_t kind;        /* fc_precision of q, k, v, out and the gradients */
@@ -223,13 +223,19 @@ typedef struct {
  * score in units of ln 2 and the sum of 2^(score - largest) (-inf, 0 in rows of 0): what the gradients and a later
  * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
  * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
- * infinities included.  out may be q (with q's strides) and must not overlap it otherwise, nor k or v.  Sums in fp32; bf16: the weights are rounded to bf16 in front of the product with v. */
+ * infinities included.  out may be q (with q's strides) and must not overlap it otherwise, nor k or v.  Sums in fp32; bf16: the weights are
+ * rounded to bf16 in front of the product with v.  Rows whose largest score is beyond 2^24 (bf16: 2^17) in units of ln 2, or that met a NaN or an
+ * infinity behind a mask, are formed once
+ * more key by key, in the gradients too: as right, and far slower. */
 FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
                       size_t scratch_bytes, fc_stream stream);
 /* Gradients of fc_attention_docs from the gradient d_out of its result: d_q, d_k, d_v of q, k, v (same element kind) and, if d_slopes
  * is given, of the slopes (dev f32 [q_heads]).  out and stats are the forward's.  Gradients of shared key heads are summed over their
- * query heads; every sum has a fixed order (no atomics).  The gradients must not overlap operands or each other.  scratch: fc_attention_docs_backward_scratch_bytes. */
+ * query heads; every sum has a fixed order (no atomics).  The gradients must not overlap operands or each other.  Sums in fp32; bf16: the
+ * weights and dS = weight (d_out.v - D) are rounded to bf16 in front of their products, and D is d_out.out with `out` as it comes, rounded,
+ * except where the weights of a row (of 32 or 128 that are formed together) add up to less than 8 times the largest: there D is formed from
+ * the weights.  d_slopes: every factor in fp32.  scratch: fc_attention_docs_backward_scratch_bytes. */
 FC_API size_t fc_attention_docs_backward_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs_backward(const fc_docs* d, const void* out, int64_t out_row, int64_t out_head, const float* stats,
                                const void* d_out, int64_t do_row, int64_t do_head, void* d_q, int64_t dq_row, int64_t dq_head,
