@@ -42,10 +42,11 @@ struct FastDiv {
 };
 
 // A weight is 2^(fma(raw score, c, -maximum)): the product keeps all its bits, the maximum is rounded to 24, and where it is large the largest weight
-// is no longer 1.  The forward's sum makes up for that (both gradients divide by it) as long as neither leaves fp32, which it can from 2^30 on; in
-// bf16 the gradients add the sum's logarithm to the maximum, which is off by half a bf16 step from 2^17 on.  Rows with a maximum as far away as
-// this are done again key by key, from rounded scores whose largest less the maximum is 0.
-template <typename T> constexpr float kFar = sizeof(T) == 4 ? 16777216.f : 131072.f;
+// is no longer 1 but 2^(up to 2^-25 of it).  The sum makes up for that as long as neither leaves fp32, which it can from 2^30 on: such rows are
+// done again key by key, from rounded scores whose largest less the maximum is 0.  The gradients do so from 2^17 on: bf16 adds the sum's
+// logarithm to the maximum, which is off by half a bf16 step there, and a key that is done again for one of its rows' sake forms its other rows'
+// scores in another order than their maxima were, whose rounding is a few 2^-24 of them.
+constexpr float kFar = 1073741824.f, kFarGrad = 131072.f;
 
 struct Args {
   const char *q, *k, *v;                                // strides in bytes

@@ -248,7 +248,7 @@ attention_docs_kernel(const Args a) {
 #pragma unroll
     for (int u = 0; u < NT; ++u) cols_dot(vf[u], s[u], o);
   }
-  const auto far_away = [](float x) { return x != -kInf && fabsf(x) >= kFar<T>; };
+  const auto far_away = [](float x) { return x != -kInf && fabsf(x) >= kFar; };
   l = swap_sum(l);
   float down = mref == mtop ? 1.f : __builtin_amdgcn_exp2f(mref - mtop);  // to the true maximum
   l *= down;

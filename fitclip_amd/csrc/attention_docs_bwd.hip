@@ -40,8 +40,9 @@ namespace docs {
 namespace {
 
 // Row table in scratch, one array of rows_pad numbers per quantity and query head: what a row needs to have its weights formed again
-enum Column : int { COL_MAX = 0, COL_D = 1, COL_LO = 2, COL_HI = 3, COL_INV = 4, COL_POS = 5, COL_DSLOPE = 6, COLS = 7 };
-// (maximum; bf16: maximum + log2 sum, and no COL_INV; fp32: 1 / sum apart, so that the forward's P is formed exactly again)
+enum Column : int { COL_MAX = 0, COL_D = 1, COL_LO = 2, COL_HI = 3, COL_INV = 4, COL_POS = 5, COL_DSLOPE = 6, COL_TOP = 7, COLS = 8 };
+// (maximum; bf16: maximum + log2 sum, and no COL_INV; fp32: 1 / sum apart, so that the forward's P is formed exactly again; NaN in rows beyond
+// kFarGrad, which have COL_TOP and COL_INV of their own)
 // and behind the columns four ints per 32 rows: lowest and highest key that one of them sees; the keys from .. to that ALL of them see
 __device__ __forceinline__ float* column(const Args& a, int c, int qh) { return a.table + ((long)c * a.kv_heads * a.share + qh) * a.rows_pad; }
 __device__ __forceinline__ int32_t* block_keys(const Args& a, int block) {
@@ -75,42 +76,49 @@ __device__ __forceinline__ float bent_by(const Args& a, float raw, float ds) {
   return ds;
 }
 
-// d_q of one row again, key by key (see attention_docs.h), with D from the same weights: where one key has all the weight, dP - D is exactly 0
+// d_q of one row again, key by key (see attention_docs.h), with its maximum, its sum and D from the same scores: where one key has all the weight, dP - D is exactly 0
 template <typename T, bool CAP, bool BIAS>
 __device__ void row_grad_again(const Args& a, int qh, int m, int lo, int hi, int pos, int lane) {
   const int head = qh / a.share;
-  const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * a.kv_heads * a.share + qh) * 2);
-  const float top = st[0], inv = 1.f / st[1];
   const float q = value_at<T>(a.q + m * a.q_row + qh * a.q_head, lane), go = value_at<T>(a.d_out + m * a.do_row + qh * a.do_head, lane);
   const float slope = BIAS ? a.slopes[qh] * kLog2e : 0.f;
   const char *kb = a.k + head * a.k_head, *vb = a.v + head * a.v_head;
-  float o = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f, raw, far, p, g;
-  const auto weigh = [&](int j) {
+  float o = 0.f, top = -kInf, l = 0.f, pd = 0.f, pf = 0.f, pdf = 0.f, raw, far, x, g;
+  const auto look = [&](int j) {
     const int key = min(j + lane, hi - 1);
     raw = row_dot<T>(kb + key * a.k_row, q), far = fabsf((float)(pos - key));
-    p = j + lane < hi ? __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - top) * inv : 0.f;
+    x = j + lane < hi ? score<CAP, BIAS>(a, raw, slope, far) : -kInf;
     g = row_dot<T>(vb + key * a.v_row, go);
   };
 #pragma unroll 1
   for (int j = lo; j < hi; j += 64) {
-    weigh(j);
-    pd = __builtin_fmaf(p, g, pd);
-    pf = __builtin_fmaf(p, far, pf);
-    pdf = __builtin_fmaf(p * g, far, pdf);
+    look(j);
+    const float mx = fmaxf(top, wave_max(x)), ref = mx == -kInf ? 0.f : mx;
+    const float p = __builtin_amdgcn_exp2f(x - ref), alpha = top == mx ? 1.f : __builtin_amdgcn_exp2f(top - ref);
+    top = mx;
+    l = __builtin_fmaf(l, alpha, p);
+    pd = __builtin_fmaf(p, g, pd * alpha);
+    pf = __builtin_fmaf(p, far, pf * alpha);
+    pdf = __builtin_fmaf(p * g, far, pdf * alpha);
   }
-  const float D = wave_sum(pd);
-  if (lane == 0) column(a, COL_D, qh)[m] = D;
+  l = wave_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l, D = wave_sum(pd) * inv;
+  if (lane == 0) {
+    const float was = a.stats[((long)m * a.kv_heads * a.share + qh) * 2];
+    if (fabsf(was) >= kFarGrad) column(a, COL_TOP, qh)[m] = top, column(a, COL_INV, qh)[m] = inv;
+    column(a, COL_D, qh)[m] = D;
+  }
 #pragma unroll 1
   for (int j = lo; j < hi; j += 64) {
-    weigh(j);
-    const float ds = bent_by<CAP>(a, raw, p * (g - D));
+    look(j);
+    const float ds = bent_by<CAP>(a, raw, __builtin_amdgcn_exp2f(x - top) * inv * (g - D));
 #pragma unroll 1
     for (int w = 0; w < min(64, hi - j); ++w) o = __builtin_fmaf(lane_value(ds, w), value_at<T>(kb + (long)(j + w) * a.k_row, lane), o);
   }
   put_at<T>(a.dq + m * a.dq_row + qh * a.dq_head, lane, hi - lo > 1 ? o * a.scale : 0.f);
   if constexpr (BIAS) {
-    pf = wave_sum(pf);
-    pdf = wave_sum(pdf);
+    pf = wave_sum(pf) * inv;
+    pdf = wave_sum(pdf) * inv;
     if (lane == 0) column(a, COL_DSLOPE, qh)[m] = hi - lo > 1 ? D * pf - pdf : 0.f;
   }
 }
@@ -155,7 +163,9 @@ __device__ void key_grad_again(const Args& a, int head, int key, int r_lo, int r
       const float raw = row_dot<T>(qb + m * a.q_row, k), g = row_dot<T>(db + m * a.do_row, v);
       const float far = BIAS ? fabsf((float)(__float_as_int(column(a, COL_POS, qh)[m]) - key)) : 0.f;
       const f32x2 st = *reinterpret_cast<const f32x2*>(a.stats + ((long)m * a.kv_heads * a.share + qh) * 2);
-      const float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - st[0]) * (1.f / st[1]);
+      const bool own = fabsf(st[0]) >= kFarGrad;  // (found by row_grad_again)
+      const float top = own ? column(a, COL_TOP, qh)[m] : st[0], inv = own ? column(a, COL_INV, qh)[m] : 1.f / st[1];
+      const float p = __builtin_amdgcn_exp2f(score<CAP, BIAS>(a, raw, slope, far) - top) * inv;
       const float ds = hi - lo == 1 ? 0.f : bent_by<CAP>(a, raw, p * (g - column(a, COL_D, qh)[m]));
 #pragma unroll 1
       for (int w = 0; w < 64; ++w) {
@@ -230,7 +240,7 @@ docs_grad_rows_kernel(const Args a) {
     if (sees) top += __builtin_amdgcn_logf(st[1]);
     inv = 1.f;
   }
-  if (sees && fabsf(st[0]) >= kFar<T>) top = __builtin_nanf("");  // (done again, by this kernel and for the keys that the row sees)
+  if (sees && fabsf(st[0]) >= kFarGrad) top = __builtin_nanf("");  // (done again, by this kernel and for the keys that the row sees)
   if (!sees) D = 0.f;
   if constexpr (FOR_D) {
     if (!peaked) {  // (uniform over the workgroup)

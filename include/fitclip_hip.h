@@ -224,9 +224,8 @@ typedef struct {
  * merge of several results need; ln 2 (stats[0] + log2 stats[1]) is the row's log-sum-exp.  scratch:
  * fc_attention_docs_scratch_bytes (0 unless few rows meet many keys).  Values of keys that a row does not see never reach it, NaN and
  * infinities included.  out may be q (with q's strides) and must not overlap it otherwise, nor k or v.  Sums in fp32; bf16: the weights are
- * rounded to bf16 in front of the product with v.  Rows whose largest score is beyond 2^24 (bf16: 2^17) in units of ln 2, or that met a NaN or an
- * infinity behind a mask, are formed once
- * more key by key, in the gradients too: as right, and far slower. */
+ * rounded to bf16 in front of the product with v.  Rows whose largest score is beyond 2^30 (in the
+ * gradients 2^17) in units of ln 2, or that met a NaN or an infinity behind a mask, are formed once more key by key: as right, and far slower. */
 FC_API size_t fc_attention_docs_scratch_bytes(const fc_docs* d);
 FC_API int fc_attention_docs(const fc_docs* d, void* out, int64_t out_row, int64_t out_head, float* stats, void* scratch,
                       size_t scratch_bytes, fc_stream stream);

@@ -85,7 +85,13 @@ def test_scores_so_large_that_one_key_has_all_the_weight(dtype, shape, scale, si
     assert plain.float().mean() > 0.9  # (a check of the inputs)
     at = chosen[..., None].expand(-1, -1, 64)
     picked = v.cpu().gather(0, at)
-    assert torch.equal(out.cpu()[plain], picked[plain])
+    # beyond 2^30 formed again, with a weight of 1: exact.  Below, the weight is 2^x, x up to 2^-25 of the score, over a sum of the same: fp32 a
+    # reciprocal's and a product's rounding, bf16 the weight's in front of the product (1 needs none, 2^x does; the sum keeps it in fp32: 2^-8 of the
+    # result) and the result's own (2^-8 of itself)
+    again = plain & (stats[..., 0].abs() >= 2.0 ** 30).cpu()
+    assert torch.equal(out.cpu()[again], picked[again])
+    loose = 4 * 2.0 ** -24 if dtype == torch.float32 else 2 * 2.0 ** -8 + 2.0 ** -16
+    assert ((out.cpu().double() - picked.double()).abs() <= loose * picked.double().abs())[plain].all()
     assert not d_q.cpu()[plain].any()
     d_out64 = d_out.cpu().double()
     want_v.scatter_add_(0, at, d_out64)
@@ -126,6 +132,33 @@ def test_weights_of_large_scores_add_up_to_one(dtype, shape):
             bound = R.HALF[dtype] * (d_v[b:b + m].double().abs().sum(0) + terms) + ((2.0 ** -7 if dtype == torch.bfloat16 else 0) + (n + m + 256) * 2.0 ** -24) * terms
             assert ((got - want).abs() <= bound).all(), (large, float(((got - want).abs() / bound).max()))
             a, b = a + n, b + m
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("far", [2.0 ** 8, 2.0 ** 14, 2.0 ** 18])
+def test_weights_of_near_and_far_rows_over_the_same_keys(dtype, shape, far):
+    """Every third row's scores are 2^12 or so, the others' 2^20 to 2^30: near rows, formed with far ones' keys, keep weights that add up to 1, so that a
+    document's d_v adds up to its d_out."""
+    q_len, k_len, heads = SHAPES[shape]
+    rows, keys = sum(q_len), sum(k_len or q_len)
+    off = (R.offsets(q_len), None if k_len is None else R.offsets(k_len))
+    q, k = _rand(rows, heads, 64, seed=25, dtype=dtype), _rand(keys, heads, 64, seed=26, dtype=dtype)
+    q[..., :8], k[..., :8] = 2.0 ** 6, 2.0 ** 6
+    q[torch.arange(rows, device=DEV) % 3 != 0] *= far
+    v, d_out = _rand(keys, heads, 64, seed=27, dtype=dtype), _rand(rows, heads, 64, seed=28, dtype=dtype)
+    out, stats = ops.attention_docs(q, k, v, *off)
+    d_q, d_k, d_v = ops.attention_docs_backward(d_out, q, k, v, out, stats, *off)
+    assert all(torch.isfinite(t).all() for t in (out, d_q, d_k, d_v))
+    a = b = 0
+    for n, m in zip(q_len, k_len or q_len):
+        got, want = d_v[b:b + m].double().sum(0), d_out[a:a + n].double().sum(0)
+        terms = d_out[a:a + n].double().abs().sum(0)
+        # d_v's and the weights' rounding, sums of n and m terms; a near row's scores (2^12, of terms of 2^15 and some 2^9 in all) in two orders of 64
+        # products: each is off by 64 half steps of 2^15 x 2^-24 / 8 at most, in the exponent
+        bound = R.HALF[dtype] * (d_v[b:b + m].double().abs().sum(0) + terms) + (2 * 64 * 2.0 ** -12 + (n + m + 256) * 2.0 ** -24) * terms
+        assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+        a, b = a + n, b + m
 
 
 @pytest.mark.parametrize("dtype", TYPES)
