@@ -51,6 +51,7 @@ def source_fingerprint(csrc: Path = CSRC) -> str:
     in the tree; other kernels do not touch it."""
     import hashlib
     import re
+    csrc = csrc.resolve()
     found, ahead = set(), [csrc / s for s in MEASURED_SOURCES]
     while ahead:
         path = ahead.pop()

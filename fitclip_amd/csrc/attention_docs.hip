@@ -14,11 +14,11 @@
 //
 // What bounds it, and what it reaches (4 x 64 operations per pair and head that see each other):
 //   bf16, long ways: vector and matrix instructions, whose times add up for a wave (32 x 32 scores are 8 matrix instructions of 32 cycles and 90
-//     vector ones of 4, 16 of them exponentials of 16): 4 x 8192 tokens, 8 heads 601 us = 914 TFLOP/s; a large product reaches 1127.  With
-//     3 x 3136 tokens, 12 heads, 888 workgroups for room for 768: 120 us = 752 TFLOP/s (127 us in a burst of 20 calls).
-//   fp32: the matrix instructions (16 times as long as bf16's for a product); 4 x 8192 tokens 4189 us = 131 TFLOP/s of 153, one document of 3136
-//     tokens (98 x 12 workgroups of 32 rows) 273 us = 111.
-//   short documents: 512 captions of 4 to 77 tokens, 8 heads, bf16, 20 us = 4.4 TB/s; a large copy reaches 5.1.
+//     vector ones of 4, 16 of them exponentials of 16): 4 x 8192 tokens, 8 heads 604 us = 910 TFLOP/s; a large product reaches 1137.  With
+//     3 x 3136 tokens, 12 heads, 888 workgroups for room for 768: 120 us = 755 TFLOP/s (127 us in a burst of 20 calls).
+//   fp32: the matrix instructions (16 times as long as bf16's for a product); 4 x 8192 tokens 4160 us = 132 TFLOP/s of 153, one document of 3136
+//     tokens (98 x 12 workgroups of 32 rows) 272 us = 111.
+//   short documents: 512 captions of 4 to 77 tokens, 8 heads, bf16, 21 us = 4.1 TB/s; a large copy reaches 5.5.
 //   single tokens: 24 over 300 to 12000 keys, 12 heads over 4, bf16, 25 + 4 us = 4.7 TB/s in the first kernel; fp32 66 + 4 us = 3.6 TB/s.
 #include "attention_docs.h"
 

@@ -22,14 +22,14 @@
 // kernel for all would have to add dQ up over workgroups in memory, with atomics (no fixed order) or with a copy per part.
 //
 // What bounds them, and what they reach (10 x 64 operations per pair and head that see each other, for both kernels):
-//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1980
-//     us = 694 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 17 + 118 us, keys 203 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
-//     31 + 103 and 170, 84 % of the latter without bringing any tiles.  The kernel in front that forms D (17 and 31 us) is not paid for by the rows
+//   bf16: vector and matrix instructions of two waves per SIMD (registers: 195 to 213 where the keys are held); 4 x 8192 tokens, 8 heads 1989
+//     us = 691 TFLOP/s, one causal document of 7777 tokens, 8 heads over 2: rows 17 + 119 us, keys 204 us; 6 clips of 784 to 1568 tokens, 12 heads, a cap:
+//     30 + 103 and 170, 84 % of the latter without bringing any tiles.  The kernel in front that forms D (17 and 30 us) is not paid for by the rows
 //     that walk (matrix instructions in less than 1 % of its cycles): all four waves of a workgroup load Q, dO and out, search the documents and
 //     form the same 32 numbers.
-//   fp32: the matrix instructions; 4 x 8192 tokens 14.3 ms = 96 TFLOP/s, 135 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
+//   fp32: the matrix instructions; 4 x 8192 tokens 14.2 ms = 97 TFLOP/s, 135 of the seven products' own; 256 captions of 4 to 77 tokens, 8 heads:
 //     rows 47 us, keys 62 us - there 32 x 32 tiles hold three times the pairs that the masks leave.  9 documents of 61 to 900, a bias, 8 heads over
-//     2: rows 107, keys 132.
+//     2: rows 106, keys 135.
 #include "attention_docs.h"
 
 #include <algorithm>

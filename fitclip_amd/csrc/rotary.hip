@@ -9,8 +9,8 @@
 //     16-byte accesses: at 24 heads one angle serves 48 values.
 //   * Angles are reduced in TURNS from a 64-bit product: position * inv_freq / (2 pi) minus its nearest integer is exact to 2^-29 turns at
 //     position 2^24 (a 32-bit product is off by a whole radian there), and what is left goes through sincospif in 32 bits.
-//   * Measured: 100352 rows x 24 heads bf16 126 us (4.9 TB/s; a large copy reaches 5.1), 36260 rows fp32 interleaved 96 us (4.6 TB/s), one
-//     frame of 196 rows 2.9 us.
+//   * Measured: 100352 rows x 24 heads bf16 117 us (5.3 TB/s; a large copy reaches 5.5), 36260 rows fp32 interleaved 90 us (5.0 TB/s), one
+//     frame of 196 rows 2.7 us.
 #include "common.h"
 
 namespace fc {
